@@ -26,8 +26,9 @@ LIB_CC1D = os.path.join(PKG, "libcc1d.so")
 LIB_TORCH = os.path.join(PKG, "_cc1d_torch.so")
 
 CU_SOURCES = ["cc1d_api.cu", "cc1d_fwd.cu", "cc1d_bwd.cu", "cc1d_update.cu", "cc1d_varlen.cu",
-              "cc1d_prefill.cu", "cc1d_peer.cu"]
+              "cc1d_prefill.cu", "cc1d_peer.cu", "cc1d_gdr_api.cu", "cc1d_gdr_update.cu"]
 CU_HEADERS = ["cc1d_common.cuh", "cc1d_kernels.h", "cc1d_tma.cuh", os.path.join(INCLUDE, "cc1d.h")]
+GDR_HEADERS = ["cc1d_gdr.cuh", os.path.join(INCLUDE, "cc1d_gdr.h")]     # read by the cc1d_gdr_*.cu only
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -74,15 +75,17 @@ def _run(cmd, log_name):
 def build_kernels(force: bool = False, verbose: bool = False) -> str:
     """nvcc: csrc/*.cu -> libcc1d.so (sm_100a)."""
     hdrs = [h if os.path.isabs(h) else os.path.join(CSRC, h) for h in CU_HEADERS]
+    gdr_hdrs = [h if os.path.isabs(h) else os.path.join(CSRC, h) for h in GDR_HEADERS]
     srcs = [os.path.join(CSRC, s) for s in CU_SOURCES]
-    if not (force or _newer(srcs + hdrs + [__file__], LIB_CC1D)):
+    if not (force or _newer(srcs + hdrs + gdr_hdrs + [__file__], LIB_CC1D)):
         return LIB_CC1D
     os.makedirs(OBJ, exist_ok=True)
     nvcc = _nvcc()
 
     def compile_one(src):
         obj = os.path.join(OBJ, os.path.basename(src) + ".o")
-        if force or _newer([src] + hdrs + [__file__], obj):
+        needs = hdrs + (gdr_hdrs if os.path.basename(src).startswith("cc1d_gdr") else [])
+        if force or _newer([src] + needs + [__file__], obj):
             out = _run([nvcc, *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", src, "-o", obj],
                        os.path.basename(src) + ".log")
             if verbose:
@@ -98,7 +101,8 @@ def build_kernels(force: bool = False, verbose: bool = False) -> str:
 def build_torch_ext(force: bool = False) -> str:
     """g++: csrc/causal_conv1d.cpp -> _cc1d_torch.so (pybind11 module linking libcc1d.so)."""
     src = os.path.join(CSRC, "causal_conv1d.cpp")
-    if not (force or _newer([src, os.path.join(INCLUDE, "cc1d.h"), LIB_CC1D, __file__], LIB_TORCH)):
+    hdrs = [os.path.join(INCLUDE, h) for h in ("cc1d.h", "cc1d_gdr.h")]
+    if not (force or _newer([src, *hdrs, LIB_CC1D, __file__], LIB_TORCH)):
         return LIB_TORCH
     import sysconfig
 

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "cc1d.h"
+#include "cc1d_gdr.h"
 
 namespace {
 
@@ -409,7 +410,85 @@ void peer_allreduce(at::Tensor &buf, const std::vector<int64_t> &peer_ptrs, int6
     raise_on(cc1d_peer_allreduce(&p, at::cuda::getCurrentCUDAStream().stream()), "peer_allreduce");
 }
 
+// ---- gated delta rule ----------------------------------------------------------------------
+namespace {
+
+struct GdrDims {
+    int64_t batch, seqlen, heads_k, heads_v, dim_k, dim_v;
+};
+
+// q, k (batch, seqlen, heads_k, dim_k), v (batch, seqlen, heads_v, dim_v), g, beta (batch, seqlen, heads_v)
+GdrDims gdr_inputs(cc1d_gdr_params &p, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
+                   const at::Tensor &beta, double scale) {
+    need_cuda(q, "q"); need_cuda(k, "k"); need_cuda(v, "v"); need_cuda(g, "g"); need_cuda(beta, "beta");
+    TORCH_CHECK(q.dim() == 4 && v.dim() == 4, "expected q, k (batch, seqlen, heads_k, dim_k) and v (batch, seqlen, heads_v, dim_v)");
+    const GdrDims d{q.size(0), q.size(1), q.size(2), v.size(2), q.size(3), v.size(3)};
+    need_shape(k, {d.batch, d.seqlen, d.heads_k, d.dim_k}, "k");
+    need_shape(v, {d.batch, d.seqlen, d.heads_v, d.dim_v}, "v");
+    need_shape(g, {d.batch, d.seqlen, d.heads_v}, "g");
+    need_shape(beta, {d.batch, d.seqlen, d.heads_v}, "beta");
+    TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
+    for (const at::Tensor *t : {&k, &v, &g, &beta}) TORCH_CHECK(t->device() == q.device(), "q, k, v, g and beta must be on one device");
+    TORCH_CHECK(q.stride(3) == 1 && k.stride(3) == 1 && v.stride(3) == 1, "q, k and v must be contiguous along their last dimension");
+    p.itype = dtype_code(q, "q"); p.gtype = dtype_code(g, "g"); p.btype = dtype_code(beta, "beta");
+    p.scale = (float)scale;
+    p.batch = d.batch; p.seqlen = d.seqlen; p.heads_k = d.heads_k; p.heads_v = d.heads_v; p.dim_k = d.dim_k; p.dim_v = d.dim_v;
+    p.q = q.data_ptr(); p.q_batch_stride = q.stride(0); p.q_l_stride = q.stride(1); p.q_h_stride = q.stride(2);
+    p.k = k.data_ptr(); p.k_batch_stride = k.stride(0); p.k_l_stride = k.stride(1); p.k_h_stride = k.stride(2);
+    p.v = v.data_ptr(); p.v_batch_stride = v.stride(0); p.v_l_stride = v.stride(1); p.v_h_stride = v.stride(2);
+    p.g = g.data_ptr(); p.g_batch_stride = g.stride(0); p.g_l_stride = g.stride(1); p.g_h_stride = g.stride(2);
+    p.beta = beta.data_ptr(); p.beta_batch_stride = beta.stride(0); p.beta_l_stride = beta.stride(1); p.beta_h_stride = beta.stride(2);
+    return d;
+}
+
+void gdr_out(cc1d_gdr_params &p, const GdrDims &d, const at::Tensor &q, at::Tensor &out) {
+    need_cuda(out, "out");
+    need_shape(out, {d.batch, d.seqlen, d.heads_v, d.dim_v}, "out");
+    TORCH_CHECK(out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(3) == 1, "out must have the dtype and device of q and be contiguous along its last dimension");
+    p.out = out.data_ptr(); p.out_batch_stride = out.stride(0); p.out_l_stride = out.stride(1); p.out_h_stride = out.stride(2);
+}
+
+// (rows, heads_v, dim_k, dim_v) fp32 state tensor, a row's last two dimensions dense
+void gdr_state(const at::Tensor &t, const GdrDims &d, const at::Tensor &q, const char *what) {
+    need_cuda(t, what);
+    TORCH_CHECK(t.scalar_type() == at::kFloat, what, " must be float32");
+    TORCH_CHECK(t.device() == q.device(), what, " must be on the device of q");
+    TORCH_CHECK(t.dim() == 4 && t.size(1) == d.heads_v && t.size(2) == d.dim_k && t.size(3) == d.dim_v, what,
+                " must be (rows, heads_v, dim_k, dim_v)");
+    TORCH_CHECK(t.stride(3) == 1 && t.stride(2) == d.dim_v, what, " must be contiguous along its last two dimensions");
+}
+
+void gdr_indices(cc1d_gdr_params &p, const OptTensor &state_indices_, int64_t n, int64_t rows, const at::Tensor &q) {
+    p.state_rows = rows;
+    if (!state_indices_.has_value()) {
+        TORCH_CHECK(rows >= n, "the state tensor has fewer rows than there are sequences");
+        return;
+    }
+    const at::Tensor &t = *state_indices_;
+    need_cuda(t, "state_indices");
+    TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.dim() == 1 && t.numel() == n && t.device() == q.device(),
+                "state_indices must be a contiguous int32 tensor with one entry per sequence, on the device of q");
+    p.state_indices = t.data_ptr<int32_t>();
+}
+
+}  // namespace
+
+void gated_delta_rule_update(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
+                             const at::Tensor &beta, at::Tensor &state, const OptTensor &state_indices_, at::Tensor &out,
+                             double scale) {
+    cc1d_gdr_params p = {};
+    const GdrDims d = gdr_inputs(p, q, k, v, g, beta, scale);
+    gdr_out(p, d, q, out);
+    gdr_state(state, d, q, "state");
+    gdr_indices(p, state_indices_, d.batch, state.size(0), q);
+    p.final_states = state.data_ptr<float>();
+    p.final_states_batch_stride = state.stride(0); p.final_states_h_stride = state.stride(1);
+    c10::cuda::CUDAGuard guard(q.device());
+    raise_on(cc1d_gdr_update(&p, at::cuda::getCurrentCUDAStream().stream()), "gated_delta_rule_update");
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.def("gated_delta_rule_update", &gated_delta_rule_update, "Gated delta rule decode step");
     m.def("causal_conv1d_fwd", &causal_conv1d_fwd, "Causal conv1d forward");
     m.def("causal_conv1d_bwd", &causal_conv1d_bwd, "Causal conv1d backward",
           py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("dout"), py::arg("seq_idx"),

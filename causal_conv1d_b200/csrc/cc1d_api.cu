@@ -171,7 +171,7 @@ using namespace cc1d;
 
 extern "C" {
 
-int cc1d_abi_version(void) { return 4; }
+int cc1d_abi_version(void) { return 5; }
 
 size_t cc1d_peer_allreduce_buffer_bytes(int32_t world, int64_t count) { return peer_allreduce_buffer_bytes(world, count); }
 
@@ -218,6 +218,8 @@ const char *cc1d_status_str(int status) {
         case CC1D_ERR_CAPTURE: return "the first cc1d_bwd_noalloc call on a device must be made outside stream capture";
         case CC1D_ERR_SEQ_IDX_STATES: return "seq_idx cannot be combined with initial_states / final_states (packed sequences with states: cc1d_prefill_varlen)";
         case CC1D_ERR_PHASE: return "cc1d_bwd_params.phase must be 0 (whole backward), 1 (main kernel) or 2 (finishing kernel)";
+        case CC1D_ERR_GDR_DIM: return "the delta rule supports key and value dims that are multiples of 8 between 8 and 128";
+        case CC1D_ERR_GDR_HEADS: return "the number of value heads must be a positive multiple of the number of key heads";
         default: return "unknown cc1d status";
     }
 }

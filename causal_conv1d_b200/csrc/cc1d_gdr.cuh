@@ -1,0 +1,52 @@
+// Shared pieces of the gated delta rule kernels: arguments, gates, sequence lookup.
+#pragma once
+
+#include "cc1d_common.cuh"
+#include "cc1d_gdr.h"
+#include "cc1d_kernels.h"
+
+namespace cc1d {
+
+constexpr int kGdrMaxDim = 128;
+
+// exp(x) to about 2^-22: ex2.approx with the rounding of x * log2(e) put back as a first-order
+// term (the plain form would lose |x| * 2^-24).  Arguments below -200 (and -inf) give 0.
+__device__ __forceinline__ float gdr_exp(float x) {
+    constexpr float kLog2e = 1.44269504088896341f, kLog2eLow = 1.92596299112661e-8f, kLn2 = 0.693147180559945309f;
+    x = x < -200.f ? -200.f : x;
+    const float hi = x * kLog2e;
+    const float lo = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -hi));
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
+    return fmaf(e, lo * kLn2, e);
+}
+
+__device__ __forceinline__ float load_any(const void *p, int64_t at, int dtype) { return load_w(p, at, dtype); }
+
+// Tokens [begin, end) of sequence n, and the batch row they lie in.
+struct GdrSeq { int64_t row; int32_t begin, end; };
+
+__device__ __forceinline__ GdrSeq gdr_sequence(const cc1d_gdr_params &p, int n) {
+    if (p.cu_seqlens == nullptr) return {n, 0, (int32_t)p.seqlen};
+    const int32_t last = (int32_t)p.seqlen;
+    int32_t a = __ldg(p.cu_seqlens + n), b = __ldg(p.cu_seqlens + n + 1);
+    a = min(max(a, 0), last);
+    b = min(max(b, a), last);
+    return {0, a, b};
+}
+
+// State row of sequence n; negative where it has none.
+__device__ __forceinline__ int64_t gdr_state_row(const cc1d_gdr_params &p, int64_t n) {
+    const int64_t r = p.state_indices != nullptr ? (int64_t)__ldg(p.state_indices + n) : n;
+    return r < p.state_rows ? r : -1;
+}
+
+__host__ __device__ inline int64_t gdr_sequences(const cc1d_gdr_params &p) { return p.cu_seqlens != nullptr ? p.nseq : p.batch; }
+
+int launch_gdr_update(const cc1d_gdr_params &p, cudaStream_t stream);
+size_t gdr_fwd_workspace_bytes(const cc1d_gdr_params &p);
+int launch_gdr_fwd(const cc1d_gdr_params &p, cudaStream_t stream);
+size_t gdr_bwd_workspace_bytes(const cc1d_gdr_bwd_params &p);
+int launch_gdr_bwd(const cc1d_gdr_bwd_params &p, cudaStream_t stream);
+
+}  // namespace cc1d

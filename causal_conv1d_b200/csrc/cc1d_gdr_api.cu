@@ -1,0 +1,50 @@
+// extern "C" entry points of the gated delta rule (include/cc1d.h): validation and hand-off.
+#include "cc1d.h"
+#include "cc1d_gdr.cuh"
+#include "cc1d_kernels.h"
+
+namespace cc1d {
+namespace {
+
+bool bad_dtype(int d) { return d != CC1D_F32 && d != CC1D_F16 && d != CC1D_BF16; }
+bool elem_aligned(const void *p, int dtype) { return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)elem_size(dtype)) == 0; }
+
+int check_gdr(const cc1d_gdr_params &p) {
+    if (bad_dtype(p.itype) || bad_dtype(p.gtype) || bad_dtype(p.btype)) return CC1D_ERR_DTYPE;
+    if (p.batch < 0 || p.seqlen < 0 || p.nseq < 0 || p.heads_k < 0 || p.heads_v < 0) return CC1D_ERR_SHAPE;
+    if (p.dim_k < 8 || p.dim_k > kGdrMaxDim || p.dim_k % 8 || p.dim_v < 8 || p.dim_v > kGdrMaxDim || p.dim_v % 8) return CC1D_ERR_GDR_DIM;
+    if (p.heads_k < 1 || p.heads_v < 1 || p.heads_v % p.heads_k != 0) return CC1D_ERR_GDR_HEADS;
+    if (p.seqlen >= (1ll << 31) - 4096 || p.heads_v >= (1 << 20) || p.batch >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
+    if (p.initial_states != nullptr && (!is_aligned16(p.initial_states) || p.initial_states_batch_stride % 4 || p.initial_states_h_stride % 4)) return CC1D_ERR_ALIGN;
+    if (p.final_states != nullptr && (!is_aligned16(p.final_states) || p.final_states_batch_stride % 4 || p.final_states_h_stride % 4)) return CC1D_ERR_ALIGN;
+    return CC1D_OK;
+}
+
+int check_tensors(const cc1d_gdr_params &p) {
+    if (p.q == nullptr || p.k == nullptr || p.v == nullptr || p.g == nullptr || p.beta == nullptr || p.out == nullptr) return CC1D_ERR_NULL;
+    if (!elem_aligned(p.q, p.itype) || !elem_aligned(p.k, p.itype) || !elem_aligned(p.v, p.itype) || !elem_aligned(p.out, p.itype) ||
+        !elem_aligned(p.g, p.gtype) || !elem_aligned(p.beta, p.btype)) return CC1D_ERR_ALIGN;
+    return CC1D_OK;
+}
+
+}  // namespace
+}  // namespace cc1d
+
+using namespace cc1d;
+
+extern "C" {
+
+int cc1d_gdr_update(const cc1d_gdr_params *p, cc1d_stream_t stream) {
+    if (p == nullptr) return CC1D_ERR_NULL;
+    cc1d_gdr_params a = *p;
+    a.initial_states = nullptr; a.cu_seqlens = nullptr; a.has_initial_state = nullptr;
+    int rc = check_gdr(a);
+    if (rc != CC1D_OK) return rc;
+    if (a.batch == 0 || a.seqlen == 0) return CC1D_OK;
+    rc = check_tensors(a);
+    if (rc != CC1D_OK) return rc;
+    if (a.final_states == nullptr) return CC1D_ERR_NULL;
+    return launch_gdr_update(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -48,7 +48,9 @@ typedef enum cc1d_status {
     CC1D_ERR_SCRATCH_ADDRESS = 16, /* cc1d_bwd_noalloc could not look up its built-in scratch on this device */
     CC1D_ERR_CAPTURE = 17,      /* first cc1d_bwd_noalloc call on a device made inside a stream capture */
     CC1D_ERR_SEQ_IDX_STATES = 18, /* seq_idx given together with initial/final states (use cc1d_prefill_varlen) */
-    CC1D_ERR_PHASE = 19         /* cc1d_bwd_params.phase not in {0, 1, 2}                 */
+    CC1D_ERR_PHASE = 19,        /* cc1d_bwd_params.phase not in {0, 1, 2}                 */
+    CC1D_ERR_GDR_DIM = 20,      /* delta rule: dim_k, dim_v must be multiples of 8 in 8..128 */
+    CC1D_ERR_GDR_HEADS = 21     /* delta rule: heads_v must be a multiple of heads_k         */
 } cc1d_status;
 
 /* ---------------------------------------------------------------------------
