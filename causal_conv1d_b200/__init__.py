@@ -14,7 +14,10 @@ from causal_conv1d_b200.causal_conv1d_interface import (  # noqa: F401
     causal_conv1d_update,
 )
 from causal_conv1d_b200.causal_conv1d_varlen import causal_conv1d_varlen_states  # noqa: F401
-from causal_conv1d_b200.gated_delta_rule import gated_delta_rule_update  # noqa: F401
+from causal_conv1d_b200.gated_delta_rule import (  # noqa: F401
+    gated_delta_rule_update,
+    gated_delta_rule_varlen_fn,
+)
 
 
 def install_as_causal_conv1d() -> None:

@@ -487,7 +487,69 @@ void gated_delta_rule_update(const at::Tensor &q, const at::Tensor &k, const at:
     raise_on(cc1d_gdr_update(&p, at::cuda::getCurrentCUDAStream().stream()), "gated_delta_rule_update");
 }
 
+namespace {
+
+void gdr_sequences(cc1d_gdr_params &p, const GdrDims &d, const at::Tensor &q, const OptTensor &cu_seqlens_) {
+    if (!cu_seqlens_.has_value()) return;
+    const at::Tensor &cu = *cu_seqlens_;
+    need_cuda(cu, "cu_seqlens");
+    TORCH_CHECK(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.is_contiguous() && cu.size(0) >= 1 && cu.device() == q.device(),
+                "cu_seqlens must be a contiguous int32 tensor (nseq + 1,) on the device of q");
+    TORCH_CHECK(d.batch == 1, "cu_seqlens needs a batch of one packed row");
+    p.cu_seqlens = cu.data_ptr<int32_t>();
+    p.nseq = cu.size(0) - 1;
+}
+
+int64_t sequence_count(const cc1d_gdr_params &p) { return p.cu_seqlens != nullptr ? p.nseq : p.batch; }
+
+at::Tensor scratch(size_t bytes, const at::Tensor &like) {
+    return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+}  // namespace
+
+// initial_states / final_states: (rows, heads_v, dim_k, dim_v) fp32
+void gated_delta_rule_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                          const OptTensor &cu_seqlens_, const OptTensor &initial_states_, const OptTensor &final_states_,
+                          const OptTensor &state_indices_, const OptTensor &has_initial_state_, at::Tensor &out, double scale) {
+    cc1d_gdr_params p = {};
+    const GdrDims d = gdr_inputs(p, q, k, v, g, beta, scale);
+    gdr_out(p, d, q, out);
+    gdr_sequences(p, d, q, cu_seqlens_);
+    const int64_t n = sequence_count(p);
+    int64_t rows = -1;
+    if (initial_states_.has_value()) {
+        const at::Tensor &t = *initial_states_;
+        gdr_state(t, d, q, "initial_states");
+        rows = t.size(0);
+        p.initial_states = t.data_ptr<float>();
+        p.initial_states_batch_stride = t.stride(0); p.initial_states_h_stride = t.stride(1);
+    }
+    if (final_states_.has_value()) {
+        const at::Tensor &t = *final_states_;
+        gdr_state(t, d, q, "final_states");
+        TORCH_CHECK(rows < 0 || t.size(0) == rows, "initial_states and final_states differ in their number of rows");
+        rows = t.size(0);
+        p.final_states = t.data_ptr<float>();
+        p.final_states_batch_stride = t.stride(0); p.final_states_h_stride = t.stride(1);
+    }
+    if (rows >= 0) gdr_indices(p, state_indices_, n, rows, q);
+    if (has_initial_state_.has_value()) {
+        const at::Tensor &t = *has_initial_state_;
+        need_cuda(t, "has_initial_state");
+        TORCH_CHECK((t.scalar_type() == at::kBool || t.scalar_type() == at::kByte) && t.is_contiguous() && t.numel() == n && t.device() == q.device(),
+                    "has_initial_state must be a contiguous bool tensor with one entry per sequence, on the device of q");
+        p.has_initial_state = reinterpret_cast<const uint8_t *>(t.data_ptr());
+    }
+    c10::cuda::CUDAGuard guard(q.device());
+    const size_t bytes = cc1d_gdr_fwd_workspace_bytes(&p);
+    at::Tensor ws;
+    if (bytes > 0) { ws = scratch(bytes, q); p.workspace = ws.data_ptr(); p.workspace_bytes = bytes; }
+    raise_on(cc1d_gdr_fwd(&p, at::cuda::getCurrentCUDAStream().stream()), "gated_delta_rule_fwd");
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.def("gated_delta_rule_fwd", &gated_delta_rule_fwd, "Gated delta rule over whole sequences");
     m.def("gated_delta_rule_update", &gated_delta_rule_update, "Gated delta rule decode step");
     m.def("causal_conv1d_fwd", &causal_conv1d_fwd, "Causal conv1d forward");
     m.def("causal_conv1d_bwd", &causal_conv1d_bwd, "Causal conv1d backward",

@@ -191,9 +191,9 @@ int cc1d_peer_allreduce(const cc1d_peer_allreduce_params *p, cc1d_stream_t strea
 }
 
 int cc1d_wait_expired(void) {
-    const int f = fwd_wait_expired(), b = bwd_wait_expired();
-    if (f < 0 || b < 0) return -1;
-    return (f != 0 ? 1 : 0) | (b != 0 ? 2 : 0);
+    const int f = fwd_wait_expired(), b = bwd_wait_expired(), g = gdr_wait_expired();
+    if (f < 0 || b < 0 || g < 0) return -1;
+    return (f != 0 ? 1 : 0) | (b != 0 ? 2 : 0) | (g != 0 ? 4 : 0);
 }
 
 const char *cc1d_status_str(int status) {

@@ -27,6 +27,27 @@ int check_tensors(const cc1d_gdr_params &p) {
     return CC1D_OK;
 }
 
+// what the chunked kernels' 16-byte loads need
+bool rows_aligned(const void *t, int64_t bs, int64_t ls, int64_t hs, int64_t batch, int64_t seqlen, int64_t heads, int dtype) {
+    const int v = vec_elems(dtype);
+    return is_aligned16(t) && (batch <= 1 || bs % v == 0) && (seqlen <= 1 || ls % v == 0) && (heads <= 1 || hs % v == 0);
+}
+
+int check_whole(const cc1d_gdr_params &p) {
+    int rc = check_gdr(p);
+    if (rc != CC1D_OK) return rc;
+    if (p.cu_seqlens != nullptr && p.batch != 1) return CC1D_ERR_SHAPE;
+    if (p.cu_seqlens == nullptr && p.nseq != 0) return CC1D_ERR_NULL;
+    return CC1D_OK;
+}
+
+int check_rows(const cc1d_gdr_params &p) {
+    if (!rows_aligned(p.q, p.q_batch_stride, p.q_l_stride, p.q_h_stride, p.batch, p.seqlen, p.heads_k, p.itype) ||
+        !rows_aligned(p.k, p.k_batch_stride, p.k_l_stride, p.k_h_stride, p.batch, p.seqlen, p.heads_k, p.itype) ||
+        !rows_aligned(p.v, p.v_batch_stride, p.v_l_stride, p.v_h_stride, p.batch, p.seqlen, p.heads_v, p.itype)) return CC1D_ERR_ALIGN;
+    return CC1D_OK;
+}
+
 }  // namespace
 }  // namespace cc1d
 
@@ -45,6 +66,29 @@ int cc1d_gdr_update(const cc1d_gdr_params *p, cc1d_stream_t stream) {
     if (rc != CC1D_OK) return rc;
     if (a.final_states == nullptr) return CC1D_ERR_NULL;
     return launch_gdr_update(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t cc1d_gdr_fwd_workspace_bytes(const cc1d_gdr_params *p) {
+    if (p == nullptr || check_whole(*p) != CC1D_OK) return 0;
+    return gdr_fwd_workspace_bytes(*p);
+}
+
+int cc1d_gdr_fwd(const cc1d_gdr_params *p, cc1d_stream_t stream) {
+    if (p == nullptr) return CC1D_ERR_NULL;
+    int rc = check_whole(*p);
+    if (rc != CC1D_OK) return rc;
+    const int64_t sequences = gdr_sequences(*p);
+    if (p->seqlen == 0 || p->batch == 0) {
+        // no tokens: nothing but the states of empty sequences, which the kernel copies
+        if (sequences == 0 || p->final_states == nullptr) return CC1D_OK;
+    } else {
+        rc = check_tensors(*p);
+        if (rc == CC1D_OK) rc = check_rows(*p);
+        if (rc != CC1D_OK) return rc;
+    }
+    const size_t need = gdr_fwd_workspace_bytes(*p);
+    if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need || !is_aligned16(p->workspace))) return CC1D_ERR_WORKSPACE;
+    return launch_gdr_fwd(*p, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -44,6 +44,7 @@ size_t peer_allreduce_buffer_bytes(int world, int64_t count);
 int launch_peer_allreduce(const cc1d_peer_allreduce_params &p, cudaStream_t stream);
 int fwd_wait_expired();   // bounded-wait flags of the TMA kernels, per translation unit (synchronise)
 int bwd_wait_expired();
+int gdr_wait_expired();
 int launch_update(const cc1d_update_params &p, cudaStream_t stream);
 int launch_varlen_states(const cc1d_varlen_states_params &p, cudaStream_t stream);
 int launch_seq_idx(const int32_t *cu, int64_t nseq, int64_t total, int32_t *seq_idx, cudaStream_t stream);

@@ -50,3 +50,57 @@ def gated_delta_rule_update(
     _ext.gated_delta_rule_update(q, k, v, g, beta, state, state_indices, out,
                                  q.shape[-1] ** -0.5 if scale is None else scale)
     return out.squeeze(1) if squeeze else out
+
+
+def _rows(t: Tensor) -> Tensor:
+    """t where the chunked kernels' 16-byte loads can read it, else a dense copy."""
+    step = 16 // t.element_size()
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n <= 1 or s % step == 0 for n, s in zip(t.shape[:-1], t.stride()))
+    return t if ok else t.contiguous()
+
+
+def gated_delta_rule_varlen_fn(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    g: Tensor,
+    beta: Tensor,
+    *,
+    cu_seqlens: Tensor,
+    states: Tensor | None = None,
+    state_indices: Tensor | None = None,
+    has_initial_state: Tensor | None = None,
+    update_states: bool = True,
+    scale: float | None = None,
+) -> Tensor:
+    """
+    Packed variable-length prefill that continues from, and leaves behind, per-sequence states: the
+    counterpart of ``causal_conv1d_varlen_fn``. Forward only.
+
+    Parameters:
+        q, k: (total_tokens, heads_k, dim_k); sequence s owns rows cu_seqlens[s]:cu_seqlens[s+1]
+        v: (total_tokens, heads_v, dim_v), dtype of q
+        g, beta: (total_tokens, heads_v), float32, float16 or bfloat16; g: logarithm of the decay
+        cu_seqlens: (nseq + 1,) int32, non-decreasing from 0, its last entry at most total_tokens
+        states: (rows, heads_v, dim_k, dim_v) float32, dense in its last two dimensions, or None.
+            Row r = state_indices[s] (s when state_indices is None) holds sequence s's state. An
+            index that is negative or not below the number of rows: the sequence starts from
+            zeros and stores nothing. No two sequences may name the same row.
+        has_initial_state: (nseq,) bool or None.  Where True (everywhere when None and states is
+            given) the sequence starts from its row; elsewhere from zeros.
+        update_states: write each sequence's last state back into its row of states (in place).
+        scale: factor of the output, dim_k ** -0.5 when None
+    Return:
+        out: (total_tokens, heads_v, dim_v); tokens at or after cu_seqlens[-1] are zero
+    """
+    q, k, v, g, beta = (t.unsqueeze(0) for t in (q, k, v, g, beta))
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if state_indices is not None:
+        state_indices = state_indices.to(torch.int32).contiguous()
+    if has_initial_state is not None:
+        has_initial_state = has_initial_state.to(torch.bool).contiguous()
+    _ext.gated_delta_rule_fwd(
+        _rows(q), _rows(k), _rows(v), g, beta, cu_seqlens.to(torch.int32).contiguous(),
+        states, states if update_states else None, state_indices if states is not None else None,
+        has_initial_state, out, q.shape[-1] ** -0.5 if scale is None else scale)
+    return out.squeeze(0)

@@ -360,10 +360,10 @@ typedef struct cc1d_peer_allreduce_params {
 size_t cc1d_peer_allreduce_buffer_bytes(int32_t world, int64_t count);
 int cc1d_peer_allreduce(const cc1d_peer_allreduce_params *p, cc1d_stream_t stream);
 
-/* Health check (no reference counterpart).  The TMA kernels wait on shared-memory barriers
+/* Health check (no reference counterpart).  The TMA and tensor-core kernels wait on shared-memory barriers
  * with an iteration limit instead of forever; a wait that runs out makes the kernel stop early
  * and raise a device-side flag.  This call SYNCHRONISES the current device, returns 0 when no
- * wait has run out since the last call (bit 0: forward, bit 1: backward; -1: the flags could
+ * wait has run out since the last call (bit 0: forward, bit 1: backward, bit 2: gated delta rule; -1: the flags could
  * not be read) and clears the flags.  A non-zero answer means outputs written since the last
  * call are incomplete.  Never expected in practice; not for the hot path. */
 int cc1d_wait_expired(void);
