@@ -49,6 +49,14 @@ int check_rows(const cc1d_gdr_params &p) {
 }
 
 }  // namespace
+
+int gdr_prep_wait_expired();   // per translation unit
+int gdr_fwd_wait_expired();
+int gdr_wait_expired() {
+    const int a = gdr_prep_wait_expired(), b = gdr_fwd_wait_expired();
+    return a < 0 || b < 0 ? -1 : a | b;
+}
+
 }  // namespace cc1d
 
 using namespace cc1d;
@@ -84,6 +92,7 @@ int cc1d_gdr_fwd(const cc1d_gdr_params *p, cc1d_stream_t stream) {
     } else {
         rc = check_tensors(*p);
         if (rc == CC1D_OK) rc = check_rows(*p);
+        if (rc == CC1D_OK && !rows_aligned(p->out, p->out_batch_stride, p->out_l_stride, p->out_h_stride, p->batch, p->seqlen, p->heads_v, p->itype)) rc = CC1D_ERR_ALIGN;
         if (rc != CC1D_OK) return rc;
     }
     const size_t need = gdr_fwd_workspace_bytes(*p);

@@ -10,12 +10,14 @@ namespace cc1d {
 constexpr int kChunk = 64;
 
 // ---- tcgen05 ---------------------------------------------------------------------------------
+// The kernels here take all 512 columns of an SM, so tensor-memory addresses are plain constants:
+// column + (lane << 16), from 0.
 __device__ __forceinline__ void tmem_alloc512(uint32_t smem_slot) {   // one whole warp
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(smem_slot) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_free512(uint32_t tmem) {         // the same warp
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+__device__ __forceinline__ void tmem_free512() {                      // the same warp
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(0) : "memory");
 }
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -27,22 +29,17 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 }
 
 template <int N> __device__ __forceinline__ void tmem_ld(float (&f)[N], uint32_t at);
+template <> __device__ __forceinline__ void tmem_ld<8>(float (&f)[8], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]) : "r"(at));
+}
 template <> __device__ __forceinline__ void tmem_ld<16>(float (&f)[16], uint32_t at) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]),
                    "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]) : "r"(at));
 }
-template <> __device__ __forceinline__ void tmem_ld<32>(float (&f)[32], uint32_t at) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-                 "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]),
-                   "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]), "=f"(f[16]),
-                   "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]), "=f"(f[21]), "=f"(f[22]), "=f"(f[23]), "=f"(f[24]),
-                   "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]), "=f"(f[31]) : "r"(at));
-}
-__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "r"(at), "r"(r[0]), "r"(r[1]),
-                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+__device__ __forceinline__ void tmem_st4(uint32_t at, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" :: "r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
 
 // Instruction descriptor of kind::f16, bf16 x bf16 -> fp32 (M rows, N columns; MN-major operands
@@ -57,6 +54,7 @@ __device__ __forceinline__ constexpr uint32_t mma_desc(int M, int N, bool a_mn, 
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead = 16) {
     return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
+__device__ __forceinline__ uint64_t desc_add(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
@@ -66,6 +64,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+
+// One lane of a converged warp.  MMAs are issued under this predicate: the compiler then keeps
+// their descriptors in uniform registers (under `threadIdx.x == 0` each one is moved there anew,
+// which costs more than the MMA).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
 }
 
 // Bounded wait.  When one runs out (never expected) the flag of the translation unit is raised and
@@ -85,9 +92,7 @@ __device__ __forceinline__ void gdr_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
 }
-template <int kId, int kThreads> __device__ __forceinline__ void group_sync() {
-    asm volatile("bar.sync %0, %1;" :: "n"(kId), "n"(kThreads) : "memory");
-}
+template <int kThreads> __device__ __forceinline__ void walk_sync() { asm volatile("bar.sync 1, %0;" :: "n"(kThreads) : "memory"); }
 
 // ---- fp32 as a sum of bf16 pieces ---------------------------------------------------------------
 // x = x1 + x2 + x3 with x1 = bf16(x), x2 = bf16(x - x1), x3 = bf16(x - x1 - x2): 8 + 8 + 8
@@ -104,18 +109,31 @@ template <int kPieces> __device__ __forceinline__ void split_pair(float2 x, uint
     #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
         r[i] = bf16_pair(x);
-        if (i + 1 < kPieces) x = add2(x, make_float2(-__uint_as_float(r[i] << 16), -__uint_as_float(r[i] & 0xffff0000u)));
+        if (i + 1 < kPieces) x = fma2(make_float2(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xffff0000u)), splat2(-1.f), x);
     }
 }
-// 16 values -> kPieces registers vectors of 8 packed pairs
-template <int kPieces> __device__ __forceinline__ void split16(const float (&x)[16], uint32_t (&r)[kPieces][8]) {
+// x[0..7] -> columns of tensor memory, two values per column: piece k at `at` + k * step, the third at `at` + third
+template <int kPieces> __device__ __forceinline__ void split8_to_tmem(const float *x, uint32_t at, uint32_t step, uint32_t third) {
+    uint32_t r[kPieces][4];
     #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
         uint32_t p[kPieces];
         split_pair<kPieces>(make_float2(x[2 * i], x[2 * i + 1]), p);
         #pragma unroll
         for (int k = 0; k < kPieces; ++k) r[k][i] = p[k];
     }
+    #pragma unroll
+    for (int k = 0; k < kPieces; ++k) tmem_st4(at + (k < 2 ? k * step : third), r[k]);
+}
+
+// x[0..7] -> shared memory: piece k, 16 bytes, at `at` + k * 8192
+template <int kPieces> __device__ __forceinline__ void store_pieces8(const float *x, uint32_t at) {
+    uint32_t r[4][kPieces];
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) split_pair<kPieces>(make_float2(x[2 * i], x[2 * i + 1]), r[i]);
+    #pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at + k * 8192), "r"(r[0][k]), "r"(r[1][k]), "r"(r[2][k]), "r"(r[3][k]) : "memory");
 }
 
 template <typename T> struct GdrType;
@@ -130,18 +148,18 @@ __device__ __forceinline__ uint32_t tile_at(int row, int chunk16, uint32_t panel
     return (chunk16 >> 3) * panel_bytes + row * 128 + (((chunk16 & 7) ^ (row & 7)) << 4);
 }
 
-// 8 elements of one row -> one 16-byte piece vector each
-template <typename T, int kPieces> __device__ __forceinline__ void row_pieces(const T *src, bool ok, uint4 (&out)[kPieces]) {
-    if constexpr (sizeof(T) == 2 && kPieces == 1) {
-        out[0] = ok ? ld_cached(src) : make_uint4(0, 0, 0, 0);
+// 8 elements of one row, as they are, and as one 16-byte vector for each piece
+template <typename T> __device__ __forceinline__ void load_row(const T *src, bool ok, uint4 (&v)[sizeof(T) / 2]) {
+    #pragma unroll
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k) v[k] = ok ? ld_cached(src + 4 * k) : make_uint4(0, 0, 0, 0);
+}
+template <typename T, int kPieces> __device__ __forceinline__ void row_pieces(const uint4 (&v)[sizeof(T) / 2], uint4 (&out)[kPieces]) {
+    if constexpr (kPieces == 1) {
+        out[0] = v[0];
     } else {
         float f[8];
-        if constexpr (sizeof(T) == 2) {
-            unpack<T>(ok ? ld_cached(src) : make_uint4(0, 0, 0, 0), f);
-        } else {
-            unpack<T>(ok ? ld_cached(src) : make_uint4(0, 0, 0, 0), f);
-            unpack<T>(ok ? ld_cached(src + 4) : make_uint4(0, 0, 0, 0), f + 4);
-        }
+        unpack<T>(v[0], f);
+        if constexpr (sizeof(T) == 4) unpack<T>(v[1], f + 4);
         uint32_t r[4][kPieces];
         #pragma unroll
         for (int i = 0; i < 4; ++i) split_pair<kPieces>(make_float2(f[2 * i], f[2 * i + 1]), r[i]);
@@ -150,253 +168,149 @@ template <typename T, int kPieces> __device__ __forceinline__ void row_pieces(co
     }
 }
 
+// bytes (a multiple of 16, both ends 16-byte aligned) from shared to global memory by the copy engine
+__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" :: "l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+// the other way; the bytes count on `bar`
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+// 16 bytes from global to shared memory without registers; zeros where !ok
+__device__ __forceinline__ void copy16_async(uint32_t at, const void *src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(at), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// Gates of a chunk.  G, the running sum of g, is summed in double and kept as two floats: a
+// Gates of a chunk.  G, the running sum of g, is kept as two floats: a
 // difference G_i - G_j of near tokens far from the chunk's start keeps its relative accuracy.
+// e^{G_i - G_j} for i in the 16 tokens of block I is row[i] * column[I][j] for j in an earlier block and
+// row[i] * same[j] for j in the same one, all taken from the end of the block before I: row and column
+// are below 1, same[j] above.  Where some block decays by more than e^-60, `steep` is set and products
+// inside a block take an exponential of their own.
 struct GdrGates {
-    float g_hi[kChunk], g_lo[kChunk], from_start[kChunk], to_end[kChunk], beta[kChunk];
+    float2 g[kChunk];                 // high and low part of G
+    float from_start[kChunk], to_end[kChunk], beta[kChunk], minus_beta_from_start[kChunk];
+    float row[kChunk], same[kChunk], column[3][48];
+    int steep;
 };
-__device__ __forceinline__ float gdr_fade(const GdrGates &s, float hi, float lo, int j) {
-    return gdr_exp((hi - s.g_hi[j]) + (lo - s.g_lo[j]));
-}
-
-// One warp: gates of tokens t0 .. t0 + 63 (those at or after `end` do not exist: g = beta = 0).
-__device__ __forceinline__ void load_gates(GdrGates &s, const cc1d_gdr_params &p, const GdrSeq &seq, int h, int t0, int lane) {
-    const int64_t ga = seq.row * p.g_batch_stride + h * p.g_h_stride, ba = seq.row * p.beta_batch_stride + h * p.beta_h_stride;
-    double v[2];
-    #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int t = t0 + 2 * lane + i;
-        const bool ok = t < seq.end;
-        const float g = ok ? load_any(p.g, ga + t * p.g_l_stride, p.gtype) : 0.f;
-        v[i] = g < -200.f ? -200.0 : (double)g;
-        s.beta[2 * lane + i] = ok ? load_any(p.beta, ba + t * p.beta_l_stride, p.btype) : 0.f;
-    }
-    v[1] += v[0];
-    double sum = v[1];
-    #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        const double o = __shfl_up_sync(kFullMask, sum, m);
-        if (lane >= m) sum += o;
-    }
-    const double before = sum - v[1], whole = __shfl_sync(kFullMask, sum, 31);
-    #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const double G = before + v[i];
-        const float hi = (float)G;
-        s.g_hi[2 * lane + i] = hi;
-        s.g_lo[2 * lane + i] = (float)(G - (double)hi);
-        s.from_start[2 * lane + i] = gdr_exp(hi) * (1.f + (float)(G - (double)hi));
-        s.to_end[2 * lane + i] = gdr_exp((float)(whole - G));
-    }
-}
-
-// ---- (I + A)^-1 of a unit lower triangular 64 x 64 matrix ------------------------------------
-// Block elimination: four 16 x 16 diagonal blocks column by column, then 16 -> 32 -> 64 with
-//   T21 = -T22 (A21 T11).
-// a: the strictly lower part (its upper blocks are scratch); t: receives the lower part of the
-// inverse, diagonal included.  Rows are kLd floats.  256 threads; ends without a barrier.
-constexpr int kLd = kChunk + 4;
-
-template <int kId> __device__ __forceinline__ void invert_unit_lower(float *a, float *t, int tid) {
-    if (tid < 64) {
-        const int b = (tid >> 4) * 16, c = tid & 15;
-        float x[16];
-        #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float acc = r == c ? 1.f : 0.f;
-            #pragma unroll
-            for (int l4 = 0; l4 < r; l4 += 4) {
-                const float4 m = *reinterpret_cast<const float4 *>(a + (b + r) * kLd + b + l4);
-                acc = fmaf(-m.x, x[l4], acc);
-                if (l4 + 1 < r) acc = fmaf(-m.y, x[l4 + 1], acc);
-                if (l4 + 2 < r) acc = fmaf(-m.z, x[l4 + 2], acc);
-                if (l4 + 3 < r) acc = fmaf(-m.w, x[l4 + 3], acc);
-            }
-            x[r] = r < c ? 0.f : acc;
-            t[(b + r) * kLd + b + c] = x[r];
-        }
-    }
-    group_sync<kId, 256>();
-    {   // 16 -> 32, two blocks: 2 outputs per thread
-        const int b = (tid >> 7) * 32, r = (tid >> 3) & 15, c = (tid & 7) * 2;
-        float2 m = make_float2(0.f, 0.f);
-        #pragma unroll
-        for (int l = 0; l < 16; ++l) {
-            const float x = a[(b + 16 + r) * kLd + b + l];
-            const float2 y = *reinterpret_cast<const float2 *>(t + (b + l) * kLd + b + c);
-            m.x = fmaf(x, y.x, m.x); m.y = fmaf(x, y.y, m.y);
-        }
-        *reinterpret_cast<float2 *>(a + (b + r) * kLd + b + 16 + c) = m;   // scratch above the diagonal
-        group_sync<kId, 256>();
-        float2 n = make_float2(0.f, 0.f);
-        #pragma unroll
-        for (int l = 0; l < 16; ++l) {
-            const float x = t[(b + 16 + r) * kLd + b + 16 + l];
-            const float2 y = *reinterpret_cast<const float2 *>(a + (b + l) * kLd + b + 16 + c);
-            n.x = fmaf(-x, y.x, n.x); n.y = fmaf(-x, y.y, n.y);
-        }
-        *reinterpret_cast<float2 *>(t + (b + 16 + r) * kLd + b + c) = n;
-        *reinterpret_cast<float2 *>(t + (b + r) * kLd + b + 16 + c) = make_float2(0.f, 0.f);   // zeros above the diagonal
-    }
-    group_sync<kId, 256>();
-    {   // 32 -> 64: 4 outputs per thread
-        const int r = tid >> 3, c = (tid & 7) * 4;
-        float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
-        #pragma unroll 8
-        for (int l = 0; l < 32; ++l) {
-            const float x = a[(32 + r) * kLd + l];
-            const float4 y = *reinterpret_cast<const float4 *>(t + l * kLd + c);
-            m.x = fmaf(x, y.x, m.x); m.y = fmaf(x, y.y, m.y); m.z = fmaf(x, y.z, m.z); m.w = fmaf(x, y.w, m.w);
-        }
-        *reinterpret_cast<float4 *>(a + r * kLd + 32 + c) = m;
-        group_sync<kId, 256>();
-        float4 n = make_float4(0.f, 0.f, 0.f, 0.f);
-        #pragma unroll 8
-        for (int l = 0; l < 32; ++l) {
-            const float x = t[(32 + r) * kLd + 32 + l];
-            const float4 y = *reinterpret_cast<const float4 *>(a + l * kLd + 32 + c);
-            n.x = fmaf(-x, y.x, n.x); n.y = fmaf(-x, y.y, n.y); n.z = fmaf(-x, y.z, n.z); n.w = fmaf(-x, y.w, n.w);
-        }
-        *reinterpret_cast<float4 *>(t + (32 + r) * kLd + c) = n;
-        *reinterpret_cast<float4 *>(t + r * kLd + 32 + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-}
+__device__ __forceinline__ float gdr_fade(float2 gi, float2 gj) { return gdr_exp((gi.x - gj.x) + (gi.y - gj.y)); }
 
 }  // namespace cc1d
 
 namespace cc1d {
 
 // ---- a chunk made ready -------------------------------------------------------------------------
-// What the walk over the chunks reads of one chunk:
-//   K, Q   token tiles, rows 0-63 k, 64-127 q (kPieces pieces)
-//   T      (I + A)^-1, A_ij = beta_i (k_i.k_j) e^{G_i - G_j} for j < i    (3 pieces, row i, column j)
-//   P      (q_i.k_j) e^{G_i - G_j} for j <= i                             (kOutPieces pieces)
-//   V      as it is, [64][128]
+// What the walks over the chunks read of one chunk, as it lies in a stage of shared memory:
+//   K, Q   token tiles, rows 0-63 k, 64-127 q (kPieces pieces), loaded by the walk itself
+//   V      as it is, [64][128]                                                 "
+//   T - I  T = (I + A)^-1, A_ij = beta_i (k_i.k_j) e^{G_i - G_j} for j < i   (2 pieces, row i, column j)
+//   P      (q_i.k_j) e^{G_i - G_j} for j <= i                                (kOutPieces pieces)
+//   gates
+// T, P and the gates are one image in the workspace, made by gdr_prep_kernel for all chunks at
+// once (inside the walk their chain of short dependent steps, 13,000 cycles a chunk, held it up).
+// The product with T is taken as x + (T - I) x, x in fp32: two pieces of both then leave 2^-17 of
+// the correction alone, not of x.
 template <typename T> struct GdrStage {
     static constexpr int kPieces = GdrType<T>::kPieces, kOut = GdrType<T>::kOutPieces;
     static constexpr uint32_t kPanel = 128 * 128, kKqPiece = 2 * kPanel;     // panel: 128 rows x 64 columns
-    static constexpr uint32_t kKq = 0, kT = kKq + kPieces * kKqPiece, kP = kT + 3 * 8192, kV = kP + kOut * 8192,
-                              kGates = kV + kChunk * kGdrMaxDim * sizeof(T), kBytes = kGates + 2048;
+    static constexpr uint32_t kKq = 0, kV = kPieces * kKqPiece, kT = kV + kChunk * kGdrMaxDim * sizeof(T), kP = kT + 2 * 8192,
+                              kGates = kP + kOut * 8192, kBytes = kGates + 3072, kImage = kBytes - kT;
 };
-static_assert(sizeof(GdrGates) <= 2048, "gates of a chunk");
-constexpr uint32_t kGdrInverseBytes = 2 * kChunk * kLd * 4;
+static_assert(sizeof(GdrGates) <= 3072, "gates of a chunk");
 
-constexpr uint32_t kColKq = 416;   // tensor-memory columns 416..479: K K^T (lanes 0-63) and Q K^T (lanes 64-127)
-
-// 256 threads (warps 0-7 of the group) fill a stage; bar_kq is theirs.  Ends without a barrier:
-// the caller orders its generic-proxy writes before the walk's MMAs.
-template <typename T, int kId>
-__device__ __forceinline__ void prepare_chunk(unsigned char *stage, float *inv, const cc1d_gdr_params &p, const GdrSeq &seq, int h, int t0,
-                                              uint32_t tmem, uint32_t bar_kq, uint32_t kq_parity, volatile int *dead, int tid) {
-    using S = GdrStage<T>;
-    constexpr int NP = S::kPieces;
-    const int warp = tid >> 5, lane = tid & 31;
-    const uint32_t base = smem_u32(stage);
-    GdrGates &gates = *reinterpret_cast<GdrGates *>(stage + S::kGates);
-    const int hk = h / (int)(p.heads_v / p.heads_k);
-    const T *kp = reinterpret_cast<const T *>(p.k) + seq.row * p.k_batch_stride + hk * p.k_h_stride;
-    const T *qp = reinterpret_cast<const T *>(p.q) + seq.row * p.q_batch_stride + hk * p.q_h_stride;
-    const T *vp = reinterpret_cast<const T *>(p.v) + seq.row * p.v_batch_stride + h * p.v_h_stride;
-    if (warp == 0) load_gates(gates, p, seq, h, t0, lane);
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = (tid >> 4) + 16 * i, c = tid & 15;
-        const int64_t t = t0 + row;
-        const bool ok = t < seq.end && c * 8 < p.dim_k;
-        uint4 kv[NP], qv[NP];
-        row_pieces<T, NP>(kp + t * p.k_l_stride + c * 8, ok, kv);
-        row_pieces<T, NP>(qp + t * p.q_l_stride + c * 8, ok, qv);
-        const uint32_t at = base + S::kKq + tile_at(row, c, S::kPanel);
-        #pragma unroll
-        for (int k = 0; k < NP; ++k) { sts128(at + k * S::kKqPiece, kv[k]); sts128(at + k * S::kKqPiece + 64 * 128, qv[k]); }
-    }
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = (tid >> 4) + 16 * i, c = tid & 15;
-        const int64_t t = t0 + row;
-        const bool ok = t < seq.end && c * 8 < p.dim_v;
-        const T *src = vp + t * p.v_l_stride + c * 8;
-        #pragma unroll
-        for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-            sts128(base + S::kV + (row * kGdrMaxDim + c * 8) * sizeof(T) + 16 * k, ok ? ld_cached(src + 4 * k) : make_uint4(0, 0, 0, 0));
-    }
-    fence_proxy_async_smem();
-    group_sync<kId, 256>();
-    if (tid == 0) {
-        fence_after_sync();
-        constexpr uint32_t id = mma_desc(128, 64, false, false);
-        const int steps = (int)(p.dim_k + 15) / 16;
-        bool add = false;
-        #pragma unroll
-        for (int a = 0; a < NP; ++a) {
-            #pragma unroll
-            for (int b = 0; b < NP && a + b < 3; ++b) {
-                for (int s = 0; s < steps; ++s) {
-                    const uint32_t off = (s >> 2) * S::kPanel + (s & 3) * 32;
-                    mma_ss(tmem + kColKq, smem_desc(base + S::kKq + a * S::kKqPiece + off), smem_desc(base + S::kKq + b * S::kKqPiece + off), id, add);
-                    add = true;
-                }
-            }
-        }
-        mma_commit(bar_kq);
-    }
-    gdr_wait(bar_kq, kq_parity, dead);
-    __syncwarp();
-    fence_after_sync();
-    {
-        const int quad = warp & 3, half = warp >> 2, i = (quad & 1) * 32 + lane;
-        const float hi = gates.g_hi[i], lo = gates.g_lo[i], beta = gates.beta[i];
-        #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int j0 = 32 * half + 16 * b;
-            float x[16];
-            tmem_ld<16>(x, tmem + ((uint32_t)(quad * 32) << 16) + kColKq + j0);
-            tmem_wait_ld();
-            if (quad < 2) {
-                #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = j0 + j < i ? beta * x[j] * gdr_fade(gates, hi, lo, j0 + j) : 0.f;
-                #pragma unroll
-                for (int j = 0; j < 16; j += 4)
-                    *reinterpret_cast<float4 *>(inv + i * kLd + j0 + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-            } else {
-                #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = j0 + j <= i ? x[j] * gdr_fade(gates, hi, lo, j0 + j) : 0.f;
-                uint32_t r[S::kOut][8];
-                split16<S::kOut>(x, r);
-                #pragma unroll
-                for (int k = 0; k < S::kOut; ++k) {
-                    sts128(base + S::kP + k * 8192 + tile_at(i, j0 / 8, 0), make_uint4(r[k][0], r[k][1], r[k][2], r[k][3]));
-                    sts128(base + S::kP + k * 8192 + tile_at(i, j0 / 8 + 1, 0), make_uint4(r[k][4], r[k][5], r[k][6], r[k][7]));
-                }
-            }
-        }
-        fence_before_sync();
-    }
-    group_sync<kId, 256>();
-    float *t = inv + kChunk * kLd;
-    invert_unit_lower<kId>(inv, t, tid);
-    group_sync<kId, 256>();
-    {
-        const int i = tid >> 2, j0 = (tid & 3) * 16;
-        float x[16];
-        #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const float4 v = *reinterpret_cast<const float4 *>(t + i * kLd + j0 + j);
-            x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
-        }
-        uint32_t r[3][8];
-        split16<3>(x, r);
-        #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            sts128(base + S::kT + k * 8192 + tile_at(i, j0 / 8, 0), make_uint4(r[k][0], r[k][1], r[k][2], r[k][3]));
-            sts128(base + S::kT + k * 8192 + tile_at(i, j0 / 8 + 1, 0), make_uint4(r[k][4], r[k][5], r[k][6], r[k][7]));
-        }
-    }
-    fence_proxy_async_smem();
+// Chunks of sequence n in the workspace: slots gdr_first_slot(n) .. ; the slots of different sequences
+// never meet (a sequence of L tokens takes ceil(L / 64) of the at least floor(L / 64) + 1 there are).
+__host__ __device__ inline int64_t gdr_slots(const cc1d_gdr_params &p) {
+    return p.cu_seqlens != nullptr ? p.seqlen / kChunk + p.nseq : p.batch * ((p.seqlen + kChunk - 1) / kChunk);
 }
+__device__ __forceinline__ int64_t gdr_first_slot(const cc1d_gdr_params &p, const GdrSeq &seq, int n) {
+    return p.cu_seqlens != nullptr ? (int64_t)(seq.begin / kChunk) + n : n * ((p.seqlen + kChunk - 1) / kChunk);
+}
+
+// kN threads bring rows of q and k (and v) into their tiles: one-piece types by asynchronous
+// copies, the others split on the way.  The caller waits for the copies and fences.
+template <typename T, int kN> struct GdrRows {
+    using S = GdrStage<T>;
+    static constexpr int NP = S::kPieces, kVecs = sizeof(T) / 2;
+    const T *kp, *qp, *vp;
+    int64_t k_step, q_step, v_step;
+    int end, dk, dv;
+    // v: 64 x dim_v rows beside k and q (the values, or the output's gradient)
+    __device__ __forceinline__ GdrRows(const cc1d_gdr_params &p, const GdrSeq &seq, int h, const void *v, int64_t v_row, int64_t v_step_)
+        : k_step(p.k_l_stride), q_step(p.q_l_stride), v_step(v_step_), end(seq.end), dk((int)p.dim_k), dv((int)p.dim_v) {
+        const int hk = h / (int)(p.heads_v / p.heads_k);
+        kp = reinterpret_cast<const T *>(p.k) + seq.row * p.k_batch_stride + hk * p.k_h_stride;
+        qp = reinterpret_cast<const T *>(p.q) + seq.row * p.q_batch_stride + hk * p.q_h_stride;
+        vp = reinterpret_cast<const T *>(v) + v_row;
+    }
+    __device__ __forceinline__ void load_kq(uint32_t stage, int t0, int tid) const {
+        const int row0 = tid >> 4, c8 = (tid & 15) * 8;
+        #pragma unroll 4
+        for (int i = 0; i < 1024 / kN; ++i) {
+            const int row = row0 + kN / 16 * i;
+            const int64_t t = t0 + row;
+            const bool ok = t < end && c8 < dk;
+            const uint32_t at = stage + S::kKq + tile_at(row, c8 / 8, S::kPanel);
+            const T *k_src = ok ? kp + t * k_step + c8 : kp, *q_src = ok ? qp + t * q_step + c8 : qp;
+            if constexpr (NP == 1) {
+                copy16_async(at, k_src, ok);
+                copy16_async(at + 64 * 128, q_src, ok);
+            } else {
+                uint4 kr[kVecs], qr[kVecs], kk[NP], qq[NP];
+                load_row<T>(k_src, ok, kr);
+                load_row<T>(q_src, ok, qr);
+                row_pieces<T, NP>(kr, kk);
+                row_pieces<T, NP>(qr, qq);
+                #pragma unroll
+                for (int k = 0; k < NP; ++k) { sts128(at + k * S::kKqPiece, kk[k]); sts128(at + k * S::kKqPiece + 64 * 128, qq[k]); }
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(uint32_t stage, int t0, int tid) const {
+        const int row0 = tid >> 4, c8 = (tid & 15) * 8;
+        #pragma unroll 4
+        for (int i = 0; i < 1024 / kN; ++i) {
+            const int row = row0 + kN / 16 * i;
+            const int64_t t = t0 + row;
+            const bool ok = t < end && c8 < dv;
+            const T *src = ok ? vp + t * v_step + c8 : vp;
+            #pragma unroll
+            for (int k = 0; k < kVecs; ++k) copy16_async(stage + S::kV + (row * kGdrMaxDim + c8) * sizeof(T) + 16 * k, src + 4 * k, ok);
+        }
+    }
+};
+
+constexpr int kFeeders = 64;
+// The last two warps of a walk: chunk after chunk into the stages, forwards or (kBack) from the last to the first.
+// bar_full counts the threads and the one that announces the image.
+template <typename T, int kStages, bool kBack>
+__device__ __forceinline__ void feed_walk(const GdrRows<T, kFeeders> &rows, const unsigned char *images, int64_t image_step, uint32_t smem, int begin, int chunks,
+                                          uint32_t bar_full, uint32_t bar_empty, volatile int *dead, int tid) {
+    using S = GdrStage<T>;
+    for (int i = 0; i < chunks; ++i) {
+        const int s = i % kStages, c = kBack ? chunks - 1 - i : i;
+        const uint32_t stage = smem + s * S::kBytes, full = bar_full + 8 * s;
+        gdr_wait(bar_empty + 8 * s, ((i / kStages) & 1) ^ 1, dead);
+        if (tid == 0) {
+            mbar_expect_tx(full, S::kImage);
+            bulk_load(stage + S::kT, images + c * image_step, S::kImage, full);
+        }
+        rows.load_kq(stage, begin + c * kChunk, tid);
+        rows.load_v(stage, begin + c * kChunk, tid);
+        copy_async_wait();
+        fence_proxy_async_smem();
+        mbar_arrive(full);
+    }
+}
+
+size_t gdr_image_bytes(const cc1d_gdr_params &p);                     // of all chunks
+int launch_gdr_prep(const cc1d_gdr_params &p, void *images, cudaStream_t stream);
 
 }  // namespace cc1d
