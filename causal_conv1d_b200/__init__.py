@@ -15,6 +15,8 @@ from causal_conv1d_b200.causal_conv1d_interface import (  # noqa: F401
 )
 from causal_conv1d_b200.causal_conv1d_varlen import causal_conv1d_varlen_states  # noqa: F401
 from causal_conv1d_b200.gated_delta_rule import (  # noqa: F401
+    GatedDeltaRuleFn,
+    gated_delta_rule_fn,
     gated_delta_rule_update,
     gated_delta_rule_varlen_fn,
 )

@@ -27,7 +27,8 @@ LIB_TORCH = os.path.join(PKG, "_cc1d_torch.so")
 
 CU_SOURCES = ["cc1d_api.cu", "cc1d_fwd.cu", "cc1d_bwd.cu", "cc1d_update.cu", "cc1d_varlen.cu",
               "cc1d_prefill.cu", "cc1d_peer.cu", "cc1d_gdr_api.cu", "cc1d_gdr_update.cu",
-              "cc1d_gdr_prep.cu", "cc1d_gdr_fwd.cu"]
+              "cc1d_gdr_prep.cu", "cc1d_gdr_fwd.cu",
+              "cc1d_gdr_bwd.cu"]
 CU_HEADERS = ["cc1d_common.cuh", "cc1d_kernels.h", "cc1d_tma.cuh", os.path.join(INCLUDE, "cc1d.h")]
 GDR_HEADERS = ["cc1d_gdr.cuh", "cc1d_gdr_mma.cuh", os.path.join(INCLUDE, "cc1d_gdr.h")]     # read by the cc1d_gdr_*.cu only
 

@@ -508,14 +508,9 @@ at::Tensor scratch(size_t bytes, const at::Tensor &like) {
 
 }  // namespace
 
-// initial_states / final_states: (rows, heads_v, dim_k, dim_v) fp32
-void gated_delta_rule_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
-                          const OptTensor &cu_seqlens_, const OptTensor &initial_states_, const OptTensor &final_states_,
-                          const OptTensor &state_indices_, const OptTensor &has_initial_state_, at::Tensor &out, double scale) {
-    cc1d_gdr_params p = {};
-    const GdrDims d = gdr_inputs(p, q, k, v, g, beta, scale);
-    gdr_out(p, d, q, out);
-    gdr_sequences(p, d, q, cu_seqlens_);
+// The sequences' states as cc1d_gdr_params takes them: (rows, heads_v, dim_k, dim_v) fp32
+static void gdr_states(cc1d_gdr_params &p, const GdrDims &d, const at::Tensor &q, const OptTensor &initial_states_,
+                       const OptTensor &final_states_, const OptTensor &state_indices_, const OptTensor &has_initial_state_) {
     const int64_t n = sequence_count(p);
     int64_t rows = -1;
     if (initial_states_.has_value()) {
@@ -541,6 +536,16 @@ void gated_delta_rule_fwd(const at::Tensor &q, const at::Tensor &k, const at::Te
                     "has_initial_state must be a contiguous bool tensor with one entry per sequence, on the device of q");
         p.has_initial_state = reinterpret_cast<const uint8_t *>(t.data_ptr());
     }
+}
+
+void gated_delta_rule_fwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                          const OptTensor &cu_seqlens_, const OptTensor &initial_states_, const OptTensor &final_states_,
+                          const OptTensor &state_indices_, const OptTensor &has_initial_state_, at::Tensor &out, double scale) {
+    cc1d_gdr_params p = {};
+    const GdrDims d = gdr_inputs(p, q, k, v, g, beta, scale);
+    gdr_out(p, d, q, out);
+    gdr_sequences(p, d, q, cu_seqlens_);
+    gdr_states(p, d, q, initial_states_, final_states_, state_indices_, has_initial_state_);
     c10::cuda::CUDAGuard guard(q.device());
     const size_t bytes = cc1d_gdr_fwd_workspace_bytes(&p);
     at::Tensor ws;
@@ -548,8 +553,45 @@ void gated_delta_rule_fwd(const at::Tensor &q, const at::Tensor &k, const at::Te
     raise_on(cc1d_gdr_fwd(&p, at::cuda::getCurrentCUDAStream().stream()), "gated_delta_rule_fwd");
 }
 
+// dq, dk, dv, dg, dbeta: dense, of the shapes and dtypes of what they belong to; dfinal_states and dinitial_states:
+// dense fp32 (sequences, heads_v, dim_k, dim_v)
+void gated_delta_rule_bwd(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g, const at::Tensor &beta,
+                          const OptTensor &cu_seqlens_, const OptTensor &initial_states_, const at::Tensor &dout, const OptTensor &dfinal_states_,
+                          at::Tensor &dq, at::Tensor &dk, at::Tensor &dv, at::Tensor &dg, at::Tensor &dbeta, OptTensor &dinitial_states_, double scale) {
+    cc1d_gdr_bwd_params b = {};
+    const GdrDims d = gdr_inputs(b.fwd, q, k, v, g, beta, scale);
+    gdr_sequences(b.fwd, d, q, cu_seqlens_);
+    gdr_states(b.fwd, d, q, initial_states_, std::nullopt, std::nullopt, std::nullopt);
+    need_cuda(dout, "dout");
+    need_shape(dout, {d.batch, d.seqlen, d.heads_v, d.dim_v}, "dout");
+    TORCH_CHECK(dout.scalar_type() == q.scalar_type() && dout.device() == q.device() && dout.stride(3) == 1,
+                "dout must have the dtype and device of q and be contiguous along its last dimension");
+    b.dout = dout.data_ptr(); b.dout_batch_stride = dout.stride(0); b.dout_l_stride = dout.stride(1); b.dout_h_stride = dout.stride(2);
+    auto grad = [&](at::Tensor &t, const at::Tensor &of, const char *what) {
+        need_cuda(t, what);
+        need_shape(t, of.sizes(), what);
+        TORCH_CHECK(t.scalar_type() == of.scalar_type() && t.device() == q.device() && t.is_contiguous(), what, " must be dense, of the dtype of what it belongs to");
+        return t.data_ptr();
+    };
+    b.dq = grad(dq, q, "dq"); b.dk = grad(dk, k, "dk"); b.dv = grad(dv, v, "dv"); b.dg = grad(dg, g, "dg"); b.dbeta = grad(dbeta, beta, "dbeta");
+    auto state = [&](const at::Tensor &t, const char *what) {
+        need_cuda(t, what);
+        need_shape(t, {sequence_count(b.fwd), d.heads_v, d.dim_k, d.dim_v}, what);
+        TORCH_CHECK(t.scalar_type() == at::kFloat && t.device() == q.device() && t.is_contiguous(), what, " must be a dense float32 tensor on the device of q");
+        return t.data_ptr<float>();
+    };
+    if (dfinal_states_.has_value()) b.dfinal_states = state(*dfinal_states_, "dfinal_states");
+    if (dinitial_states_.has_value()) b.dinitial_states = state(*dinitial_states_, "dinitial_states");
+    c10::cuda::CUDAGuard guard(q.device());
+    const size_t bytes = cc1d_gdr_bwd_workspace_bytes(&b);
+    at::Tensor ws;
+    if (bytes > 0) { ws = scratch(bytes, q); b.workspace = ws.data_ptr(); b.workspace_bytes = bytes; }
+    raise_on(cc1d_gdr_bwd(&b, at::cuda::getCurrentCUDAStream().stream()), "gated_delta_rule_bwd");
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gated_delta_rule_fwd", &gated_delta_rule_fwd, "Gated delta rule over whole sequences");
+    m.def("gated_delta_rule_bwd", &gated_delta_rule_bwd, "Gradients of the gated delta rule");
     m.def("gated_delta_rule_update", &gated_delta_rule_update, "Gated delta rule decode step");
     m.def("causal_conv1d_fwd", &causal_conv1d_fwd, "Causal conv1d forward");
     m.def("causal_conv1d_bwd", &causal_conv1d_bwd, "Causal conv1d backward",

@@ -23,6 +23,12 @@ __device__ __forceinline__ float gdr_exp(float x) {
 
 __device__ __forceinline__ float load_any(const void *p, int64_t at, int dtype) { return load_w(p, at, dtype); }
 
+__device__ __forceinline__ void store_any(void *p, int64_t at, int dtype, float v) {
+    if (dtype == CC1D_F32) reinterpret_cast<float *>(p)[at] = v;
+    else if (dtype == CC1D_BF16) reinterpret_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v);
+    else reinterpret_cast<__half *>(p)[at] = __float2half_rn(v);
+}
+
 // Tokens [begin, end) of sequence n, and the batch row they lie in.
 struct GdrSeq { int64_t row; int32_t begin, end; };
 

@@ -52,9 +52,10 @@ int check_rows(const cc1d_gdr_params &p) {
 
 int gdr_prep_wait_expired();   // per translation unit
 int gdr_fwd_wait_expired();
+int gdr_bwd_wait_expired();
 int gdr_wait_expired() {
-    const int a = gdr_prep_wait_expired(), b = gdr_fwd_wait_expired();
-    return a < 0 || b < 0 ? -1 : a | b;
+    const int a = gdr_prep_wait_expired(), b = gdr_fwd_wait_expired(), c = gdr_bwd_wait_expired();
+    return a < 0 || b < 0 || c < 0 ? -1 : a | b | c;
 }
 
 }  // namespace cc1d
@@ -98,6 +99,32 @@ int cc1d_gdr_fwd(const cc1d_gdr_params *p, cc1d_stream_t stream) {
     const size_t need = gdr_fwd_workspace_bytes(*p);
     if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need || !is_aligned16(p->workspace))) return CC1D_ERR_WORKSPACE;
     return launch_gdr_fwd(*p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t cc1d_gdr_bwd_workspace_bytes(const cc1d_gdr_bwd_params *p) {
+    if (p == nullptr || check_whole(p->fwd) != CC1D_OK) return 0;
+    return gdr_bwd_workspace_bytes(*p);
+}
+
+int cc1d_gdr_bwd(const cc1d_gdr_bwd_params *p, cc1d_stream_t stream) {
+    if (p == nullptr) return CC1D_ERR_NULL;
+    const cc1d_gdr_params &f = p->fwd;
+    int rc = check_whole(f);
+    if (rc != CC1D_OK) return rc;
+    if (f.seqlen == 0 || f.batch == 0) {
+        if (gdr_sequences(f) == 0 || p->dinitial_states == nullptr) return CC1D_OK;
+    } else {
+        if (f.q == nullptr || f.k == nullptr || f.v == nullptr || f.g == nullptr || f.beta == nullptr || p->dout == nullptr || p->dq == nullptr ||
+            p->dk == nullptr || p->dv == nullptr || p->dg == nullptr || p->dbeta == nullptr) return CC1D_ERR_NULL;
+        if (!elem_aligned(f.g, f.gtype) || !elem_aligned(f.beta, f.btype) || !elem_aligned(p->dg, f.gtype) || !elem_aligned(p->dbeta, f.btype)) return CC1D_ERR_ALIGN;
+        rc = check_rows(f);
+        if (rc != CC1D_OK) return rc;
+        if (!rows_aligned(p->dout, p->dout_batch_stride, p->dout_l_stride, p->dout_h_stride, f.batch, f.seqlen, f.heads_v, f.itype) ||
+            !is_aligned16(p->dq) || !is_aligned16(p->dk) || !is_aligned16(p->dv)) return CC1D_ERR_ALIGN;
+    }
+    const size_t need = gdr_bwd_workspace_bytes(*p);
+    if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need || !is_aligned16(p->workspace))) return CC1D_ERR_WORKSPACE;
+    return launch_gdr_bwd(*p, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

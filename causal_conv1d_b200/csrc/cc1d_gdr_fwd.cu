@@ -29,8 +29,9 @@ template <typename T> struct Fwd {
 // rows) in tensor memory and the right one (K, Q, T, P) in shared memory, so nothing that the walk
 // computes passes through shared memory.  S itself is kept and decayed in fp32 registers; only
 // its pieces are rewritten every chunk.
-template <typename T, int kSteps>
-__global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_constant__ cc1d_gdr_params p, const unsigned char *images) {
+// kKeep: the backward's walk, which leaves S and U of every chunk in its record instead of an output.
+template <typename T, int kSteps, bool kKeep>
+__global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_constant__ cc1d_gdr_params p, const unsigned char *images, GdrRecord *records) {
     using L = Fwd<T>;
     using St = GdrStage<T>;
     constexpr int NP = St::kPieces, PO = St::kOut;
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
                 }
                 mma_commit(bar_x);
                 #pragma unroll
-                for (int a = 0; a < PO; ++a) {
+                for (int a = 0; a < (kKeep ? 0 : PO); ++a) {
                     #pragma unroll
                     for (int b = 0; b < NP && a + b < PO; ++b) {
                         #pragma unroll
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
                 }
                 mma_commit(bar_d);
                 #pragma unroll
-                for (int a = 0; a < PO; ++a) {
+                for (int a = 0; a < (kKeep ? 0 : PO); ++a) {
                     #pragma unroll
                     for (int b = 0; a + b < PO; ++b) {
                         #pragma unroll
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
             gdr_wait(bar_out, c & 1, dead);
             __syncwarp();
             const int rows = min(kChunk, seq.end - seq.begin - c * kChunk);
-            if (at < dv) {
+            if (!kKeep && at < dv) {
                 #pragma unroll 8
                 for (int i = lane / kLanes; i < rows; i += kRows) {
                     const uint4 v = *reinterpret_cast<const uint4 *>(V + (i * kGdrMaxDim + at) * sizeof(T));
@@ -182,7 +183,12 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
+        GdrRecord *record = kKeep ? records + gdr_first_slot(p, seq, n) * heads + h : nullptr;
         auto put_state = [&]() {
+            if (kKeep) {
+                #pragma unroll
+                for (int j = 0; j < 32; ++j) record->S0[32 * part + j][col] = S[j];
+            }
             #pragma unroll
             for (int b = 0; b < 4; ++b) split8_to_tmem<3>(S + 8 * b, mine + kColS + 16 * part + 4 * b, 64, 128);
             ready(bar_s);
@@ -235,8 +241,14 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
                     const float2 v = add2(make_float2(x[j], x[j + 1]), make_float2(R[j], R[j + 1]));
                     x[j] = v.x; x[j + 1] = v.y;
                 }
-                #pragma unroll
-                for (int j = 0; j < 16; j += 8) split8_to_tmem<PO>(x + j, mine + kColU + first / 2 + j / 2, 32, 480 - kColU);
+                if (kKeep) {
+                    #pragma unroll
+                    for (int j = 0; j < 16; ++j) record->U[first + j][col] = x[j];
+                    record += heads;
+                } else {
+                    #pragma unroll
+                    for (int j = 0; j < 16; j += 8) split8_to_tmem<PO>(x + j, mine + kColU + first / 2 + j / 2, 32, 480 - kColU);
+                }
                 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
                     const float4 f = *reinterpret_cast<const float4 *>(gates.to_end + first + j);
@@ -262,23 +274,25 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
                 }
             }
             // the output is taken out of tensor memory before the next chunk's products go there
-            gdr_wait(bar_o, par, dead);
-            __syncwarp();
-            fence_after_sync();
-            #pragma unroll
-            for (int b = 0; b < 16; b += 8) {
-                float x[8], y[8];
-                tmem_ld<8>(x, mine + kColO + first + b);
-                tmem_ld<8>(y, mine + kColX + first + b);
-                tmem_wait_ld();
+            if (!kKeep) {
+                gdr_wait(bar_o, par, dead);
+                __syncwarp();
+                fence_after_sync();
                 #pragma unroll
-                for (int j = 0; j < 8; j += 4) {
-                    const float4 f = *reinterpret_cast<const float4 *>(gates.from_start + first + b + j);
-                    x[j] = fmaf(f.x, x[j], y[j]); x[j + 1] = fmaf(f.y, x[j + 1], y[j + 1]);
-                    x[j + 2] = fmaf(f.z, x[j + 2], y[j + 2]); x[j + 3] = fmaf(f.w, x[j + 3], y[j + 3]);
+                for (int b = 0; b < 16; b += 8) {
+                    float x[8], y[8];
+                    tmem_ld<8>(x, mine + kColO + first + b);
+                    tmem_ld<8>(y, mine + kColX + first + b);
+                    tmem_wait_ld();
+                    #pragma unroll
+                    for (int j = 0; j < 8; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(gates.from_start + first + b + j);
+                        x[j] = fmaf(f.x, x[j], y[j]); x[j + 1] = fmaf(f.y, x[j + 1], y[j + 1]);
+                        x[j + 2] = fmaf(f.z, x[j + 2], y[j + 2]); x[j + 3] = fmaf(f.w, x[j + 3], y[j + 3]);
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j) V[(b + j) * kGdrMaxDim] = Elem<T>::from_f(p.scale * x[j]);   // where this thread read its v
                 }
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) V[(b + j) * kGdrMaxDim] = Elem<T>::from_f(p.scale * x[j]);   // where this thread read its v
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_out);
@@ -287,13 +301,13 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
             fence_after_sync();
             if (c + 1 < chunks) put_state();
         }
-        if (p.final_states != nullptr && row >= 0) {
+        if (!kKeep && p.final_states != nullptr && row >= 0) {
             float *dst = p.final_states + row * p.final_states_batch_stride + h * p.final_states_h_stride + state_at;
             #pragma unroll
             for (int j = 0; j < 32; ++j) if (32 * part + j < dk && col < dv) dst[(int64_t)j * dv] = S[j];
         }
         // tokens that belong to no sequence
-        if (p.cu_seqlens != nullptr && n + 1 >= sequences) {
+        if (!kKeep && p.cu_seqlens != nullptr && n + 1 >= sequences) {
             for (int64_t t = seq.end + part; t < p.seqlen; t += 4)
                 if (col < dv) out[t * p.out_l_stride] = Elem<T>::from_f(0.f);
         }
@@ -307,19 +321,27 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
 
 size_t gdr_fwd_workspace_bytes(const cc1d_gdr_params &p) { return gdr_image_bytes(p); }
 
-int launch_gdr_fwd(const cc1d_gdr_params &p, cudaStream_t stream) {
+template <bool kKeep> static int launch_walk(const cc1d_gdr_params &p, const void *images, GdrRecord *records, cudaStream_t stream) {
     const int64_t sequences = gdr_sequences(p), ctas = (sequences > 0 ? sequences : 1) * p.heads_v;
     if (ctas >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
-    const int rc = launch_gdr_prep(p, p.workspace, stream);
-    if (rc != CC1D_OK) return rc;
     CC1D_DISPATCH_ITYPE(p.itype, {
         CC1D_DISPATCH_BOOL(p.dim_k <= 64, kNarrow, {
             constexpr int kSteps = kNarrow ? 4 : 8;     // contraction steps of 16 over dim_k
-            allow_dynamic_smem(reinterpret_cast<const void *>(gdr_fwd_kernel<T, kSteps>), Fwd<T>::kBytes);
-            launch_k(gdr_fwd_kernel<T, kSteps>, dim3((unsigned)ctas), dim3(kThreads), Fwd<T>::kBytes, stream, p, reinterpret_cast<const unsigned char *>(p.workspace));
+            allow_dynamic_smem(reinterpret_cast<const void *>(gdr_fwd_kernel<T, kSteps, kKeep>), Fwd<T>::kBytes);
+            launch_k(gdr_fwd_kernel<T, kSteps, kKeep>, dim3((unsigned)ctas), dim3(kThreads), Fwd<T>::kBytes, stream, p,
+                     reinterpret_cast<const unsigned char *>(images), records);
         });
     });
     return check_launch();
+}
+
+int launch_gdr_fwd(const cc1d_gdr_params &p, cudaStream_t stream) {
+    const int rc = launch_gdr_prep(p, p.workspace, stream);
+    return rc != CC1D_OK ? rc : launch_walk<false>(p, p.workspace, nullptr, stream);
+}
+
+int launch_gdr_keep(const cc1d_gdr_params &p, const void *images, GdrRecord *records, cudaStream_t stream) {
+    return launch_walk<true>(p, images, records, stream);
 }
 
 int gdr_fwd_wait_expired() { return read_and_clear_wait_expired(); }

@@ -234,6 +234,47 @@ __device__ __forceinline__ int64_t gdr_first_slot(const cc1d_gdr_params &p, cons
     return p.cu_seqlens != nullptr ? (int64_t)(seq.begin / kChunk) + n : n * ((p.seqlen + kChunk - 1) / kChunk);
 }
 
+// Sequence and place in it of a slot; false where the slot holds no chunk.
+__device__ __forceinline__ bool gdr_find_chunk(const cc1d_gdr_params &p, int64_t slot, int &n, GdrSeq &seq, int &c) {
+    n = 0;
+    if (p.cu_seqlens == nullptr) {
+        n = (int)(slot / ((p.seqlen + kChunk - 1) / kChunk));
+    } else {
+        int last = (int)p.nseq - 1;            // the last sequence whose first slot is not behind this one
+        while (n < last) {
+            const int mid = (n + last + 1) / 2;
+            if (gdr_first_slot(p, gdr_sequence(p, mid), mid) <= slot) n = mid; else last = mid - 1;
+        }
+    }
+    seq = gdr_sequence(p, n);
+    c = (int)(slot - gdr_first_slot(p, seq, n));
+    return c >= 0 && c < (seq.end - seq.begin + kChunk - 1) / kChunk;
+}
+
+// kN threads: rows t0 .. t0 + 63 of a tensor (those at or after `end` and columns at or after `cols` as
+// zeros) into a token tile, one piece `piece_bytes` behind the other.
+template <typename T, int NP, int kN>
+__device__ __forceinline__ void load_tile(uint32_t dst, uint32_t panel_bytes, uint32_t piece_bytes, const T *src, int64_t step, int t0, int end, int cols, int tid) {
+    const int row0 = tid >> 4, c8 = (tid & 15) * 8;
+    #pragma unroll 4
+    for (int i = 0; i < 1024 / kN; ++i) {
+        const int row = row0 + kN / 16 * i;
+        const int64_t t = t0 + row;
+        const bool ok = t < end && c8 < cols;
+        const uint32_t at = dst + tile_at(row, c8 / 8, panel_bytes);
+        const T *from = ok ? src + t * step + c8 : src;
+        if constexpr (NP == 1) {
+            copy16_async(at, from, ok);
+        } else {
+            uint4 r[sizeof(T) / 2], pieces[NP];
+            load_row<T>(from, ok, r);
+            row_pieces<T, NP>(r, pieces);
+            #pragma unroll
+            for (int k = 0; k < NP; ++k) sts128(at + k * piece_bytes, pieces[k]);
+        }
+    }
+}
+
 // kN threads bring rows of q and k (and v) into their tiles: one-piece types by asynchronous
 // copies, the others split on the way.  The caller waits for the copies and fences.
 template <typename T, int kN> struct GdrRows {
@@ -251,27 +292,8 @@ template <typename T, int kN> struct GdrRows {
         vp = reinterpret_cast<const T *>(v) + v_row;
     }
     __device__ __forceinline__ void load_kq(uint32_t stage, int t0, int tid) const {
-        const int row0 = tid >> 4, c8 = (tid & 15) * 8;
-        #pragma unroll 4
-        for (int i = 0; i < 1024 / kN; ++i) {
-            const int row = row0 + kN / 16 * i;
-            const int64_t t = t0 + row;
-            const bool ok = t < end && c8 < dk;
-            const uint32_t at = stage + S::kKq + tile_at(row, c8 / 8, S::kPanel);
-            const T *k_src = ok ? kp + t * k_step + c8 : kp, *q_src = ok ? qp + t * q_step + c8 : qp;
-            if constexpr (NP == 1) {
-                copy16_async(at, k_src, ok);
-                copy16_async(at + 64 * 128, q_src, ok);
-            } else {
-                uint4 kr[kVecs], qr[kVecs], kk[NP], qq[NP];
-                load_row<T>(k_src, ok, kr);
-                load_row<T>(q_src, ok, qr);
-                row_pieces<T, NP>(kr, kk);
-                row_pieces<T, NP>(qr, qq);
-                #pragma unroll
-                for (int k = 0; k < NP; ++k) { sts128(at + k * S::kKqPiece, kk[k]); sts128(at + k * S::kKqPiece + 64 * 128, qq[k]); }
-            }
-        }
+        load_tile<T, NP, kN>(stage + S::kKq, S::kPanel, S::kKqPiece, kp, k_step, t0, end, dk, tid);
+        load_tile<T, NP, kN>(stage + S::kKq + 64 * 128, S::kPanel, S::kKqPiece, qp, q_step, t0, end, dk, tid);
     }
     __device__ __forceinline__ void load_v(uint32_t stage, int t0, int tid) const {
         const int row0 = tid >> 4, c8 = (tid & 15) * 8;
@@ -310,6 +332,12 @@ __device__ __forceinline__ void feed_walk(const GdrRows<T, kFeeders> &rows, cons
     }
 }
 
+// What the backward keeps of a chunk and value head, all fp32 and padded to 128 columns: the state before
+// it, U, the gradient of the state behind it, and the gradient dB of R.
+struct GdrRecord {
+    float S0[kGdrMaxDim][kGdrMaxDim], U[kChunk][kGdrMaxDim], dS[kGdrMaxDim][kGdrMaxDim], dB[kChunk][kGdrMaxDim];
+};
+int launch_gdr_keep(const cc1d_gdr_params &p, const void *images, GdrRecord *records, cudaStream_t stream);   // forward walk: S0 and U
 size_t gdr_image_bytes(const cc1d_gdr_params &p);                     // of all chunks
 int launch_gdr_prep(const cc1d_gdr_params &p, void *images, cudaStream_t stream);
 

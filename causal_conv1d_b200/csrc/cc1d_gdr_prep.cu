@@ -239,23 +239,12 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
     uint32_t *slot_at = reinterpret_cast<uint32_t *>(smem + L::kBars + 12);
     const int tid = threadIdx.x, warp = __shfl_sync(kFullMask, tid >> 5, 0), lane = tid & 31;
     pdl_wait();
-    // the chunk: value head, sequence (the last one whose first slot is not behind this one), place in it
     const int heads = (int)p.heads_v, h = blockIdx.x % heads;
     const int64_t slot = blockIdx.x / heads;
-    int n = 0;
-    if (p.cu_seqlens == nullptr) {
-        n = (int)(slot / ((p.seqlen + kChunk - 1) / kChunk));
-    } else {
-        int last = (int)p.nseq - 1;
-        while (n < last) {
-            const int mid = (n + last + 1) / 2;
-            if (gdr_first_slot(p, gdr_sequence(p, mid), mid) <= slot) n = mid; else last = mid - 1;
-        }
-    }
-    const GdrSeq seq = gdr_sequence(p, n);
-    const int64_t c = slot - gdr_first_slot(p, seq, n);
-    if (c < 0 || c >= (seq.end - seq.begin + kChunk - 1) / kChunk) return;    // the whole CTA
-    const int t0 = seq.begin + (int)c * kChunk;
+    int n, c;
+    GdrSeq seq;
+    if (!gdr_find_chunk(p, slot, n, seq, c)) return;      // the whole CTA
+    const int t0 = seq.begin + c * kChunk;
 
     if (tid == 0) { mbar_init(bar, 1); *dead = 0; fence_mbar_init(); }
     if (warp == 0) {

@@ -17,6 +17,84 @@ from torch import Tensor
 from causal_conv1d_b200._ext import ext as _ext
 
 
+def _rows(t: Tensor) -> Tensor:
+    """t where the chunked kernels' 16-byte loads can read it, else a dense copy."""
+    step = 16 // t.element_size()
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n <= 1 or s % step == 0 for n, s in zip(t.shape[:-1], t.stride()))
+    return t if ok else t.contiguous()
+
+
+class GatedDeltaRuleFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, initial_state=None, return_final_state=False, cu_seqlens=None, scale=None):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        if initial_state is not None:
+            initial_state = initial_state.contiguous()
+        if cu_seqlens is not None:
+            cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        scale = q.shape[-1] ** -0.5 if scale is None else scale
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        final_state = None
+        if return_final_state:
+            n = q.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
+            final_state = torch.empty(n, v.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=v.device)
+        if initial_state is not None and final_state is not None and initial_state.shape[0] != final_state.shape[0]:
+            raise RuntimeError("initial_state must have one row per sequence")
+        _ext.gated_delta_rule_fwd(q, k, v, g, beta, cu_seqlens, initial_state, final_state, None, None, out, scale)
+        ctx.save_for_backward(q, k, v, g, beta, initial_state, cu_seqlens)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return (out, final_state) if return_final_state else out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dfinal_state=None):
+        q, k, v, g, beta, initial_state, cu_seqlens = ctx.saved_tensors
+        if dout is None:
+            dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
+        if dfinal_state is not None:
+            dfinal_state = dfinal_state.contiguous()
+        dq, dk, dv, dg, dbeta = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, g, beta))
+        dinitial_state = None
+        if initial_state is not None and ctx.needs_input_grad[5]:
+            dinitial_state = torch.empty(initial_state.shape, dtype=torch.float32, device=v.device)
+        _ext.gated_delta_rule_bwd(q, k, v, g, beta, cu_seqlens, initial_state, _rows(dout), dfinal_state,
+                                  dq, dk, dv, dg, dbeta, dinitial_state, ctx.scale)
+        return dq, dk, dv, dg, dbeta, dinitial_state, None, None, None
+
+
+def gated_delta_rule_fn(
+    q: Tensor,
+    k: Tensor,
+    v: Tensor,
+    g: Tensor,
+    beta: Tensor,
+    initial_state: Tensor | None = None,
+    return_final_state: bool = False,
+    cu_seqlens: Tensor | None = None,
+    scale: float | None = None,
+):
+    """
+    Whole sequences, with gradients for q, k, v, g, beta and initial_state.
+
+    q, k: (batch, seqlen, heads_k, dim_k), contiguous along dim_k (slices of a wider tensor are read in
+        place where their rows are 16-byte aligned)
+    v: (batch, seqlen, heads_v, dim_v), dtype of q (float32, float16 or bfloat16)
+    g, beta: (batch, seqlen, heads_v), float32, float16 or bfloat16; g is the logarithm of the decay
+        (-inf: the state is forgotten)
+    initial_state: (sequences, heads_v, dim_k, dim_v) float32; zeros when None
+    cu_seqlens: (nseq + 1,) int32: the one row of the batch holds nseq packed sequences, sequence s at
+        tokens cu_seqlens[s]:cu_seqlens[s+1]; tokens behind the last one have zero outputs and gradients
+    scale: factor of the output, dim_k ** -0.5 when None
+
+    out: (batch, seqlen, heads_v, dim_v); with return_final_state also (sequences, heads_v, dim_k, dim_v)
+
+    The backward computes the forward's states again; it needs about 230 KB of workspace for each 64
+    tokens of a value head while it runs. Sums are taken in a fixed order.
+    """
+    return GatedDeltaRuleFn.apply(q, k, v, g, beta, initial_state, return_final_state, cu_seqlens, scale)
+
+
 def gated_delta_rule_update(
     q: Tensor,
     k: Tensor,
@@ -50,13 +128,6 @@ def gated_delta_rule_update(
     _ext.gated_delta_rule_update(q, k, v, g, beta, state, state_indices, out,
                                  q.shape[-1] ** -0.5 if scale is None else scale)
     return out.squeeze(1) if squeeze else out
-
-
-def _rows(t: Tensor) -> Tensor:
-    """t where the chunked kernels' 16-byte loads can read it, else a dense copy."""
-    step = 16 // t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n <= 1 or s % step == 0 for n, s in zip(t.shape[:-1], t.stride()))
-    return t if ok else t.contiguous()
 
 
 def gated_delta_rule_varlen_fn(
