@@ -15,15 +15,16 @@ constexpr uint32_t kColS = 0;      // 3 x 64: pieces of dS^T; later in a chunk
 constexpr uint32_t kColDelta = 0;  //   128: E^T Q + F^T K
 constexpr uint32_t kColX = 192;    // 64: dS^T K^T, then dU^T (T - I)
 constexpr uint32_t kColA = 256;    // 64: dO^T P
-constexpr uint32_t kColF = 320;    // 2 x 32: pieces of dU^T, then 3 x 32: of F^T = (-beta e^G dB)^T
+constexpr uint32_t kColF = 320;    // 3 x 32: pieces of dU^T, then of F^T = (-beta e^G dB)^T
 constexpr uint32_t kColE = 416;    // 3 x 32: pieces of E^T = (scale e^G dO)^T
 
 template <typename T> struct Back {
-    using S = GdrStage<T>;
+    using S = GdrStage<T, true>;
     static constexpr int kStages = S::kPieces == 1 ? 2 : 1;
-    static constexpr uint32_t kDoPiece = 16384, kDo = S::kPieces * S::kKqPiece, kT = kDo + S::kPieces * kDoPiece, kP = kT + 2 * 8192,
-                              kGates = kP + S::kOut * 8192, kStage = kGates + 3072;
+    static constexpr uint32_t kDoPiece = 16384, kDo = S::kPieces * S::kKqPiece, kT = kDo + S::kPieces * kDoPiece, kGates = kT + (S::kGates - S::kT),
+                              kP = kT + (S::kP - S::kT), kStage = kT + S::kImage;
     static constexpr uint32_t kBars = kStages * kStage, kBytes = kBars + 128 + 1024;
+    static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
 
 // One CTA walks one sequence of one value head from its end, with dS^T (dim_v x dim_k) in registers:
@@ -34,8 +35,8 @@ template <typename T> struct Back {
 template <typename T, int kSteps>
 __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, GdrRecord *records) {
     using L = Back<T>;
-    using St = GdrStage<T>;
-    constexpr int NP = St::kPieces, PO = St::kOut;
+    using St = GdrStage<T, true>;
+    constexpr int NP = St::kPieces, PO = St::kOut, PT = St::kSolve;
     const cc1d_gdr_params &p = b.fwd;
     extern __shared__ unsigned char raw[];
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -79,22 +80,28 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
             __syncwarp();
             if (elect_one()) {
                 fence_after_sync();
+                bool more = false;
                 #pragma unroll
-                for (int x = 0; x < 3; ++x) {          // dS^T K^T
+                for (int o = 2; o >= 0; --o) {          // dS^T K^T
                     #pragma unroll
-                    for (int y = 0; y < NP && x + y < 3; ++y) {
+                    for (int x = 0; x <= o; ++x) {
+                        const int y = o - x;
+                        if (x >= 3 || y >= NP) continue;
                         #pragma unroll
                         for (int k = 0; k < kSteps; ++k)
-                            mma_ts(kColX, kColS + 64 * x + 8 * k, desc_add(kq, y * St::kKqPiece + (k >> 2) * St::kPanel + (k & 3) * 32), id, x + y + k > 0);
+                            mma_ts(kColX, kColS + 64 * x + 8 * k, desc_add(kq, y * St::kKqPiece + (k >> 2) * St::kPanel + (k & 3) * 32), id, again(more));
                     }
                 }
+                more = false;
                 #pragma unroll
-                for (int x = 0; x < NP; ++x) {         // dO^T P, both with the tokens as the slow index
+                for (int o = PO - 1; o >= 0; --o) {         // dO^T P, both with the tokens as the slow index
                     #pragma unroll
-                    for (int y = 0; y < PO && x + y < PO; ++y) {
+                    for (int x = 0; x <= o; ++x) {
+                        const int y = o - x;
+                        if (x >= NP || y >= PO) continue;
                         #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_ss(kColA, desc_add(dout, x * L::kDoPiece + 2048 * k), desc_add(kq, L::kP + y * 8192 + 2048 * k), id_mm, x + y + k > 0);
+                            mma_ss(kColA, desc_add(dout, x * L::kDoPiece + 2048 * k), desc_add(kq, L::kP + y * 8192 + 2048 * k), id_mm, again(more));
                     }
                 }
                 mma_commit(bar_x);
@@ -105,12 +112,15 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
             __syncwarp();
             if (elect_one()) {
                 fence_after_sync();
+                bool more = false;
                 #pragma unroll
-                for (int x = 0; x < 3; ++x) {          // E^T Q
+                for (int o = 2; o >= 0; --o) {          // E^T Q
                     #pragma unroll
-                    for (int y = 0; y < NP && x + y < 3; ++y) {
+                    for (int x = 0; x <= o; ++x) {
+                        const int y = o - x;
+                        if (x >= 3 || y >= NP) continue;
                         #pragma unroll
-                        for (int k = 0; k < 4; ++k) mma_ts(kColDelta, kColE + 32 * x + 8 * k, desc_add(kmn, y * St::kKqPiece + 64 * 128 + 2048 * k), idd, x + y + k > 0);
+                        for (int k = 0; k < 4; ++k) mma_ts(kColDelta, kColE + 32 * x + 8 * k, desc_add(kmn, y * St::kKqPiece + 64 * 128 + 2048 * k), idd, again(more));
                     }
                 }
             }
@@ -119,12 +129,15 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
             __syncwarp();
             if (elect_one()) {
                 fence_after_sync();
+                bool more = false;
                 #pragma unroll
-                for (int x = 0; x < 2; ++x) {          // dU^T (T - I)
+                for (int o = PT - 1; o >= 0; --o) {         // dU^T (T - I)
                     #pragma unroll
-                    for (int y = 0; x + y < 2; ++y) {
+                    for (int x = 0; x <= o; ++x) {
+                        const int y = o - x;
+                        if (x >= PT || y >= PT) continue;
                         #pragma unroll
-                        for (int k = 0; k < 4; ++k) mma_ts(kColX, kColF + 32 * x + 8 * k, desc_add(kq, L::kT + y * 8192 + 2048 * k), id_mn, x + y + k > 0);
+                        for (int k = 0; k < 4; ++k) mma_ts(kColX, kColF + 32 * x + 8 * k, desc_add(kq, L::kT + y * 8192 + 2048 * k), id_mn, again(more));
                     }
                 }
                 mma_commit(bar_u);
@@ -135,9 +148,11 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
             if (elect_one()) {
                 fence_after_sync();
                 #pragma unroll
-                for (int x = 0; x < 3; ++x) {          // + F^T K
+                for (int o = 2; o >= 0; --o) {          // + F^T K
                     #pragma unroll
-                    for (int y = 0; y < NP && x + y < 3; ++y) {
+                    for (int x = 0; x <= o; ++x) {
+                        const int y = o - x;
+                        if (x >= 3 || y >= NP) continue;
                         #pragma unroll
                         for (int k = 0; k < 4; ++k) mma_ts(kColDelta, kColF + 32 * x + 8 * k, desc_add(kmn, y * St::kKqPiece + 2048 * k), idd, true);
                     }
@@ -226,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
                     R[j + k] = fmaf(f.x, x[k], p.scale * y[k]); R[j + k + 1] = fmaf(f.y, x[k + 1], p.scale * y[k + 1]);
                     R[j + k + 2] = fmaf(f.z, x[k + 2], p.scale * y[k + 2]); R[j + k + 3] = fmaf(f.w, x[k + 3], p.scale * y[k + 3]);
                 }
-                split8_to_tmem<2>(R + j, mine + kColF + first / 2 + j / 2, 32, 64);
+                split8_to_tmem<PT>(R + j, mine + kColF + first / 2 + j / 2, 32, 64);
             }
             ready(bar_r);
             gdr_wait(bar_u, par, dead);
@@ -303,10 +318,13 @@ constexpr uint32_t kColQk = 192;   // 64: Q K^T | K K^T
 constexpr uint32_t kColU = 256;    // 128: - | U dS^T
 
 template <typename T> struct Grads {
-    using S = GdrStage<T>;
-    static constexpr int NP = S::kPieces, NB = S::kOut;
+    using S = GdrStage<T, true>;
+    static constexpr int NP = S::kPieces;
+    // three pieces in every type: the gradient of g, fp32 as a rule, is a difference of larger sums
+    static constexpr int NB = 3;
     static constexpr uint32_t kKq = 0, kA = NP * S::kKqPiece, kAPiece = 16384, kB = kA + NB * kAPiece, kBPiece = 192 * 128, kMPiece = 32768,
                               kGates = kB + NB * kBPiece, kDots = kGates + 3072, kBars = kDots + 3 * 4 * 128 * 4, kBytes = kBars + 64 + 1024;
+    static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
 
 // 8 fp32 values -> kPieces vectors of a tile
@@ -349,13 +367,14 @@ template <int kPieces> __device__ __forceinline__ void put1(float x, unsigned ch
 //   dQ = scale e^G dO S0^T + M_P K
 //   dK = -beta e^G dB S0^T + e^{G_C - G} U dS^T + M_P^T Q + (M_A + M_A^T) K
 //   dbeta = dB.V - e^G k.(dB S0^T) + sum_j t_ij,  t = dA (k_i.k_j) e^{Gi - Gj}
-//   dG = q.dQ - k.dK + 2 k.(-beta e^G dB S0^T) + 2 beta sum_j t_ij   (what q and k see of G they see
-//        through their own products), and at the chunk's end + sum k.(e^{G_C - G} U dS^T) + e^{G_C} <S0, dS>;
+//   dG = q.dQ - k.(M_P^T Q + (M_A + M_A^T) K) - beta e^G k.(dB S0^T) - k.(e^{G_C - G} U dS^T) + 2 beta sum_j t_ij
+//        (what q and k see of G they see through their own products; the sum over j of t_ij is k.(M_A K), which
+//        counts with the other sign), and at the chunk's end + sum k.(e^{G_C - G} U dS^T) + e^{G_C} <S0, dS>;
 //   dg is its sum from the chunk's end.
 template <typename T, int kSteps>
 __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, const GdrRecord *records) {
     using L = Grads<T>;
-    using S = GdrStage<T>;
+    using S = GdrStage<T, true>;
     constexpr int NP = L::NP, NB = L::NB;
     const cc1d_gdr_params &p = b.fwd;
     extern __shared__ unsigned char raw[];
@@ -437,25 +456,31 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
             if (warp == 0) {
                 if (elect_one()) {
                     fence_after_sync();
-                    constexpr uint32_t id = mma_desc(128, 192, false, false), idq = mma_desc(128, 64, false, false);
+                                        constexpr uint32_t id = mma_desc(128, 192, false, false), idq = mma_desc(128, 64, false, false);
                     const uint64_t a = smem_desc(base + L::kA), bb = smem_desc(base + L::kB), kq = smem_desc(base + L::kKq);
+                    bool more = q > 0;
                     #pragma unroll
-                    for (int m = 0; m < NB; ++m) {
+                    for (int o = NB - 1; o >= 0; --o) {
                         #pragma unroll
-                        for (int k = 0; m + k < NB; ++k) {
+                        for (int m = 0; m <= o; ++m) {
+                            const int k = o - m;
+                            if (m >= NB || k >= NB) continue;
                             #pragma unroll
-                            for (int s = 0; s < 4; ++s) mma_ss(kColG, desc_add(a, m * L::kAPiece + 32 * s), desc_add(bb, k * L::kBPiece + 32 * s), id, m + k + s > 0 || q > 0);
+                            for (int s = 0; s < 4; ++s) mma_ss(kColG, desc_add(a, m * L::kAPiece + 32 * s), desc_add(bb, k * L::kBPiece + 32 * s), id, again(more));
                         }
                     }
                     if (q == 0 && h == hk * group) {
+                        more = false;
                         #pragma unroll
-                        for (int m = 0; m < NP; ++m) {
+                        for (int o = 2; o >= 0; --o) {
                             #pragma unroll
-                            for (int k = 0; k < NP && m + k < 3; ++k) {
+                            for (int m = 0; m <= o; ++m) {
+                                const int k = o - m;
+                                if (m >= NP || k >= NP) continue;
                                 #pragma unroll
                                 for (int s = 0; s < kSteps; ++s) {
                                     const uint32_t off = (s >> 2) * S::kPanel + (s & 3) * 32;
-                                    mma_ss(kColQk, desc_add(kq, m * S::kKqPiece + off), desc_add(kq, k * S::kKqPiece + 64 * 128 + off), idq, m + k + s > 0);
+                                    mma_ss(kColQk, desc_add(kq, m * S::kKqPiece + off), desc_add(kq, k * S::kKqPiece + 64 * 128 + off), idq, again(more));
                                 }
                             }
                         }
@@ -477,15 +502,19 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
             if (warp == 0) {
                 if (elect_one()) {
                     fence_after_sync();
+                    bool more;
                     constexpr uint32_t id = mma_desc(128, 128, false, false);
                     // rows 64-191 of [S0; U]: the upper half of the result is U dS^T, the lower one is not used
                     const uint64_t u = smem_desc(base + L::kB + 64 * 128), d = smem_desc(base + L::kA);
+                    more = q > 0;
                     #pragma unroll
-                    for (int m = 0; m < NB; ++m) {
+                    for (int o = NB - 1; o >= 0; --o) {
                         #pragma unroll
-                        for (int k = 0; m + k < NB; ++k) {
+                        for (int m = 0; m <= o; ++m) {
+                            const int k = o - m;
+                            if (m >= NB || k >= NB) continue;
                             #pragma unroll
-                            for (int s = 0; s < 4; ++s) mma_ss(kColU, desc_add(u, m * L::kBPiece + 32 * s), desc_add(d, k * L::kAPiece + 32 * s), id, m + k + s > 0 || q > 0);
+                            for (int s = 0; s < 4; ++s) mma_ss(kColU, desc_add(u, m * L::kBPiece + 32 * s), desc_add(d, k * L::kAPiece + 32 * s), id, again(more));
                         }
                     }
                     mma_commit(bar);
@@ -597,15 +626,18 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
         if (warp == 0) {
             if (elect_one()) {
                 fence_after_sync();
-                constexpr uint32_t id = mma_desc(128, 128, false, true);
+                                constexpr uint32_t id = mma_desc(128, 128, false, true);
                 const uint64_t m0 = smem_desc(base + L::kA), qk = smem_desc(base + L::kKq, S::kPanel);
+                bool more = false;
                 #pragma unroll
-                for (int m = 0; m < NB; ++m) {
+                for (int o = NB - 1; o >= 0; --o) {
                     #pragma unroll
-                    for (int k = 0; k < NP && m + k < NB; ++k) {
+                    for (int m = 0; m <= o; ++m) {
+                        const int k = o - m;
+                        if (m >= NB || k >= NP) continue;
                         #pragma unroll
                         for (int s = 0; s < 8; ++s)
-                            mma_ss(kColG, desc_add(m0, m * L::kMPiece + (s >> 2) * 16384 + (s & 3) * 32), desc_add(qk, k * S::kKqPiece + 2048 * s), id, m + k + s > 0);
+                            mma_ss(kColG, desc_add(m0, m * L::kMPiece + (s >> 2) * 16384 + (s & 3) * 32), desc_add(qk, k * S::kKqPiece + 2048 * s), id, again(more));
                     }
                 }
                 mma_commit(bar);
@@ -622,9 +654,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
             own8(own, e);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] += mineq[8 * e + j];
-                dot = fmaf(own[j], x[j], dot);
-                total[8 * e + j] += x[j];
+                const float sum = x[j] + mineq[8 * e + j];
+                dot = fmaf(own[j], is_k ? x[j] : sum, dot);
+                total[8 * e + j] += sum;
             }
         }
         fence_before_sync();
@@ -637,12 +669,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
             #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int k = 2 * lane + e;
-                float qd = 0.f, kd = 0.f, g2 = 0.f, ts = 0.f;
+                float qd = 0.f, kd = 0.f, g2 = 0.f, ts = 0.f, uk = 0.f;
                 #pragma unroll
-                for (int w = 0; w < 4; ++w) { qd += dots[0][w][k]; kd += dots[0][w][64 + k]; g2 += dots[1][w][64 + k]; ts += dots[1][w][k]; u += dots[2][w][64 + k]; }
+                for (int w = 0; w < 4; ++w) { qd += dots[0][w][k]; kd += dots[0][w][64 + k]; g2 += dots[1][w][64 + k]; ts += dots[1][w][k]; uk += dots[2][w][64 + k]; }
+                u += uk;
                 const float seen = -gates.from_start[k] * g2;      // -e^G k.(dB S0^T)
                 db[e] = dots[2][1][k] + seen + ts;
-                d[e] = (qd - kd) + 2.f * gates.beta[k] * (seen + ts);
+                d[e] = (qd - kd) - uk + gates.beta[k] * (seen + 2.f * ts);
             }
             #pragma unroll
             for (int m = 16; m >= 1; m >>= 1) { u += __shfl_xor_sync(kFullMask, u, m); s += __shfl_xor_sync(kFullMask, s, m); }
@@ -677,7 +710,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
 
 }  // namespace
 
-static size_t images_bytes(const cc1d_gdr_params &p) { return (gdr_image_bytes(p) + 255) / 256 * 256; }
+static size_t images_bytes(const cc1d_gdr_params &p) { return (gdr_image_bytes(p, true) + 255) / 256 * 256; }
 
 size_t gdr_bwd_workspace_bytes(const cc1d_gdr_bwd_params &b) {
     return images_bytes(b.fwd) + (size_t)gdr_slots(b.fwd) * (size_t)b.fwd.heads_v * sizeof(GdrRecord);
@@ -687,7 +720,7 @@ int launch_gdr_bwd(const cc1d_gdr_bwd_params &b, cudaStream_t stream) {
     const cc1d_gdr_params &p = b.fwd;
     unsigned char *images = reinterpret_cast<unsigned char *>(b.workspace);
     GdrRecord *records = reinterpret_cast<GdrRecord *>(images + images_bytes(p));
-    int rc = launch_gdr_prep(p, images, stream);
+    int rc = launch_gdr_prep(p, true, images, stream);
     if (rc == CC1D_OK) rc = launch_gdr_keep(p, images, records, stream);
     if (rc != CC1D_OK) return rc;
     const int64_t sequences = gdr_sequences(p), walks = (sequences > 0 ? sequences : 1) * p.heads_v, chunks = gdr_slots(p) * p.heads_k;

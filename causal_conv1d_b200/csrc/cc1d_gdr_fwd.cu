@@ -10,13 +10,13 @@ constexpr int kWalkers = 512, kThreads = kWalkers + 64 + kFeeders;   // warps 0-
 constexpr uint32_t kColS = 0;      // 3 x 64: pieces of S^T, two dim_k per column; later in a chunk
 constexpr uint32_t kColDelta = 0;  //   128: U''^T K, and
 constexpr uint32_t kColU = 128;    //   2 x 32: pieces of U^T (the third, fp32 inputs only, at 480)
-constexpr uint32_t kColR = 192;    // 2 x 32: pieces of R^T, then 3 x 32: of U''^T
+constexpr uint32_t kColR = 192;    // 3 x 32: pieces of R^T, then of U''^T
 constexpr uint32_t kColX = 288;    // 64: S^T K^T, then R^T (T - I)^T, then U^T P^T
 constexpr uint32_t kColO = 352;    // 64: S^T Q^T
 __device__ __forceinline__ uint32_t col_u(int piece) { return piece < 2 ? kColU + 32 * piece : 480; }
 
-template <typename T> struct Fwd {
-    using S = GdrStage<T>;
+template <typename T, bool kKeep> struct Fwd {
+    using S = GdrStage<T, kKeep>;
     static constexpr int kStages = S::kPieces == 1 ? 2 : 1;
     static constexpr uint32_t kBars = kStages * S::kBytes, kBytes = kBars + 128 + 1024;
 };
@@ -32,9 +32,9 @@ template <typename T> struct Fwd {
 // kKeep: the backward's walk, which leaves S and U of every chunk in its record instead of an output.
 template <typename T, int kSteps, bool kKeep>
 __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_constant__ cc1d_gdr_params p, const unsigned char *images, GdrRecord *records) {
-    using L = Fwd<T>;
-    using St = GdrStage<T>;
-    constexpr int NP = St::kPieces, PO = St::kOut;
+    using L = Fwd<T, kKeep>;
+    using St = GdrStage<T, kKeep>;
+    constexpr int NP = St::kPieces, PO = GdrType<T>::kOutPieces, PT = St::kSolve;
     extern __shared__ unsigned char raw[];
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     const uint32_t bars = smem_u32(smem + L::kBars);
@@ -77,23 +77,29 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
             __syncwarp();
             if (elect_one()) {
                 fence_after_sync();
+                bool more = false;
                 #pragma unroll
-                for (int a = 0; a < 3; ++a) {
+                for (int o = 2; o >= 0; --o) {
                     #pragma unroll
-                    for (int b = 0; b < NP && a + b < 3; ++b) {
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= 3 || b >= NP) continue;
                         #pragma unroll
                         for (int i = 0; i < kSteps; ++i)
-                            mma_ts(kColX, kColS + 64 * a + 8 * i, desc_add(kq, b * St::kKqPiece + (i >> 2) * St::kPanel + (i & 3) * 32), id, a + b + i > 0);
+                            mma_ts(kColX, kColS + 64 * a + 8 * i, desc_add(kq, b * St::kKqPiece + (i >> 2) * St::kPanel + (i & 3) * 32), id, again(more));
                     }
                 }
                 mma_commit(bar_x);
+                more = false;
                 #pragma unroll
-                for (int a = 0; a < (kKeep ? 0 : PO); ++a) {
+                for (int o = kKeep ? -1 : PO - 1; o >= 0; --o) {
                     #pragma unroll
-                    for (int b = 0; b < NP && a + b < PO; ++b) {
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= PO || b >= NP) continue;
                         #pragma unroll
                         for (int i = 0; i < kSteps; ++i)
-                            mma_ts(kColO, kColS + 64 * a + 8 * i, desc_add(kq, b * St::kKqPiece + 64 * 128 + (i >> 2) * St::kPanel + (i & 3) * 32), id, a + b + i > 0);
+                            mma_ts(kColO, kColS + 64 * a + 8 * i, desc_add(kq, b * St::kKqPiece + 64 * 128 + (i >> 2) * St::kPanel + (i & 3) * 32), id, again(more));
                     }
                 }
             }
@@ -102,12 +108,15 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
             __syncwarp();
             if (elect_one()) {
                 fence_after_sync();
+                bool more = false;
                 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
+                for (int o = PT - 1; o >= 0; --o) {
                     #pragma unroll
-                    for (int b = 0; a + b < 2; ++b) {
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= PT || b >= PT) continue;
                         #pragma unroll
-                        for (int i = 0; i < 4; ++i) mma_ts(kColX, kColR + 32 * a + 8 * i, desc_add(kq, St::kT + b * 8192 + 32 * i), id, a + b + i > 0);
+                        for (int i = 0; i < 4; ++i) mma_ts(kColX, kColR + 32 * a + 8 * i, desc_add(kq, St::kT + b * 8192 + 32 * i), id, again(more));
                     }
                 }
                 mma_commit(bar_u);
@@ -117,21 +126,27 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
             __syncwarp();
             if (elect_one()) {
                 fence_after_sync();
+                bool more = false;
                 #pragma unroll
-                for (int a = 0; a < 3; ++a) {
+                for (int o = 2; o >= 0; --o) {
                     #pragma unroll
-                    for (int b = 0; b < NP && a + b < 3; ++b) {
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= 3 || b >= NP) continue;
                         #pragma unroll
-                        for (int i = 0; i < 4; ++i) mma_ts(kColDelta, kColR + 32 * a + 8 * i, desc_add(kmn, b * St::kKqPiece + 2048 * i), idd, a + b + i > 0);
+                        for (int i = 0; i < 4; ++i) mma_ts(kColDelta, kColR + 32 * a + 8 * i, desc_add(kmn, b * St::kKqPiece + 2048 * i), idd, again(more));
                     }
                 }
                 mma_commit(bar_d);
+                more = false;
                 #pragma unroll
-                for (int a = 0; a < (kKeep ? 0 : PO); ++a) {
+                for (int o = kKeep ? -1 : PO - 1; o >= 0; --o) {
                     #pragma unroll
-                    for (int b = 0; a + b < PO; ++b) {
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= PO || b >= PO) continue;
                         #pragma unroll
-                        for (int i = 0; i < 4; ++i) mma_ts(kColX, col_u(a) + 8 * i, desc_add(kq, St::kP + b * 8192 + 32 * i), id, a + b + i > 0);
+                        for (int i = 0; i < 4; ++i) mma_ts(kColX, col_u(a) + 8 * i, desc_add(kq, St::kP + b * 8192 + 32 * i), id, again(more));
                     }
                 }
                 mma_commit(bar_o);
@@ -162,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
     } else if (warp > kWalkers / 32) {
         const GdrRows<T, kFeeders> rows(p, seq, h, p.v, seq.row * p.v_batch_stride + h * p.v_h_stride, p.v_l_stride);
         const int64_t step = (int64_t)heads * St::kImage;
-        feed_walk<T, L::kStages, false>(rows, images + gdr_first_slot(p, seq, n) * step + h * (int64_t)St::kImage, step, smem_u32(smem), seq.begin, chunks,
+        feed_walk<T, L::kStages, kKeep>(rows, images + gdr_first_slot(p, seq, n) * step + h * (int64_t)St::kImage, step, smem_u32(smem), seq.begin, chunks,
                                         bar_full, bar_empty, dead, tid - kWalkers - 64);
     } else {
         const int quad = warp & 3, part = warp >> 2, col = quad * 32 + lane;   // part: a quarter of the dim_k and of the tokens
@@ -226,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
                     x[j + 2] = R[j + 2] = v.x; x[j + 3] = R[j + 3] = v.y;
                 }
                 #pragma unroll
-                for (int j = 0; j < 16; j += 8) split8_to_tmem<2>(x + j, mine + kColR + first / 2 + j / 2, 32, 64);
+                for (int j = 0; j < 16; j += 8) split8_to_tmem<PT>(x + j, mine + kColR + first / 2 + j / 2, 32, 64);
             }
             ready(bar_r);
             gdr_wait(bar_u, par, dead);
@@ -319,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_fwd_kernel(const __grid_const
 
 }  // namespace
 
-size_t gdr_fwd_workspace_bytes(const cc1d_gdr_params &p) { return gdr_image_bytes(p); }
+size_t gdr_fwd_workspace_bytes(const cc1d_gdr_params &p) { return gdr_image_bytes(p, false); }
 
 template <bool kKeep> static int launch_walk(const cc1d_gdr_params &p, const void *images, GdrRecord *records, cudaStream_t stream) {
     const int64_t sequences = gdr_sequences(p), ctas = (sequences > 0 ? sequences : 1) * p.heads_v;
@@ -327,8 +342,9 @@ template <bool kKeep> static int launch_walk(const cc1d_gdr_params &p, const voi
     CC1D_DISPATCH_ITYPE(p.itype, {
         CC1D_DISPATCH_BOOL(p.dim_k <= 64, kNarrow, {
             constexpr int kSteps = kNarrow ? 4 : 8;     // contraction steps of 16 over dim_k
-            allow_dynamic_smem(reinterpret_cast<const void *>(gdr_fwd_kernel<T, kSteps, kKeep>), Fwd<T>::kBytes);
-            launch_k(gdr_fwd_kernel<T, kSteps, kKeep>, dim3((unsigned)ctas), dim3(kThreads), Fwd<T>::kBytes, stream, p,
+            constexpr uint32_t kBytes = Fwd<T, kKeep>::kBytes;
+            allow_dynamic_smem(reinterpret_cast<const void *>(gdr_fwd_kernel<T, kSteps, kKeep>), kBytes);
+            launch_k(gdr_fwd_kernel<T, kSteps, kKeep>, dim3((unsigned)ctas), dim3(kThreads), kBytes, stream, p,
                      reinterpret_cast<const unsigned char *>(images), records);
         });
     });
@@ -336,7 +352,7 @@ template <bool kKeep> static int launch_walk(const cc1d_gdr_params &p, const voi
 }
 
 int launch_gdr_fwd(const cc1d_gdr_params &p, cudaStream_t stream) {
-    const int rc = launch_gdr_prep(p, p.workspace, stream);
+    const int rc = launch_gdr_prep(p, false, p.workspace, stream);
     return rc != CC1D_OK ? rc : launch_walk<false>(p, p.workspace, nullptr, stream);
 }
 

@@ -75,6 +75,15 @@ __device__ __forceinline__ bool elect_one() {
     return yes != 0;
 }
 
+// First product into an accumulator: false, and true from then on.  A sum over pieces starts with the
+// smallest products: the tensor core cuts its sums off at 24 bits, and so only the last, large ones
+// are cut at the size of the result.
+__device__ __forceinline__ bool again(bool &more) {
+    const bool was = more;
+    more = true;
+    return was;
+}
+
 // Bounded wait.  When one runs out (never expected) the flag of the translation unit is raised and
 // `dead` makes every later wait of the CTA return at once: the CTA then runs to its end on
 // incomplete data, releases its tensor memory and returns.
@@ -137,9 +146,11 @@ template <int kPieces> __device__ __forceinline__ void store_pieces8(const float
 }
 
 template <typename T> struct GdrType;
-template <> struct GdrType<__nv_bfloat16> { static constexpr int kPieces = 1, kOutPieces = 2; };
-template <> struct GdrType<__half> { static constexpr int kPieces = 2, kOutPieces = 2; };
-template <> struct GdrType<float> { static constexpr int kPieces = 3, kOutPieces = 3; };
+// kPieces: of the inputs; kOutPieces: of the factors of an output of this type; kSolve: of T - I and of what it is
+// multiplied with
+template <> struct GdrType<__nv_bfloat16> { static constexpr int kPieces = 1, kOutPieces = 2, kSolve = 2; };
+template <> struct GdrType<__half> { static constexpr int kPieces = 2, kOutPieces = 2, kSolve = 2; };
+template <> struct GdrType<float> { static constexpr int kPieces = 3, kOutPieces = 3, kSolve = 3; };
 
 // ---- operand tiles ------------------------------------------------------------------------------
 // Token tile of one piece: panels of 64 columns, a panel `rows` x 128 bytes in the 128-byte swizzle.
@@ -210,20 +221,21 @@ namespace cc1d {
 // What the walks over the chunks read of one chunk, as it lies in a stage of shared memory:
 //   K, Q   token tiles, rows 0-63 k, 64-127 q (kPieces pieces), loaded by the walk itself
 //   V      as it is, [64][128]                                                 "
-//   T - I  T = (I + A)^-1, A_ij = beta_i (k_i.k_j) e^{G_i - G_j} for j < i   (2 pieces, row i, column j)
-//   P      (q_i.k_j) e^{G_i - G_j} for j <= i                                (kOutPieces pieces)
+//   T - I  T = (I + A)^-1, A_ij = beta_i (k_i.k_j) e^{G_i - G_j} for j < i   (kSolve pieces, row i, column j)
 //   gates
+//   P      (q_i.k_j) e^{G_i - G_j} for j <= i    (kOut pieces; kBack: the backward's, where P also leads to fp32
+//          gradients, has all three)
 // T, P and the gates are one image in the workspace, made by gdr_prep_kernel for all chunks at
 // once (inside the walk their chain of short dependent steps, 13,000 cycles a chunk, held it up).
-// The product with T is taken as x + (T - I) x, x in fp32: two pieces of both then leave 2^-17 of
-// the correction alone, not of x.
-template <typename T> struct GdrStage {
-    static constexpr int kPieces = GdrType<T>::kPieces, kOut = GdrType<T>::kOutPieces;
+// The product with T is taken as x + (T - I) x, x in fp32: two pieces of both (16-bit types) then leave
+// 2^-17 of the correction alone, not of x.
+template <typename T, bool kBack> struct GdrStage {
+    static constexpr int kPieces = GdrType<T>::kPieces, kOut = kBack ? 3 : GdrType<T>::kOutPieces, kSolve = GdrType<T>::kSolve;
     static constexpr uint32_t kPanel = 128 * 128, kKqPiece = 2 * kPanel;     // panel: 128 rows x 64 columns
-    static constexpr uint32_t kKq = 0, kV = kPieces * kKqPiece, kT = kV + kChunk * kGdrMaxDim * sizeof(T), kP = kT + 2 * 8192,
-                              kGates = kP + kOut * 8192, kBytes = kGates + 3072, kImage = kBytes - kT;
+    static constexpr uint32_t kKq = 0, kV = kPieces * kKqPiece, kT = kV + kChunk * kGdrMaxDim * sizeof(T), kGates = kT + kSolve * 8192,
+                              kP = kGates + 4096, kBytes = kP + kOut * 8192, kImage = kBytes - kT;
 };
-static_assert(sizeof(GdrGates) <= 3072, "gates of a chunk");
+static_assert(sizeof(GdrGates) <= 3072, "gates of a chunk (4096 bytes of an image, for the alignment of P)");
 
 // Chunks of sequence n in the workspace: slots gdr_first_slot(n) .. ; the slots of different sequences
 // never meet (a sequence of L tokens takes ceil(L / 64) of the at least floor(L / 64) + 1 there are).
@@ -278,7 +290,7 @@ __device__ __forceinline__ void load_tile(uint32_t dst, uint32_t panel_bytes, ui
 // kN threads bring rows of q and k (and v) into their tiles: one-piece types by asynchronous
 // copies, the others split on the way.  The caller waits for the copies and fences.
 template <typename T, int kN> struct GdrRows {
-    using S = GdrStage<T>;
+    using S = GdrStage<T, false>;     // K, Q and V lie alike in both
     static constexpr int NP = S::kPieces, kVecs = sizeof(T) / 2;
     const T *kp, *qp, *vp;
     int64_t k_step, q_step, v_step;
@@ -310,19 +322,20 @@ template <typename T, int kN> struct GdrRows {
 };
 
 constexpr int kFeeders = 64;
-// The last two warps of a walk: chunk after chunk into the stages, forwards or (kBack) from the last to the first.
+// The last two warps of the forward walk: chunk after chunk into the stages.
 // bar_full counts the threads and the one that announces the image.
-template <typename T, int kStages, bool kBack>
+template <typename T, int kStages, bool kKeep>
 __device__ __forceinline__ void feed_walk(const GdrRows<T, kFeeders> &rows, const unsigned char *images, int64_t image_step, uint32_t smem, int begin, int chunks,
                                           uint32_t bar_full, uint32_t bar_empty, volatile int *dead, int tid) {
-    using S = GdrStage<T>;
-    for (int i = 0; i < chunks; ++i) {
-        const int s = i % kStages, c = kBack ? chunks - 1 - i : i;
+    using S = GdrStage<T, kKeep>;
+    constexpr uint32_t kBytes = kKeep ? S::kP - S::kT : S::kImage;      // what is kept needs no P
+    for (int c = 0; c < chunks; ++c) {
+        const int s = c % kStages;
         const uint32_t stage = smem + s * S::kBytes, full = bar_full + 8 * s;
-        gdr_wait(bar_empty + 8 * s, ((i / kStages) & 1) ^ 1, dead);
+        gdr_wait(bar_empty + 8 * s, ((c / kStages) & 1) ^ 1, dead);
         if (tid == 0) {
-            mbar_expect_tx(full, S::kImage);
-            bulk_load(stage + S::kT, images + c * image_step, S::kImage, full);
+            mbar_expect_tx(full, kBytes);
+            bulk_load(stage + S::kT, images + c * image_step, kBytes, full);
         }
         rows.load_kq(stage, begin + c * kChunk, tid);
         rows.load_v(stage, begin + c * kChunk, tid);
@@ -338,7 +351,7 @@ struct GdrRecord {
     float S0[kGdrMaxDim][kGdrMaxDim], U[kChunk][kGdrMaxDim], dS[kGdrMaxDim][kGdrMaxDim], dB[kChunk][kGdrMaxDim];
 };
 int launch_gdr_keep(const cc1d_gdr_params &p, const void *images, GdrRecord *records, cudaStream_t stream);   // forward walk: S0 and U
-size_t gdr_image_bytes(const cc1d_gdr_params &p);                     // of all chunks
-int launch_gdr_prep(const cc1d_gdr_params &p, void *images, cudaStream_t stream);
+size_t gdr_image_bytes(const cc1d_gdr_params &p, bool back);          // of all chunks
+int launch_gdr_prep(const cc1d_gdr_params &p, bool back, void *images, cudaStream_t stream);
 
 }  // namespace cc1d

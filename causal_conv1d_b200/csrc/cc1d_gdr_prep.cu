@@ -214,21 +214,21 @@ __device__ __forceinline__ void invert_unit_lower(float *a, int warp, int lane) 
 
 constexpr int kThreads = 128;
 
-template <typename T> struct Prep {
-    using S = GdrStage<T>;
-    // the tiles of P and T take the place of K and Q once their product is there
-    static constexpr uint32_t kInv = S::kPieces * S::kKqPiece, kGates = kInv + kChunk * kLd * 4, kBars = kGates + 3072, kBytes = kBars + 64 + 1024;
-    static_assert((2 + S::kOut) * 8192 <= kInv, "room for T and P");
+template <typename T, bool kBack> struct Prep {
+    using S = GdrStage<T, kBack>;
+    // the image takes the place of K and Q once their product is there; its gates lie beside them till then
+    static constexpr uint32_t kTiles = S::kPieces * S::kKqPiece, kImageTiles = S::kImage;
+    static constexpr uint32_t kInv = kTiles > kImageTiles ? kTiles : kImageTiles, kBars = kInv + kChunk * kLd * 4, kGates = kBars + 64, kBytes = kGates + 4096 + 1024;
 };
 
 // One CTA makes one chunk of one value head: K K^T and Q K^T by one MMA with the 128 rows [K; Q], then
 // warps 0, 1 the rows of A and warps 2, 3 those of P, the inverse, and the image out by one bulk copy.
 // A chain of short dependent steps: what fills the SM is that four CTAs (bf16) share it.
-template <typename T, int kSteps>
+template <typename T, int kSteps, bool kBack>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : sizeof(T) == 2 && GdrType<T>::kPieces == 1 ? 4 : 2)
 gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images) {
-    using S = GdrStage<T>;
-    using L = Prep<T>;
+    using S = GdrStage<T, kBack>;
+    using L = Prep<T, kBack>;
     constexpr int NP = S::kPieces;
     extern __shared__ unsigned char raw[];
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -261,19 +261,23 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
+            bool more;
     const uint32_t tmem = *slot_at;
     if (warp == 1) {
         if (elect_one()) {
             constexpr uint32_t id = mma_desc(128, 64, false, false);
             const uint64_t kq = smem_desc(base);
+            more = false;
             #pragma unroll
-            for (int a = 0; a < NP; ++a) {
+            for (int o = 2; o >= 0; --o) {
                 #pragma unroll
-                for (int b = 0; b < NP && a + b < 3; ++b) {
+                for (int a = 0; a <= o; ++a) {
+                    const int b = o - a;
+                    if (a >= NP || b >= NP) continue;
                     #pragma unroll
                     for (int s = 0; s < kSteps; ++s) {
                         const uint32_t off = (s >> 2) * S::kPanel + (s & 3) * 32;
-                        mma_ss(tmem, desc_add(kq, a * S::kKqPiece + off), desc_add(kq, b * S::kKqPiece + off), id, a + b + s > 0);
+                        mma_ss(tmem, desc_add(kq, a * S::kKqPiece + off), desc_add(kq, b * S::kKqPiece + off), id, again(more));
                     }
                 }
             }
@@ -327,7 +331,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
                     *reinterpret_cast<float4 *>(inv + i * kLd + j0 + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
             } else {
                 #pragma unroll
-                for (int j = 0; j < 16; j += 8) store_pieces8<S::kOut>(x + j, base + 2 * 8192 + tile_at(i, (j0 + j) / 8, 0));
+                for (int j = 0; j < 16; j += 8) store_pieces8<S::kOut>(x + j, base + (S::kP - S::kT) + tile_at(i, (j0 + j) / 8, 0));
             }
         }
     }
@@ -347,14 +351,15 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
         #pragma unroll
         for (int j = 0; j < 16; ++j) if (j0 + j == i) x[j] = 0.f;      // T - I
         #pragma unroll
-        for (int j = 0; j < 16; j += 8) store_pieces8<2>(x + j, base + tile_at(i, (j0 + j) / 8, 0));
+        for (int j = 0; j < 16; j += 8) store_pieces8<S::kSolve>(x + j, base + tile_at(i, (j0 + j) / 8, 0));
     }
     fence_proxy_async_smem();
     __syncthreads();
     if (tid == 0) {
         unsigned char *image = images + (slot * heads + h) * (int64_t)S::kImage;
-        bulk_store(image, base, (2 + S::kOut) * 8192);
-        bulk_store(image + (2 + S::kOut) * 8192, base + L::kGates, 3072);
+        bulk_store(image, base, S::kSolve * 8192);
+        bulk_store(image + S::kSolve * 8192, base + L::kGates, 4096);
+        bulk_store(image + (S::kP - S::kT), base + (S::kP - S::kT), S::kOut * 8192);
         bulk_commit();
         bulk_wait_read();
     }
@@ -362,21 +367,24 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
 
 }  // namespace
 
-size_t gdr_image_bytes(const cc1d_gdr_params &p) {
+size_t gdr_image_bytes(const cc1d_gdr_params &p, bool back) {
     size_t one = 0;
-    CC1D_DISPATCH_ITYPE(p.itype, { one = GdrStage<T>::kImage; });
+    CC1D_DISPATCH_ITYPE(p.itype, { one = back ? GdrStage<T, true>::kImage : GdrStage<T, false>::kImage; });
     return one * (size_t)gdr_slots(p) * (size_t)p.heads_v;
 }
 
-int launch_gdr_prep(const cc1d_gdr_params &p, void *images, cudaStream_t stream) {
+int launch_gdr_prep(const cc1d_gdr_params &p, bool back, void *images, cudaStream_t stream) {
     const int64_t ctas = gdr_slots(p) * p.heads_v;
     if (ctas == 0) return CC1D_OK;
     if (ctas >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
     CC1D_DISPATCH_ITYPE(p.itype, {
         CC1D_DISPATCH_BOOL(p.dim_k <= 64, kNarrow, {
-            constexpr int kSteps = kNarrow ? 4 : 8;     // contraction steps of 16 over dim_k
-            allow_dynamic_smem(reinterpret_cast<const void *>(gdr_prep_kernel<T, kSteps>), Prep<T>::kBytes);
-            launch_k(gdr_prep_kernel<T, kSteps>, dim3((unsigned)ctas), dim3(kThreads), Prep<T>::kBytes, stream, p, reinterpret_cast<unsigned char *>(images));
+            CC1D_DISPATCH_BOOL(back, kBack, {
+                constexpr int kSteps = kNarrow ? 4 : 8;     // contraction steps of 16 over dim_k
+                constexpr uint32_t kBytes = Prep<T, kBack>::kBytes;
+                allow_dynamic_smem(reinterpret_cast<const void *>(gdr_prep_kernel<T, kSteps, kBack>), kBytes);
+                launch_k(gdr_prep_kernel<T, kSteps, kBack>, dim3((unsigned)ctas), dim3(kThreads), kBytes, stream, p, reinterpret_cast<unsigned char *>(images));
+            });
         });
     });
     return check_launch();
