@@ -26,10 +26,10 @@ LIB_CC1D = os.path.join(PKG, "libcc1d.so")
 LIB_TORCH = os.path.join(PKG, "_cc1d_torch.so")
 
 CU_SOURCES = ["cc1d_api.cu", "cc1d_fwd.cu", "cc1d_bwd.cu", "cc1d_update.cu", "cc1d_varlen.cu",
-              "cc1d_prefill.cu", "cc1d_peer.cu", "cc1d_gdr_api.cu", "cc1d_gdr_update.cu",
+              "cc1d_prefill.cu", "cc1d_peer.cu", "cc1d_checkpoint.cu", "cc1d_gdr_api.cu", "cc1d_gdr_update.cu",
               "cc1d_gdr_prep.cu", "cc1d_gdr_fwd.cu",
               "cc1d_gdr_bwd.cu"]
-CU_HEADERS = ["cc1d_common.cuh", "cc1d_kernels.h", "cc1d_tma.cuh", os.path.join(INCLUDE, "cc1d.h")]
+CU_HEADERS = ["cc1d_common.cuh", "cc1d_checkpoint.cuh", os.path.join(INCLUDE, "cc1d_checkpoint.h"), "cc1d_kernels.h", "cc1d_tma.cuh", os.path.join(INCLUDE, "cc1d.h")]
 GDR_HEADERS = ["cc1d_gdr.cuh", "cc1d_gdr_mma.cuh", os.path.join(INCLUDE, "cc1d_gdr.h")]     # read by the cc1d_gdr_*.cu only
 
 NVCC_FLAGS = [
@@ -103,7 +103,7 @@ def build_kernels(force: bool = False, verbose: bool = False) -> str:
 def build_torch_ext(force: bool = False) -> str:
     """g++: csrc/causal_conv1d.cpp -> _cc1d_torch.so (pybind11 module linking libcc1d.so)."""
     src = os.path.join(CSRC, "causal_conv1d.cpp")
-    hdrs = [os.path.join(INCLUDE, h) for h in ("cc1d.h", "cc1d_gdr.h")]
+    hdrs = [os.path.join(INCLUDE, h) for h in ("cc1d.h", "cc1d_gdr.h", "cc1d_checkpoint.h")]
     if not (force or _newer([src, *hdrs, LIB_CC1D, __file__], LIB_TORCH)):
         return LIB_TORCH
     import sysconfig

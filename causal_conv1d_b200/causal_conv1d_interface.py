@@ -6,13 +6,16 @@ against, are re-exported from ``torch_reference``; the CUDA entry points never c
 import torch
 
 from causal_conv1d_b200.cpp_functions import (
+    causal_conv1d_bwd_e4m3_function,
     causal_conv1d_bwd_function,
+    causal_conv1d_fwd_e4m3_function,
     causal_conv1d_fwd_function,
     causal_conv1d_update_function,
 )
 from causal_conv1d_b200.torch_reference import causal_conv1d_ref, causal_conv1d_update_ref  # noqa: F401
 
 _ACTIVATIONS = (None, "silu", "swish")
+_CHECKPOINTS = (None, "e4m3")
 
 
 def _unit_inner_stride(t: torch.Tensor) -> bool:
@@ -22,9 +25,11 @@ def _unit_inner_stride(t: torch.Tensor) -> bool:
 class CausalConv1dFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias=None, seq_idx=None, initial_states=None, return_final_states=False,
-                final_states_out=None, activation=None):
+                final_states_out=None, activation=None, checkpoint=None):
         if activation not in _ACTIVATIONS:
             raise NotImplementedError("activation must be None, silu, or swish")
+        if checkpoint not in _CHECKPOINTS:
+            raise NotImplementedError("checkpoint must be None or e4m3")
         if not _unit_inner_stride(x):
             x = x.contiguous()
         if bias is not None:
@@ -46,8 +51,15 @@ class CausalConv1dFn(torch.autograd.Function):
         else:
             final_states_out = None
         ctx.activation = activation in ("silu", "swish")
-        out = causal_conv1d_fwd_function(x, weight, bias, seq_idx, initial_states, final_states_out, ctx.activation)
-        ctx.save_for_backward(x, weight, bias, seq_idx, initial_states)
+        ctx.checkpoint = checkpoint
+        if checkpoint is None:
+            out = causal_conv1d_fwd_function(x, weight, bias, seq_idx, initial_states, final_states_out, ctx.activation)
+            ctx.save_for_backward(x, weight, bias, seq_idx, initial_states)
+        else:
+            out, codes, scales = causal_conv1d_fwd_e4m3_function(
+                x, weight, bias, seq_idx, initial_states, final_states_out, ctx.activation)
+            ctx.save_for_backward(codes, weight, bias, seq_idx, initial_states, scales)
+            ctx.x_dtype, ctx.x_channel_last = x.dtype, x.stride(1) == 1 and x.stride(2) > 1
         ctx.return_final_states = return_final_states
         ctx.return_dinitial_states = initial_states is not None and initial_states.requires_grad
         if return_final_states:
@@ -56,14 +68,20 @@ class CausalConv1dFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, *args):
-        x, weight, bias, seq_idx, initial_states = ctx.saved_tensors
+        x, weight, bias, seq_idx, initial_states, *scales = ctx.saved_tensors
         dfinal_states = args[0] if ctx.return_final_states else None
         if not _unit_inner_stride(dout):
             dout = dout.contiguous()
-        dx, dweight, dbias, dinitial_states = causal_conv1d_bwd_function(
-            x, weight, bias, dout, seq_idx, initial_states, dfinal_states, None,
-            ctx.return_dinitial_states, ctx.activation,
-        )
+        if ctx.checkpoint is None:
+            dx, dweight, dbias, dinitial_states = causal_conv1d_bwd_function(
+                x, weight, bias, dout, seq_idx, initial_states, dfinal_states, None,
+                ctx.return_dinitial_states, ctx.activation,
+            )
+        else:
+            dx, dweight, dbias, dinitial_states = causal_conv1d_bwd_e4m3_function(
+                x, scales[0], ctx.x_dtype, ctx.x_channel_last, weight, bias, dout, seq_idx, initial_states,
+                dfinal_states, ctx.return_dinitial_states, ctx.activation,
+            )
         return (
             dx,
             dweight,
@@ -73,11 +91,12 @@ class CausalConv1dFn(torch.autograd.Function):
             None,
             None,
             None,
+            None,
         )
 
 
 def causal_conv1d_fn(x, weight, bias=None, seq_idx=None, initial_states=None, return_final_states=False,
-                     final_states_out=None, activation=None):
+                     final_states_out=None, activation=None, checkpoint=None):
     """
     x: (batch, dim, seqlen)
     weight: (dim, width)
@@ -86,11 +105,17 @@ def causal_conv1d_fn(x, weight, bias=None, seq_idx=None, initial_states=None, re
     initial_states: (batch, dim, width - 1)
     final_states_out: (batch, dim, width - 1), to be written to
     activation: either None or "silu" or "swish"
+    checkpoint: None, or "e4m3" (not in the reference's signature): keep x for the backward in 8
+        bits, with a power-of-two scale for each 32 neighbours along x's contiguous axis, instead of
+        x itself. The output is what it is without; the backward sees x rounded to 4 significant
+        bits (relative error at most 2^-4), which reaches dweight and, with an activation, dx and
+        dbias. Saves memory where nothing else keeps x; x in a group with an infinity or a NaN
+        comes back as NaN.
 
     out: (batch, dim, seqlen)
     """
     return CausalConv1dFn.apply(x, weight, bias, seq_idx, initial_states, return_final_states,
-                                final_states_out, activation)
+                                final_states_out, activation, checkpoint)
 
 
 def causal_conv1d_update(x, conv_state, weight, bias=None, activation=None, cache_seqlens=None,

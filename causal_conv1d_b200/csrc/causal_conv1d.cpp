@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "cc1d.h"
+#include "cc1d_checkpoint.h"
 #include "cc1d_gdr.h"
 
 namespace {
@@ -81,11 +82,24 @@ void check_state(const at::Tensor &t, const at::Tensor &x, const ConvDims &d, co
 
 bool channel_last(const at::Tensor &x) { return x.stride(1) == 1 && x.stride(2) > 1; }
 
+// x in 8 bits: codes dense in x's layout class, scales (batch, dim, ceil(seqlen / 32)) or (batch, seqlen, ceil(dim / 32))
+cc1d_codes code_tensors(const at::Tensor &codes, const OptTensor &scales_, const at::Tensor &like, const ConvDims &d, bool cl) {
+    TORCH_CHECK(scales_.has_value(), "codes need their scales");
+    const at::Tensor &scales = *scales_;
+    need_cuda(codes, "codes"); need_cuda(scales, "scales");
+    TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, "codes and scales must be uint8");
+    TORCH_CHECK(codes.device() == like.device() && scales.device() == like.device(), "codes and scales must be on the device of x");
+    if (cl) need_shape(codes, {d.batch, d.seqlen, d.dim}, "codes"); else need_shape(codes, {d.batch, d.dim, d.seqlen}, "codes");
+    if (cl) need_shape(scales, {d.batch, d.seqlen, (d.dim + 31) / 32}, "scales"); else need_shape(scales, {d.batch, d.dim, (d.seqlen + 31) / 32}, "scales");
+    TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous(), "codes and scales must be contiguous");
+    return {codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>()};
+}
+
 }  // namespace
 
 void causal_conv1d_fwd(const at::Tensor &x, const at::Tensor &weight, const OptTensor &bias_,
                        const OptTensor &seq_idx_, const OptTensor &initial_states_, at::Tensor &out,
-                       OptTensor &final_states_out_, bool silu_activation) {
+                       OptTensor &final_states_out_, bool silu_activation, const OptTensor &codes_, const OptTensor &scales_) {
     need_cuda(x, "x"); need_cuda(weight, "weight"); need_cuda(out, "out");
     const ConvDims d = conv_dims(x, weight);
     need_shape(out, {d.batch, d.dim, d.seqlen}, "out");
@@ -120,6 +134,11 @@ void causal_conv1d_fwd(const at::Tensor &x, const at::Tensor &weight, const OptT
         p.final_states_batch_stride = s.stride(0); p.final_states_c_stride = s.stride(1); p.final_states_l_stride = s.stride(2);
     }
     c10::cuda::CUDAGuard guard(x.device());
+    if (codes_.has_value()) {
+        const cc1d_codes kept = code_tensors(*codes_, scales_, x, d, cl);
+        raise_on(cc1d_fwd_e4m3(&p, &kept, at::cuda::getCurrentCUDAStream().stream()), "causal_conv1d_fwd");
+        return;
+    }
     raise_on(cc1d_fwd(&p, at::cuda::getCurrentCUDAStream().stream()), "causal_conv1d_fwd");
 }
 
@@ -128,7 +147,7 @@ void causal_conv1d_bwd(const at::Tensor &x, const at::Tensor &weight, const OptT
                        at::Tensor &dx, at::Tensor &dweight, OptTensor &dbias_, OptTensor &dinitial_states_,
                        bool silu_activation, bool accumulate, const std::vector<int64_t> &peer_ptrs, int64_t peer_rank,
                        int64_t peer_capacity, const OptTensor &peer_status_, int64_t peer_spin_limit, int64_t phase,
-                       const OptTensor &workspace_) {
+                       const OptTensor &workspace_, const OptTensor &codes_, const OptTensor &scales_) {
     need_cuda(x, "x"); need_cuda(weight, "weight"); need_cuda(dout, "dout"); need_cuda(dx, "dx"); need_cuda(dweight, "dweight");
     TORCH_CHECK(bias_.has_value() == dbias_.has_value(), "dbias must be given exactly when bias is");
     const ConvDims d = conv_dims(x, weight);
@@ -230,12 +249,21 @@ void causal_conv1d_bwd(const at::Tensor &x, const at::Tensor &weight, const OptT
         peers.spin_limit = (uint32_t)peer_spin_limit;
         p.peers = &peers;
     }
-    int rc = cc1d_bwd(&p, at::cuda::getCurrentCUDAStream().stream());
+    const auto run = [&]() {
+        const cc1d_stream_t stream = at::cuda::getCurrentCUDAStream().stream();
+        if (!codes_.has_value()) return cc1d_bwd(&p, stream);
+        const cc1d_codes kept = code_tensors(*codes_, scales_, x, d, cl);
+        at::Tensor restored;                       // room for x where the kernel does not read the codes themselves
+        const size_t bytes = cc1d_bwd_e4m3_restore_bytes(&p);
+        if (bytes > 0) restored = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+        return cc1d_bwd_e4m3(&p, &kept, bytes > 0 ? restored.data_ptr() : nullptr, stream);
+    };
+    int rc = run();
     if (dout_in_place && (rc == CC1D_ERR_STRIDE || rc == CC1D_ERR_ALIGN)) {
         // the library could not serve this dout where it lies (e.g. no tensor map for its strides): one copy
         dout_l = to_channel_last(dout);
         p.dout = dout_l.data_ptr(); p.dout_batch_stride = dout_l.stride(0); p.dout_c_stride = dout_l.stride(1); p.dout_l_stride = dout_l.stride(2);
-        rc = cc1d_bwd(&p, at::cuda::getCurrentCUDAStream().stream());
+        rc = run();
     }
     raise_on(rc, "causal_conv1d_bwd");
 }
@@ -593,14 +621,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gated_delta_rule_fwd", &gated_delta_rule_fwd, "Gated delta rule over whole sequences");
     m.def("gated_delta_rule_bwd", &gated_delta_rule_bwd, "Gradients of the gated delta rule");
     m.def("gated_delta_rule_update", &gated_delta_rule_update, "Gated delta rule decode step");
-    m.def("causal_conv1d_fwd", &causal_conv1d_fwd, "Causal conv1d forward");
+    m.def("causal_conv1d_fwd", &causal_conv1d_fwd, "Causal conv1d forward",
+          py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("seq_idx"), py::arg("initial_states"), py::arg("out"),
+          py::arg("final_states_out"), py::arg("silu_activation"), py::arg("codes") = py::none(), py::arg("scales") = py::none());
     m.def("causal_conv1d_bwd", &causal_conv1d_bwd, "Causal conv1d backward",
           py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("dout"), py::arg("seq_idx"),
           py::arg("initial_states"), py::arg("dfinal_states"), py::arg("dx"), py::arg("dweight"),
           py::arg("dbias"), py::arg("dinitial_states"), py::arg("silu_activation"),
           py::arg("accumulate") = true, py::arg("peer_ptrs") = std::vector<int64_t>(), py::arg("peer_rank") = 0,
           py::arg("peer_capacity") = 0, py::arg("peer_status") = py::none(), py::arg("peer_spin_limit") = 0,
-          py::arg("phase") = 0, py::arg("workspace") = py::none());
+          py::arg("phase") = 0, py::arg("workspace") = py::none(), py::arg("codes") = py::none(), py::arg("scales") = py::none());
     m.def("bwd_workspace_bytes", [](int64_t batch, int64_t dim, int64_t seqlen, int64_t width, int64_t elem_bytes, bool channel_last) {
         cc1d_bwd_params q = {};
         q.itype = elem_bytes == 4 ? CC1D_F32 : CC1D_BF16; q.wtype = CC1D_F32; q.width = (int32_t)width;

@@ -224,7 +224,10 @@ const char *cc1d_status_str(int status) {
     }
 }
 
-int cc1d_fwd(const cc1d_fwd_params *p, cc1d_stream_t stream) {
+}  // extern "C"
+
+// cc1d_fwd; channel-first rows that fwd_keeps_codes() also leave x in `codes`
+int cc1d::cc1d_fwd_keeping(const cc1d_fwd_params *p, const cc1d_codes *codes, cc1d_stream_t stream) {
     if (p == nullptr) return CC1D_ERR_NULL;
     bool cl = false;
     int rc = check_conv_common(p->itype, p->wtype, p->width, p->batch, p->dim, p->seqlen, p->x,
@@ -244,8 +247,12 @@ int cc1d_fwd(const cc1d_fwd_params *p, cc1d_stream_t stream) {
     cc1d_fwd_params q = *p;
     if (q.batch <= 1) q.x_batch_stride = q.out_batch_stride = q.initial_states_batch_stride = q.final_states_batch_stride = 0;
     if (q.width == 2) q.initial_states_l_stride = q.final_states_l_stride = 0;
-    return cl ? launch_fwd_channel_last(q, s) : launch_fwd_channel_first(q, s);
+    return cl ? launch_fwd_channel_last(q, s) : launch_fwd_channel_first(q, s, codes != nullptr && fwd_keeps_codes(q) ? codes : nullptr);
 }
+
+extern "C" {
+
+int cc1d_fwd(const cc1d_fwd_params *p, cc1d_stream_t stream) { return cc1d_fwd_keeping(p, nullptr, stream); }
 
 static int check_bwd(const cc1d_bwd_params *p, bool *cl) {
     if (p == nullptr) return CC1D_ERR_NULL;
@@ -297,7 +304,7 @@ size_t cc1d_bwd_workspace_bytes(const cc1d_bwd_params *p) {
 
 // Checked parameters -> launcher.  The launchers test the workspace against the partial rows of
 // the tiling they actually pick (CC1D_ERR_WORKSPACE when it is too small).
-static int run_bwd(const cc1d_bwd_params *p, bool cl, cc1d_stream_t stream) {
+static int run_bwd(const cc1d_bwd_params *p, bool cl, cc1d_stream_t stream, const cc1d_codes *codes = nullptr) {
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cc1d_bwd_params q = *p;
     if (q.batch <= 1) {
@@ -305,7 +312,7 @@ static int run_bwd(const cc1d_bwd_params *p, bool cl, cc1d_stream_t stream) {
         q.initial_states_batch_stride = q.dfinal_states_batch_stride = q.dinitial_states_batch_stride = 0;
     }
     if (q.width == 2) q.initial_states_l_stride = q.dfinal_states_l_stride = q.dinitial_states_l_stride = 0;
-    return cl ? launch_bwd_channel_last(q, s) : launch_bwd_channel_first(q, s);
+    return cl ? launch_bwd_channel_last(q, s) : launch_bwd_channel_first(q, s, codes);
 }
 
 int cc1d_bwd(const cc1d_bwd_params *p, cc1d_stream_t stream) {
@@ -317,6 +324,18 @@ int cc1d_bwd(const cc1d_bwd_params *p, cc1d_stream_t stream) {
 }
 
 }  // extern "C"
+
+int cc1d::cc1d_bwd_check(const cc1d_bwd_params *p) {
+    bool cl = false;
+    const int rc = check_bwd(p, &cl);
+    if (rc != CC1D_OK) return rc;
+    return p->workspace == nullptr || p->workspace_bytes < cc1d_bwd_workspace_bytes(p) ? CC1D_ERR_WORKSPACE : CC1D_OK;
+}
+
+int cc1d::cc1d_bwd_reading(const cc1d_bwd_params *p, const cc1d_codes *codes, cc1d_stream_t stream) {
+    const int rc = cc1d_bwd_check(p);
+    return rc != CC1D_OK ? rc : run_bwd(p, false, stream, codes);
+}
 
 // Scratch of cc1d_bwd_noalloc: part of the library image, so no allocation is ever needed.
 // In host code the name below is only a host-side stand-in for the symbol, not a device

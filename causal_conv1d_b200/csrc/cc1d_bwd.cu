@@ -11,6 +11,7 @@
 //
 // Replaces csrc/causal_conv1d_bwd.cu:53-259 (channel-first), :329-589 (channel-last) and
 // the deterministic-mode workspaces + ATen sums of csrc/causal_conv1d.cpp:388-462.
+#include "cc1d_checkpoint.cuh"
 #include "cc1d_common.cuh"
 #include "cc1d_kernels.h"
 #include "cc1d_tma.cuh"
@@ -188,6 +189,8 @@ struct BwdCfArgs {
     uint32_t dim, seqlen;
     int wtype;
     uint32_t vpr, gpr, gpu, upr, n_units;   // see FwdCfArgs
+    const uint8_t *codes, *scales;          // x in 8 bits (kCodes); x is then not read
+    uint32_t spr;
 };
 
 // g = dout * silu'(y) for one element, times ActGrad<kTanh>::kGScale; `v` is the pre-activation
@@ -511,17 +514,39 @@ template <int kSlots> struct WideGroup {
     uint32_t cz, cw;          // lane 31: the 4 elements of x before the group (zeros at the row start)
 };
 
+// x of a group in 8 bits: a lane's 16 elements are the 16 bytes in xa, to be expanded once they are used
+struct WideCodes {
+    const uint8_t *codes, *scales;   // of this row
+};
+template <typename T, int kSlots>
+__device__ __forceinline__ void wide_expand(WideGroup<kSlots> &r) {
+    #pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+        const uint4 v = r.xa[j];
+        const float s = scale_value(r.xb[j].x);
+        r.xa[j] = expand8<T>(make_uint2(v.x, v.y), s);
+        r.xb[j] = expand8<T>(make_uint2(v.z, v.w), s);
+    }
+    const uint2 t = expand4<T>(r.cz, scale_value(r.cw));
+    r.cz = t.x; r.cw = t.y;
+}
+
 // kWhole: every slot of the row is complete; otherwise seqlen is only a multiple of 16, a lane's 16
 // elements are either all inside the row or all past its end (then they read as zeros: g = 0 there).
-template <typename T, int kSlots, bool kWhole>
-__device__ __forceinline__ void wide_load(WideGroup<kSlots> &r, const T *__restrict__ xr, const T *__restrict__ dr,
+template <typename T, int kSlots, bool kWhole, bool kCodes>
+__device__ __forceinline__ void wide_load(WideGroup<kSlots> &r, const T *__restrict__ xr, const WideCodes &xc, const T *__restrict__ dr,
                                           uint32_t g, int lane, uint32_t L) {
     const uint32_t gs = g * (kSlots * kWideSlotElems);
     #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
         const uint32_t e = gs + j * kWideSlotElems + lane * 16;
         if (kWhole || e < L) {
-            ld_stream32(r.xa[j], r.xb[j], xr + e);
+            if constexpr (kCodes) {
+                r.xa[j] = ld_stream(xc.codes + e);
+                r.xb[j].x = __ldg(xc.scales + e / kCodeGroup);
+            } else {
+                ld_stream32(r.xa[j], r.xb[j], xr + e);
+            }
             ld_stream32(r.da[j], r.db[j], dr + e);
         } else {
             r.xa[j] = r.xb[j] = r.da[j] = r.db[j] = make_uint4(0, 0, 0, 0);
@@ -529,18 +554,24 @@ __device__ __forceinline__ void wide_load(WideGroup<kSlots> &r, const T *__restr
     }
     r.cz = 0; r.cw = 0;
     if (lane == 31 && g > 0) {
-        const uint2 t = *reinterpret_cast<const uint2 *>(xr + gs - 4);
-        r.cz = t.x; r.cw = t.y;
+        if constexpr (kCodes) {
+            r.cz = *reinterpret_cast<const uint32_t *>(xc.codes + gs - 4);
+            r.cw = __ldg(xc.scales + (gs - 4) / kCodeGroup);
+        } else {
+            const uint2 t = *reinterpret_cast<const uint2 *>(xr + gs - 4);
+            r.cz = t.x; r.cw = t.y;
+        }
     }
 }
 
-template <typename T, int W, bool kSilu, int kSlots, bool kWhole>
-__device__ __forceinline__ void wide_group(const WideGroup<kSlots> &r, const float (&wv)[W], const float (&wy)[W], float by,
+template <typename T, int W, bool kSilu, int kSlots, bool kWhole, bool kCodes>
+__device__ __forceinline__ void wide_group(WideGroup<kSlots> &r, const float (&wv)[W], const float (&wy)[W], float by,
                                            float (&gfirst)[W - 1], float2 (&dw2)[W], float2 &db2, T *__restrict__ dxr,
                                            uint32_t g, int lane, uint32_t L) {
     constexpr bool kTanh = kSilu && UseTanhSilu<T>::value;
     const int src_prev = (lane + 31) & 31, src_next = (lane + 1) & 31;
     const uint32_t gs = g * (kSlots * kWideSlotElems);
+    if constexpr (kCodes) wide_expand<T>(r);
     #pragma unroll
     for (int j = kSlots - 1; j >= 0; --j) {
         // left x halo of A: the previous lane's B tail; lane 0 gets what lane 31 holds of the slot before
@@ -592,7 +623,7 @@ __device__ __forceinline__ void wide_group(const WideGroup<kSlots> &r, const flo
     }
 }
 
-template <typename T, int W, bool kSilu, int kSlots, bool kPrefetch, bool kWhole>
+template <typename T, int W, bool kSilu, int kSlots, bool kPrefetch, bool kWhole, bool kCodes>
 __global__ void __launch_bounds__(CC1D_BWD_WIDE_THREADS, CC1D_BWD_WIDE_MINBLK) bwd_cf_wide_kernel(const BwdCfArgs a) {
     pdl_wait();
     static_assert(sizeof(T) == 2, "16-bit I/O only");
@@ -608,6 +639,7 @@ __global__ void __launch_bounds__(CC1D_BWD_WIDE_THREADS, CC1D_BWD_WIDE_MINBLK) b
         const uint32_t b = row / a.dim;
         const uint32_t c = row - b * a.dim;
         const T *__restrict__ xr = reinterpret_cast<const T *>(a.x) + b * a.x_bs + c * a.x_cs;
+        const WideCodes xc = {a.codes + (uint64_t)row * a.seqlen, a.scales + (uint64_t)row * a.spr};
         const T *__restrict__ dr = reinterpret_cast<const T *>(a.dout) + b * a.d_bs + c * a.d_cs;
         T *__restrict__ dxr = reinterpret_cast<T *>(a.dx) + b * a.o_bs + c * a.o_cs;
         const uint32_t g0 = seg * a.gpu;
@@ -618,7 +650,7 @@ __global__ void __launch_bounds__(CC1D_BWD_WIDE_THREADS, CC1D_BWD_WIDE_MINBLK) b
         constexpr int kStep = kPrefetch ? 1 : (CC1D_BWD_WIDE_STEP < kSlots ? CC1D_BWD_WIDE_STEP : kSlots);   // slots per load/compute step
         const uint32_t s0 = g0 * (kSlots / kStep), s1 = g1 * (kSlots / kStep);
         WideGroup<kStep> cur;
-        wide_load<T, kStep, kWhole>(cur, xr, dr, s1 - 1, lane, a.seqlen);
+        wide_load<T, kStep, kWhole, kCodes>(cur, xr, xc, dr, s1 - 1, lane, a.seqlen);
         // A warp cannot hold the next step's vectors in registers while it computes this one, so its loads
         // come after the arithmetic and would wait on DRAM; instead the step after the one being loaded is
         // asked into L2, where those loads then find it: one 128-byte line per lane, lanes 0-15 the 2 KB of
@@ -627,7 +659,11 @@ __global__ void __launch_bounds__(CC1D_BWD_WIDE_THREADS, CC1D_BWD_WIDE_MINBLK) b
             if (CC1D_BWD_WIDE_L2PF > 0 && !kPrefetch) {
                 static_assert(kPrefetch || kStep * kWideSlotElems * sizeof(T) == 16 * 128, "16 lines per tensor and step");
                 const uint32_t e = s * (kStep * kWideSlotElems) + (lane & 15) * 64;
-                const T *p = (lane < 16 ? xr : dr) + e;
+                const void *p = (lane < 16 ? xr : dr) + e;
+                if constexpr (kCodes) {
+                    // half as many lines of x, and the few scales with the first of them
+                    if (lane < 16) p = lane & 1 ? (lane == 1 ? xc.scales + e / kCodeGroup : xc.codes + e - 64) : xc.codes + e;
+                }
                 if (kWhole || e < a.seqlen) asm volatile("prefetch.global.L2 [%0];" :: "l"(p));
             }
         };
@@ -656,7 +692,10 @@ __global__ void __launch_bounds__(CC1D_BWD_WIDE_THREADS, CC1D_BWD_WIDE_MINBLK) b
         if (g1 < a.gpr) {   // warp-uniform
             const uint32_t en = g1 * kGroupElems;
             uint4 xlast = make_uint4(0, 0, 0, 0), xedge = make_uint4(0, 0, 0, 0);
-            if (kSilu) { xlast = ld_cached(xr + en - 8); xedge = ld_cached(xr + en); }
+            if constexpr (kSilu && kCodes) {
+                xlast = expand8<T>(*reinterpret_cast<const uint2 *>(xc.codes + en - 8), scale_value(__ldg(xc.scales + (en - 8) / kCodeGroup)));
+                xedge = expand8<T>(*reinterpret_cast<const uint2 *>(xc.codes + en), scale_value(__ldg(xc.scales + en / kCodeGroup)));
+            } else if (kSilu) { xlast = ld_cached(xr + en - 8); xedge = ld_cached(xr + en); }
             const uint4 dedge = ld_cached(dr + en);
             seed_right_halo<T, W, kSilu, kTanh>(xlast, xedge, dedge, wy, by, gfirst);
         }
@@ -665,20 +704,20 @@ __global__ void __launch_bounds__(CC1D_BWD_WIDE_THREADS, CC1D_BWD_WIDE_MINBLK) b
             WideGroup<kStep> nxt;
             uint32_t s = s1 - 1;
             while (true) {
-                if (s > s0) wide_load<T, kStep, kWhole>(nxt, xr, dr, s - 1, lane, a.seqlen);
-                wide_group<T, W, kSilu, kStep, kWhole>(cur, wv, wy, by, gfirst, dw2, db2, dxr, s, lane, a.seqlen);
+                if (s > s0) wide_load<T, kStep, kWhole, kCodes>(nxt, xr, xc, dr, s - 1, lane, a.seqlen);
+                wide_group<T, W, kSilu, kStep, kWhole, kCodes>(cur, wv, wy, by, gfirst, dw2, db2, dxr, s, lane, a.seqlen);
                 if (s == s0) break;
                 --s;
-                if (s > s0) wide_load<T, kStep, kWhole>(cur, xr, dr, s - 1, lane, a.seqlen);
-                wide_group<T, W, kSilu, kStep, kWhole>(nxt, wv, wy, by, gfirst, dw2, db2, dxr, s, lane, a.seqlen);
+                if (s > s0) wide_load<T, kStep, kWhole, kCodes>(cur, xr, xc, dr, s - 1, lane, a.seqlen);
+                wide_group<T, W, kSilu, kStep, kWhole, kCodes>(nxt, wv, wy, by, gfirst, dw2, db2, dxr, s, lane, a.seqlen);
                 if (s == s0) break;
                 --s;
             }
         } else {
             for (uint32_t s = s1 - 1;; --s) {
-                wide_group<T, W, kSilu, kStep, kWhole>(cur, wv, wy, by, gfirst, dw2, db2, dxr, s, lane, a.seqlen);
+                wide_group<T, W, kSilu, kStep, kWhole, kCodes>(cur, wv, wy, by, gfirst, dw2, db2, dxr, s, lane, a.seqlen);
                 if (s == s0) break;
-                wide_load<T, kStep, kWhole>(cur, xr, dr, s - 1, lane, a.seqlen);
+                wide_load<T, kStep, kWhole, kCodes>(cur, xr, xc, dr, s - 1, lane, a.seqlen);
                 if (s - 1 >= s0 + CC1D_BWD_WIDE_L2PF) prefetch_step(s - 1 - CC1D_BWD_WIDE_L2PF);
             }
         }
@@ -819,7 +858,21 @@ size_t bwd_workspace_bytes_channel_first(const cc1d_bwd_params &p) {
     return (size_t)(rows * upr * (uint64_t)(p.width + 1) * sizeof(float));
 }
 
-int launch_bwd_channel_first(const cc1d_bwd_params &p, cudaStream_t stream) {
+// 16-bit rows whose length is a multiple of 16 elements and whose starts are 32-byte aligned: 32 bytes per
+// lane (a lane's 16 elements are then never cut by the row end).  x's own address does not count when x is
+// in 8 bits: its rows lie dense.
+static bool bwd_wide(const cc1d_bwd_params &p, bool codes) {
+    const int64_t x_bs = p.batch > 1 && !codes ? p.x_batch_stride : 0, x_cs = p.dim > 1 && !codes ? p.x_c_stride : 0;
+    const int64_t d_bs = p.batch > 1 ? p.dout_batch_stride : 0, d_cs = p.dim > 1 ? p.dout_c_stride : 0;
+    const int64_t o_bs = p.batch > 1 ? p.dx_batch_stride : 0, o_cs = p.dim > 1 ? p.dx_c_stride : 0;
+    return CC1D_BWD_WIDE && kCfVecs % 2 == 0 && p.itype != CC1D_F32 && p.seqlen % 16 == 0 &&
+           (((codes ? 0 : reinterpret_cast<uintptr_t>(p.x)) | reinterpret_cast<uintptr_t>(p.dout) | reinterpret_cast<uintptr_t>(p.dx)) & 31u) == 0 &&
+           (x_bs | x_cs | d_bs | d_cs | o_bs | o_cs) % 16 == 0;
+}
+
+bool bwd_reads_codes(const cc1d_bwd_params &p) { return bwd_wide(p, true); }
+
+int launch_bwd_channel_first(const cc1d_bwd_params &p, cudaStream_t stream, const cc1d_codes *codes) {
     const uint64_t rows = (uint64_t)p.batch * (uint64_t)p.dim;
     if (p.seqlen >= (1ll << 31) - 4096 || p.dim >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
     const CfPlan pl = plan_channel_first(p);
@@ -836,32 +889,29 @@ int launch_bwd_channel_first(const cc1d_bwd_params &p, cudaStream_t stream) {
     a.dim = (uint32_t)p.dim; a.seqlen = (uint32_t)p.seqlen; a.wtype = p.wtype;
     a.vpr = (uint32_t)pl.vpr; a.gpr = (uint32_t)pl.gpr; a.gpu = (uint32_t)pl.gpu; a.upr = (uint32_t)pl.upr;
     a.n_units = (uint32_t)pl.n_units;
+    a.codes = codes != nullptr ? codes->codes : nullptr; a.scales = codes != nullptr ? codes->scales : nullptr;
+    a.spr = (uint32_t)((p.seqlen + kCodeGroup - 1) / kCodeGroup);
     if (rows > 0 && p.seqlen > 0 && p.phase != 2) {
         if (pl.vec) {
             const uint64_t ctas = (pl.n_units + 7) / 8;
             const bool full = p.seqlen % vec_elems(p.itype) == 0 && pl.vpr % kCfGroupVecs == 0;
-            // 16-bit rows whose length is a multiple of 16 elements and whose starts are 32-byte aligned: 32
-            // bytes per lane (a lane's 16 elements are then never cut by the row end)
-            const bool wide = CC1D_BWD_WIDE && kCfVecs % 2 == 0 && p.itype != CC1D_F32 && p.seqlen % 16 == 0 &&
-                              ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.dout) |
-                                reinterpret_cast<uintptr_t>(p.dx)) & 31u) == 0 &&
-                              (a.x_bs | a.x_cs | a.d_bs | a.d_cs | a.o_bs | a.o_cs) % 16 == 0;
+            const bool wide = bwd_wide(p, codes != nullptr);
             if (wide) {
                 const uint64_t wctas = (pl.n_units + CC1D_BWD_WIDE_THREADS / 32 - 1) / (CC1D_BWD_WIDE_THREADS / 32);
                 if (p.itype == CC1D_BF16) {
                     using T = __nv_bfloat16;
-                    CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(full, kWhole, {
-                        auto kernel = bwd_cf_wide_kernel<T, W, kSilu, kWideSlots, CC1D_BWD_WIDE_PREFETCH != 0, kWhole>;
+                    CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(full, kWhole, CC1D_DISPATCH_BOOL(codes != nullptr, kCodes, {
+                        auto kernel = bwd_cf_wide_kernel<T, W, kSilu, kWideSlots, CC1D_BWD_WIDE_PREFETCH != 0, kWhole, kCodes>;
                         launch_k(kernel, dim3(persistent_grid(kernel, CC1D_BWD_WIDE_THREADS, wctas, CC1D_BWD_WIDE_PERSISTENT != 0)),
                                  dim3(CC1D_BWD_WIDE_THREADS), 0, stream, a);
-                    });););
+                    }););););
                 } else {
                     using T = __half;
-                    CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(full, kWhole, {
-                        auto kernel = bwd_cf_wide_kernel<T, W, kSilu, kWideSlots, CC1D_BWD_WIDE_PREFETCH != 0, kWhole>;
+                    CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(full, kWhole, CC1D_DISPATCH_BOOL(codes != nullptr, kCodes, {
+                        auto kernel = bwd_cf_wide_kernel<T, W, kSilu, kWideSlots, CC1D_BWD_WIDE_PREFETCH != 0, kWhole, kCodes>;
                         launch_k(kernel, dim3(persistent_grid(kernel, CC1D_BWD_WIDE_THREADS, wctas, CC1D_BWD_WIDE_PERSISTENT != 0)),
                                  dim3(CC1D_BWD_WIDE_THREADS), 0, stream, a);
-                    });););
+                    }););););
                 }
             } else
             CC1D_DISPATCH_ITYPE(p.itype, CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu,

@@ -16,6 +16,7 @@
 //
 // Replaces csrc/causal_conv1d_fwd.cu:46-137 (channel-first) and :205-348 (channel-last)
 // of the reference.
+#include "cc1d_checkpoint.cuh"
 #include "cc1d_common.cuh"
 #include "cc1d_kernels.h"
 #include "cc1d_tma.cuh"
@@ -38,6 +39,8 @@ struct FwdCfArgs {
     uint32_t gpu;      // groups per warp unit
     uint32_t upr;      // warp units per row
     uint32_t n_units;  // rows * upr
+    uint8_t *codes, *scales;   // x kept in 8 bits beside the output (kCodes)
+    uint32_t spr;              // scales per row
 };
 
 // A warp unit is `gpu` consecutive groups of 32 * kVecs vectors of one row, walked front to
@@ -142,7 +145,7 @@ __device__ __forceinline__ void fwd_st32(void *p, const uint4 &a, const uint4 &b
 
 // kWhole: every slot of the row is complete; otherwise seqlen is only a multiple of 16 and a lane's 16
 // elements are either all inside the row or all past its end (nothing loaded, nothing stored).
-template <typename T, int W, bool kSilu, int kSlots, bool kWhole>
+template <typename T, int W, bool kSilu, int kSlots, bool kWhole, bool kCodes>
 __global__ void __launch_bounds__(CC1D_FWD_WIDE_THREADS, CC1D_FWD_WIDE_MINBLK) fwd_cf_wide_kernel(const FwdCfArgs a) {
     pdl_wait();
     static_assert(sizeof(T) == 2, "16-bit I/O only");
@@ -201,6 +204,26 @@ __global__ void __launch_bounds__(CC1D_FWD_WIDE_THREADS, CC1D_FWD_WIDE_MINBLK) f
                     for (int k = 0; k < W - 1; ++k) xx[k] = make_float2(p[4 - (W - 1) + k], af[8 - (W - 1) + k]);
                     #pragma unroll
                     for (int i = 0; i < 8; ++i) xx[W - 1 + i] = make_float2(af[i], bf[i]);
+                    if constexpr (kCodes) {
+                        // a group is this lane's 16 elements and its neighbour's
+                        float most = 0.f;
+                        #pragma unroll
+                        for (int i = 0; i < 8; ++i) most = max_abs(max_abs(most, af[i]), bf[i]);
+                        most = max_abs(most, __shfl_xor_sync(kFullMask, most, 1));
+                        const uint32_t s = code_scale(most), e = g * kGroupElems + j * kSlotElems + lane * 16;
+                        const float2 inv = splat2(scale_inverse(s));
+                        #pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            const float2 u = mul2(make_float2(af[i], af[i + 1]), inv), v = mul2(make_float2(bf[i], bf[i + 1]), inv);
+                            af[i] = u.x; af[i + 1] = u.y; bf[i] = v.x; bf[i + 1] = v.y;
+                        }
+                        if (kWhole || e < L) {
+                            st_stream(a.codes + (uint64_t)row * L + e,
+                                      make_uint4(to_codes(af[0], af[1], af[2], af[3]), to_codes(af[4], af[5], af[6], af[7]),
+                                                 to_codes(bf[0], bf[1], bf[2], bf[3]), to_codes(bf[4], bf[5], bf[6], bf[7])));
+                            if ((lane & 1) == 0) a.scales[(uint64_t)row * a.spr + e / kCodeGroup] = (uint8_t)s;
+                        }
+                    }
                 }
                 float o0[8], o1[8];
                 #pragma unroll
@@ -263,7 +286,17 @@ uint64_t groups_per_unit(uint64_t rows, uint64_t groups_per_row) {
     return gpu > 0 ? gpu : 1;
 }
 
-int launch_fwd_channel_first(const cc1d_fwd_params &p, cudaStream_t stream) {
+// 16-bit rows whose length is a multiple of 16 elements and whose starts are 32-byte aligned: a lane takes 32 bytes
+static bool fwd_wide(const cc1d_fwd_params &p) {
+    const int64_t x_bs = p.batch > 1 ? p.x_batch_stride : 0, x_cs = p.dim > 1 ? p.x_c_stride : 0;
+    const int64_t o_bs = p.batch > 1 ? p.out_batch_stride : 0, o_cs = p.dim > 1 ? p.out_c_stride : 0;
+    return CC1D_FWD_WIDE && kCfVecs % 2 == 0 && p.itype != CC1D_F32 && p.seqlen % 16 == 0 &&
+           ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.out)) & 31u) == 0 && (x_bs | x_cs | o_bs | o_cs) % 16 == 0;
+}
+
+bool fwd_keeps_codes(const cc1d_fwd_params &p) { return fwd_wide(p); }
+
+int launch_fwd_channel_first(const cc1d_fwd_params &p, cudaStream_t stream, const cc1d_codes *codes) {
     const int V = vec_elems(p.itype);
     const uint64_t rows = (uint64_t)p.batch * (uint64_t)p.dim;
     if (rows == 0 || p.seqlen == 0) return CC1D_OK;
@@ -275,6 +308,8 @@ int launch_fwd_channel_first(const cc1d_fwd_params &p, cudaStream_t stream) {
     a.o_bs = p.batch > 1 ? p.out_batch_stride : 0; a.o_cs = p.dim > 1 ? p.out_c_stride : 0;
     a.w_cs = p.weight_c_stride; a.w_ws = p.weight_width_stride;
     a.dim = (uint32_t)p.dim; a.seqlen = (uint32_t)p.seqlen; a.wtype = p.wtype;
+    a.codes = codes != nullptr ? codes->codes : nullptr; a.scales = codes != nullptr ? codes->scales : nullptr;
+    a.spr = (uint32_t)((p.seqlen + kCodeGroup - 1) / kCodeGroup);
 
     const bool vec_ok = is_aligned16(p.x) && is_aligned16(p.out) && a.x_bs % V == 0 && a.x_cs % V == 0 &&
                         a.o_bs % V == 0 && a.o_cs % V == 0;
@@ -290,21 +325,19 @@ int launch_fwd_channel_first(const cc1d_fwd_params &p, cudaStream_t stream) {
         a.n_units = (uint32_t)n_units;
         const uint64_t ctas = (n_units + 7) / 8;
         const bool full = p.seqlen % V == 0 && vpr % (32 * kVecs) == 0;
-        const bool wide = CC1D_FWD_WIDE && kCfVecs % 2 == 0 && p.itype != CC1D_F32 && p.seqlen % 16 == 0 &&
-                          ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.out)) & 31u) == 0 &&
-                          (a.x_bs | a.x_cs | a.o_bs | a.o_cs) % 16 == 0;
+        const bool wide = fwd_wide(p);
         if (wide) {
             const uint64_t wctas = (n_units + CC1D_FWD_WIDE_THREADS / 32 - 1) / (CC1D_FWD_WIDE_THREADS / 32);
             if (p.itype == CC1D_BF16) {
                 using T = __nv_bfloat16;
-                CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(full, kWhole, {
-                    launch_k(fwd_cf_wide_kernel<T, W, kSilu, kCfVecs / 2, kWhole>, dim3((unsigned)wctas), dim3(CC1D_FWD_WIDE_THREADS), 0, stream, a);
-                });););
+                CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(full, kWhole, CC1D_DISPATCH_BOOL(codes != nullptr, kCodes, {
+                    launch_k(fwd_cf_wide_kernel<T, W, kSilu, kCfVecs / 2, kWhole, kCodes>, dim3((unsigned)wctas), dim3(CC1D_FWD_WIDE_THREADS), 0, stream, a);
+                }););););
             } else {
                 using T = __half;
-                CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(full, kWhole, {
-                    launch_k(fwd_cf_wide_kernel<T, W, kSilu, kCfVecs / 2, kWhole>, dim3((unsigned)wctas), dim3(CC1D_FWD_WIDE_THREADS), 0, stream, a);
-                });););
+                CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(full, kWhole, CC1D_DISPATCH_BOOL(codes != nullptr, kCodes, {
+                    launch_k(fwd_cf_wide_kernel<T, W, kSilu, kCfVecs / 2, kWhole, kCodes>, dim3((unsigned)wctas), dim3(CC1D_FWD_WIDE_THREADS), 0, stream, a);
+                }););););
             }
         } else
         CC1D_DISPATCH_ITYPE(p.itype, CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu,

@@ -7,6 +7,7 @@
 #include <utility>
 
 #include "cc1d.h"
+#include "cc1d_checkpoint.h"
 
 // Compile-time tunables (overridable with -D for experiments).
 #ifndef CC1D_CF_KVECS
@@ -31,13 +32,20 @@ inline bool is_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p)
 inline int elem_size(int dtype) { return dtype == CC1D_F32 ? 4 : 2; }
 inline int vec_elems(int dtype) { return 16 / elem_size(dtype); }
 
+// The calls of include/cc1d.h with x kept in, or taken from, 8 bits (where the kernels can: see below)
+int cc1d_fwd_keeping(const cc1d_fwd_params *p, const cc1d_codes *codes, cc1d_stream_t stream);
+int cc1d_bwd_check(const cc1d_bwd_params *p);
+int cc1d_bwd_reading(const cc1d_bwd_params *p, const cc1d_codes *codes, cc1d_stream_t stream);
+
 uint64_t groups_per_unit(uint64_t rows, uint64_t groups_per_row);
-int launch_fwd_channel_first(const cc1d_fwd_params &p, cudaStream_t stream);
+int launch_fwd_channel_first(const cc1d_fwd_params &p, cudaStream_t stream, const cc1d_codes *codes = nullptr);   // codes: only where fwd_keeps_codes
+bool fwd_keeps_codes(const cc1d_fwd_params &p);     // channel-first rows whose kernel can keep x in 8 bits on its way
 int launch_fwd_channel_last(const cc1d_fwd_params &p, cudaStream_t stream);
 
 size_t bwd_workspace_bytes_channel_first(const cc1d_bwd_params &p);
 size_t bwd_workspace_bytes_channel_last(const cc1d_bwd_params &p);
-int launch_bwd_channel_first(const cc1d_bwd_params &p, cudaStream_t stream);
+int launch_bwd_channel_first(const cc1d_bwd_params &p, cudaStream_t stream, const cc1d_codes *codes = nullptr);   // codes: only where bwd_reads_codes
+bool bwd_reads_codes(const cc1d_bwd_params &p);     // ... and whose backward can read x in 8 bits
 int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream);
 
 size_t peer_allreduce_buffer_bytes(int world, int64_t count);
