@@ -21,7 +21,13 @@ __device__ __forceinline__ float gdr_exp(float x) {
     return fmaf(e, lo * kLn2, e);
 }
 
-__device__ __forceinline__ float load_any(const void *p, int64_t at, int dtype) { return load_w(p, at, dtype); }
+// A gate as it lies in memory, and its value: a conversion beside the load would wait for it
+__device__ __forceinline__ uint32_t load_bits(const void *p, int64_t at, int dtype) {
+    return dtype == CC1D_F32 ? __ldg(reinterpret_cast<const uint32_t *>(p) + at) : (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + at);
+}
+__device__ __forceinline__ float from_bits(uint32_t v, int dtype) {
+    return dtype == CC1D_F32 ? __uint_as_float(v) : dtype == CC1D_BF16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half((unsigned short)v));
+}
 
 __device__ __forceinline__ void store_any(void *p, int64_t at, int dtype, float v) {
     if (dtype == CC1D_F32) reinterpret_cast<float *>(p)[at] = v;

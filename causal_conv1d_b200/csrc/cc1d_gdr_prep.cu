@@ -8,13 +8,6 @@ namespace {
 // Gates of two tokens as they lie in memory, converted where they are used.
 struct GateRegs { uint32_t g[2], beta[2]; };
 struct GateSums { float4 G; float2 beta; };   // (high, low) of G and beta of two tokens
-__device__ __forceinline__ uint32_t load_bits(const void *p, int64_t at, int dtype) {
-    return dtype == CC1D_F32 ? __ldg(reinterpret_cast<const uint32_t *>(p) + at) : (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + at);
-}
-__device__ __forceinline__ float from_bits(uint32_t v, int dtype) {
-    return dtype == CC1D_F32 ? __uint_as_float(v) : dtype == CC1D_BF16 ? __uint_as_float(v << 16) : __half2float(__ushort_as_half((unsigned short)v));
-}
-
 // One warp: gates of tokens t0 .. t0 + 63 (those at or after `end` do not exist: g = beta = 0).
 __device__ __forceinline__ void load_gates(GateRegs &r, const cc1d_gdr_params &p, const GdrSeq &seq, int h, int t0, int lane) {
     const int64_t ga = seq.row * p.g_batch_stride + h * p.g_h_stride, ba = seq.row * p.beta_batch_stride + h * p.beta_h_stride;
