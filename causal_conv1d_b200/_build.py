@@ -30,7 +30,7 @@ CU_SOURCES = ["cc1d_api.cu", "cc1d_fwd.cu", "cc1d_bwd.cu", "cc1d_update.cu", "cc
               "cc1d_gdr_prep.cu", "cc1d_gdr_fwd.cu",
               "cc1d_gdr_bwd.cu"]
 CU_HEADERS = ["cc1d_common.cuh", "cc1d_checkpoint.cuh", os.path.join(INCLUDE, "cc1d_checkpoint.h"), "cc1d_kernels.h", "cc1d_tma.cuh", os.path.join(INCLUDE, "cc1d.h")]
-GDR_HEADERS = ["cc1d_gdr.cuh", "cc1d_gdr_mma.cuh", os.path.join(INCLUDE, "cc1d_gdr.h")]     # read by the cc1d_gdr_*.cu only
+GDR_HEADERS = ["cc1d_gdr.cuh", "cc1d_gdr_mma.cuh", "cc1d_gdr_walk.cuh", os.path.join(INCLUDE, "cc1d_gdr.h")]     # read by the cc1d_gdr_*.cu only
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,15 +1,17 @@
-// Gradients of the gated delta rule: cc1d_gdr_bwd (include/cc1d_gdr.h).  Four launches:
-//   gdr_prep_kernel        T, P and the gates of every chunk (as in the forward)
-//   gdr_fwd_kernel<kKeep>  the forward walk again; leaves the state before each chunk and U
-//   gdr_bwd_walk_kernel    the walk from the last chunk to the first; leaves the state's gradient and dB
-//   gdr_grads_kernel       all other gradients, every chunk by itself
-#include "cc1d_gdr_mma.cuh"
+// Gradients of the gated delta rule: cc1d_gdr_bwd (include/cc1d_gdr.h).  Three launches:
+//   gdr_prep_kernel       T, P and the gates of every chunk (as in the forward)
+//   gdr_bwd_walks_kernel  half of the CTAs walk forwards again and leave the state before each chunk and U, half
+//                         walk from the last chunk to the first and leave the state's gradient and dB (neither
+//                         needs the other: one after the other they took 287 + 312 us where 64 CTAs of each
+//                         fit the SMs together)
+//   gdr_grads_kernel      all other gradients, every chunk by itself
+#include "cc1d_gdr_walk.cuh"
 
 namespace cc1d {
 namespace {
 
 // ---- the walk backwards -------------------------------------------------------------------------
-constexpr int kWalkers = 512, kThreads = kWalkers + 32 + kFeeders;   // warps 0-15 walk, 16 issues their products, 17, 18 load
+// warps 0-15 walk, 16 issues their products, 17 does nothing, 18, 19 load
 
 constexpr uint32_t kColS = 0;      // 3 x 64: pieces of dS^T; later in a chunk
 constexpr uint32_t kColDelta = 0;  //   128: E^T Q + F^T K
@@ -33,7 +35,7 @@ template <typename T> struct Back {
 // Same division of work and same precision as the forward walk; P^T dO and Q^T E do not wait for the
 // walk and run beside its arithmetic.
 template <typename T, int kSteps>
-__global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, GdrRecord *records) {
+__device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const unsigned char *images, GdrRecord *records, int block) {
     using L = Back<T>;
     using St = GdrStage<T, true>;
     constexpr int NP = St::kPieces, PO = St::kOut, PT = St::kSolve;
@@ -59,7 +61,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
     __syncthreads();
     fence_after_sync();
 
-    const int heads = (int)p.heads_v, h = blockIdx.x % heads, n = blockIdx.x / heads;
+    const int heads = (int)p.heads_v, h = block % heads, n = block / heads;
     const int sequences = (int)gdr_sequences(p);
     GdrSeq seq = {0, 0, 0};
     if (n < sequences) seq = gdr_sequence(p, n);
@@ -161,8 +163,8 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
             }
             __syncwarp();
         }
-    } else if (warp > kWalkers / 32) {
-        const int ft = tid - kWalkers - 32;
+    } else if (warp > kWalkers / 32 + 1) {
+        const int ft = tid - kWalkers - 64;
         const T *dout = reinterpret_cast<const T *>(b.dout) + seq.row * b.dout_batch_stride + h * b.dout_h_stride;
         const GdrRows<T, kFeeders> rows(p, seq, h, dout, 0, b.dout_l_stride);
         const int64_t step = (int64_t)heads * St::kImage;
@@ -181,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
             fence_proxy_async_smem();
             mbar_arrive(full);
         }
-    } else {
+    } else if (warp < kWalkers / 32) {
         const int quad = warp & 3, part = warp >> 2, col = quad * 32 + lane;   // part: a quarter of the dim_k and of the tokens
         const uint32_t mine = (uint32_t)(quad * 32) << 16;
         const int64_t state_at = ((int64_t)n * heads + h) * dk * dv + (int64_t)(32 * part) * dv + col;
@@ -306,6 +308,13 @@ __global__ void __launch_bounds__(kThreads, 1) gdr_bwd_walk_kernel(const __grid_
     fence_before_sync();
     __syncthreads();
     if (warp == 0) tmem_free512();
+}
+
+template <typename T, int kSteps>
+__global__ void __launch_bounds__(kWalkThreads, 1) gdr_bwd_walks_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, GdrRecord *records, int walks) {
+    const int block = blockIdx.x;
+    if (block < walks) walk_back<T, kSteps>(b, images, records, block);
+    else walk_forward<T, kSteps, true>(b.fwd, images, records, block - walks);
 }
 
 // ---- everything else, chunk by chunk --------------------------------------------------------------
@@ -720,16 +729,16 @@ int launch_gdr_bwd(const cc1d_gdr_bwd_params &b, cudaStream_t stream) {
     const cc1d_gdr_params &p = b.fwd;
     unsigned char *images = reinterpret_cast<unsigned char *>(b.workspace);
     GdrRecord *records = reinterpret_cast<GdrRecord *>(images + images_bytes(p));
-    int rc = launch_gdr_prep(p, true, images, stream);
-    if (rc == CC1D_OK) rc = launch_gdr_keep(p, images, records, stream);
+    const int rc = launch_gdr_prep(p, true, images, stream);
     if (rc != CC1D_OK) return rc;
     const int64_t sequences = gdr_sequences(p), walks = (sequences > 0 ? sequences : 1) * p.heads_v, chunks = gdr_slots(p) * p.heads_k;
-    if (walks >= (1ll << 31) || chunks >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
+    if (walks >= (1ll << 30) || chunks >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
     CC1D_DISPATCH_ITYPE(p.itype, {
         CC1D_DISPATCH_BOOL(p.dim_k <= 64, kNarrow, {
             constexpr int kSteps = kNarrow ? 4 : 8;     // contraction steps of 16 over dim_k
-            allow_dynamic_smem(reinterpret_cast<const void *>(gdr_bwd_walk_kernel<T, kSteps>), Back<T>::kBytes);
-            launch_k(gdr_bwd_walk_kernel<T, kSteps>, dim3((unsigned)walks), dim3(kThreads), Back<T>::kBytes, stream, b, (const unsigned char *)images, records);
+            constexpr uint32_t kBytes = Back<T>::kBytes > Fwd<T, true>::kBytes ? Back<T>::kBytes : Fwd<T, true>::kBytes;
+            allow_dynamic_smem(reinterpret_cast<const void *>(gdr_bwd_walks_kernel<T, kSteps>), kBytes);
+            launch_k(gdr_bwd_walks_kernel<T, kSteps>, dim3((unsigned)(2 * walks)), dim3(kWalkThreads), kBytes, stream, b, (const unsigned char *)images, records, (int)walks);
             allow_dynamic_smem(reinterpret_cast<const void *>(gdr_grads_kernel<T, kSteps>), Grads<T>::kBytes);
             if (chunks > 0)
                 launch_k(gdr_grads_kernel<T, kSteps>, dim3((unsigned)chunks), dim3(kGradThreads), Grads<T>::kBytes, stream, b, (const unsigned char *)images, (const GdrRecord *)records);

@@ -350,7 +350,6 @@ __device__ __forceinline__ void feed_walk(const GdrRows<T, kFeeders> &rows, cons
 struct GdrRecord {
     float S0[kGdrMaxDim][kGdrMaxDim], U[kChunk][kGdrMaxDim], dS[kGdrMaxDim][kGdrMaxDim], dB[kChunk][kGdrMaxDim];
 };
-int launch_gdr_keep(const cc1d_gdr_params &p, const void *images, GdrRecord *records, cudaStream_t stream);   // forward walk: S0 and U
 size_t gdr_image_bytes(const cc1d_gdr_params &p, bool back);          // of all chunks
 int launch_gdr_prep(const cc1d_gdr_params &p, bool back, void *images, cudaStream_t stream);
 

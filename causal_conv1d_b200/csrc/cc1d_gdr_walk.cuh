@@ -1,0 +1,338 @@
+// The forward walk over the chunks of the gated delta rule, for the forward and for the backward.
+#pragma once
+
+#include "cc1d_gdr_mma.cuh"
+
+namespace cc1d {
+namespace {
+
+constexpr int kWalkers = 512, kWalkThreads = kWalkers + 64 + kFeeders;   // warps 0-15 walk the chunks, 16 issues their products, 17 stores, 18, 19 load
+
+// Columns of the walk's tensor memory (128 lanes = the dim_v rows of S^T, R^T, U^T, O^T).
+constexpr uint32_t kFwdColS = 0;      // 3 x 64: pieces of S^T, two dim_k per column; later in a chunk
+constexpr uint32_t kFwdColDelta = 0;  //   128: U''^T K, and
+constexpr uint32_t kFwdColU = 128;    //   2 x 32: pieces of U^T (the third, fp32 inputs only, at 480)
+constexpr uint32_t kFwdColR = 192;    // 3 x 32: pieces of R^T, then of U''^T
+constexpr uint32_t kFwdColX = 288;    // 64: S^T K^T, then R^T (T - I)^T, then U^T P^T
+constexpr uint32_t kFwdColO = 352;    // 64: S^T Q^T
+__device__ __forceinline__ uint32_t col_u(int piece) { return piece < 2 ? kFwdColU + 32 * piece : 480; }
+
+template <typename T, bool kKeep> struct Fwd {
+    using S = GdrStage<T, kKeep>;
+    static constexpr int kStages = S::kPieces == 1 ? 2 : 1;
+    static constexpr uint32_t kBars = kStages * S::kBytes, kBytes = kBars + 128 + 1024;
+};
+
+// One CTA walks one sequence of one value head, chunk by chunk, with S^T (dim_v x dim_k) in the
+// registers of warps 0-15 (thread: one dim_v, a quarter of the dim_k):
+//   X = K S        R = beta (V - e^G X)        U = R + (T - I) R        U'' = e^{G_C - G} U
+//   O = scale (e^G Q S + P U)                  S <- e^{G_C} S + K^T U''
+// All five products run on tcgen05 with the transposed left factor (S^T, R^T, U^T, U''^T: 128 dim_v
+// rows) in tensor memory and the right one (K, Q, T, P) in shared memory, so nothing that the walk
+// computes passes through shared memory.  S itself is kept and decayed in fp32 registers; only
+// its pieces are rewritten every chunk.
+// kKeep: the backward's walk, which leaves S and U of every chunk in its record instead of an output.
+template <typename T, int kSteps, bool kKeep>
+__device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const unsigned char *images, GdrRecord *records, int block) {
+    using L = Fwd<T, kKeep>;
+    using St = GdrStage<T, kKeep>;
+    constexpr int NP = St::kPieces, PO = GdrType<T>::kOutPieces, PT = St::kSolve;
+    extern __shared__ unsigned char raw[];
+    unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    const uint32_t bars = smem_u32(smem + L::kBars);
+    const uint32_t bar_full = bars, bar_empty = bars + 16, bar_x = bars + 56, bar_u = bars + 64, bar_o = bars + 72, bar_d = bars + 80,
+                   bar_s = bars + 88, bar_r = bars + 96, bar_w = bars + 104, bar_out = bars + 112;
+    volatile int *dead = reinterpret_cast<volatile int *>(smem + L::kBars + 120);
+    uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 124);
+    const int tid = threadIdx.x, warp = __shfl_sync(kFullMask, tid >> 5, 0), lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < 2; ++s) { mbar_init(bar_full + 8 * s, kFeeders + 1); mbar_init(bar_empty + 8 * s, 1); }
+        mbar_init(bar_x, 1); mbar_init(bar_u, 1); mbar_init(bar_o, 1); mbar_init(bar_d, 1);
+        mbar_init(bar_s, kWalkers / 32); mbar_init(bar_r, kWalkers / 32); mbar_init(bar_w, kWalkers / 32); mbar_init(bar_out, kWalkers / 32);
+        *dead = 0;
+        fence_mbar_init();
+    }
+    pdl_wait();
+    if (warp == 0) tmem_alloc512(smem_u32(slot));
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+
+    const int heads = (int)p.heads_v, h = block % heads, n = block / heads;
+    const int sequences = (int)gdr_sequences(p);
+    GdrSeq seq = {0, 0, 0};
+    if (n < sequences) seq = gdr_sequence(p, n);
+    const int chunks = (seq.end - seq.begin + kChunk - 1) / kChunk;
+    const int dk = (int)p.dim_k, dv = (int)p.dim_v;
+
+    if (warp == kWalkers / 32) {
+        // issues the walk's products: a thread that issues is held up while earlier ones still run,
+        // which no warp with other work should be
+        for (int c = 0; c < chunks; ++c) {
+            const int s = c % L::kStages;
+            const uint32_t par = c & 1;
+            const uint32_t stage = smem_u32(smem) + s * St::kBytes;
+            const uint64_t kq = smem_desc(stage + St::kKq), kmn = smem_desc(stage + St::kKq, St::kPanel);
+            constexpr uint32_t id = mma_desc(128, 64, false, false), idd = mma_desc(128, 128, false, true);
+            gdr_wait(bar_full + 8 * s, (c / L::kStages) & 1, dead);
+            gdr_wait(bar_s, par, dead);
+            __syncwarp();
+            if (elect_one()) {
+                fence_after_sync();
+                bool more = false;
+                #pragma unroll
+                for (int o = 2; o >= 0; --o) {
+                    #pragma unroll
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= 3 || b >= NP) continue;
+                        #pragma unroll
+                        for (int i = 0; i < kSteps; ++i)
+                            mma_ts(kFwdColX, kFwdColS + 64 * a + 8 * i, desc_add(kq, b * St::kKqPiece + (i >> 2) * St::kPanel + (i & 3) * 32), id, again(more));
+                    }
+                }
+                mma_commit(bar_x);
+                more = false;
+                #pragma unroll
+                for (int o = kKeep ? -1 : PO - 1; o >= 0; --o) {
+                    #pragma unroll
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= PO || b >= NP) continue;
+                        #pragma unroll
+                        for (int i = 0; i < kSteps; ++i)
+                            mma_ts(kFwdColO, kFwdColS + 64 * a + 8 * i, desc_add(kq, b * St::kKqPiece + 64 * 128 + (i >> 2) * St::kPanel + (i & 3) * 32), id, again(more));
+                    }
+                }
+            }
+            __syncwarp();
+            gdr_wait(bar_r, par, dead);
+            __syncwarp();
+            if (elect_one()) {
+                fence_after_sync();
+                bool more = false;
+                #pragma unroll
+                for (int o = PT - 1; o >= 0; --o) {
+                    #pragma unroll
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= PT || b >= PT) continue;
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) mma_ts(kFwdColX, kFwdColR + 32 * a + 8 * i, desc_add(kq, St::kT + b * 8192 + 32 * i), id, again(more));
+                    }
+                }
+                mma_commit(bar_u);
+            }
+            __syncwarp();
+            gdr_wait(bar_w, par, dead);
+            __syncwarp();
+            if (elect_one()) {
+                fence_after_sync();
+                bool more = false;
+                #pragma unroll
+                for (int o = 2; o >= 0; --o) {
+                    #pragma unroll
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= 3 || b >= NP) continue;
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) mma_ts(kFwdColDelta, kFwdColR + 32 * a + 8 * i, desc_add(kmn, b * St::kKqPiece + 2048 * i), idd, again(more));
+                    }
+                }
+                mma_commit(bar_d);
+                more = false;
+                #pragma unroll
+                for (int o = kKeep ? -1 : PO - 1; o >= 0; --o) {
+                    #pragma unroll
+                    for (int a = 0; a <= o; ++a) {
+                        const int b = o - a;
+                        if (a >= PO || b >= PO) continue;
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i) mma_ts(kFwdColX, col_u(a) + 8 * i, desc_add(kq, St::kP + b * 8192 + 32 * i), id, again(more));
+                    }
+                }
+                mma_commit(bar_o);
+            }
+            __syncwarp();
+        }
+    } else if (warp == kWalkers / 32 + 1) {
+        // stores the output, which the walkers leave in the place of the stage's V, by rows, 16 bytes a
+        // lane (64 bulk copies of a row each took 4600 cycles to issue); then the stage is free
+        T *out = reinterpret_cast<T *>(p.out) + seq.row * p.out_batch_stride + h * p.out_h_stride;
+        constexpr int kVec = 16 / (int)sizeof(T), kLanes = kGdrMaxDim / kVec, kRows = 32 / kLanes;
+        const int at = lane % kLanes * kVec;
+        for (int c = 0; c < chunks; ++c) {
+            const unsigned char *V = smem + (c % L::kStages) * St::kBytes + St::kV;
+            gdr_wait(bar_out, c & 1, dead);
+            __syncwarp();
+            const int rows = min(kChunk, seq.end - seq.begin - c * kChunk);
+            if (!kKeep && at < dv) {
+                #pragma unroll 8
+                for (int i = lane / kLanes; i < rows; i += kRows) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(V + (i * kGdrMaxDim + at) * sizeof(T));
+                    *reinterpret_cast<uint4 *>(out + ((int64_t)seq.begin + c * kChunk + i) * p.out_l_stride + at) = v;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_empty + 8 * (c % L::kStages));
+        }
+    } else if (warp > kWalkers / 32) {
+        const GdrRows<T, kFeeders> rows(p, seq, h, p.v, seq.row * p.v_batch_stride + h * p.v_h_stride, p.v_l_stride);
+        const int64_t step = (int64_t)heads * St::kImage;
+        feed_walk<T, L::kStages, kKeep>(rows, images + gdr_first_slot(p, seq, n) * step + h * (int64_t)St::kImage, step, smem_u32(smem), seq.begin, chunks,
+                                        bar_full, bar_empty, dead, tid - kWalkers - 64);
+    } else {
+        const int quad = warp & 3, part = warp >> 2, col = quad * 32 + lane;   // part: a quarter of the dim_k and of the tokens
+        const uint32_t mine = (uint32_t)(quad * 32) << 16;
+        const int64_t row = n < sequences ? gdr_state_row(p, n) : -1;
+        const int64_t state_at = (int64_t)(32 * part) * dv + col;
+        float S[32];
+        {
+            const bool from = p.initial_states != nullptr && row >= 0 && (p.has_initial_state == nullptr || p.has_initial_state[n] != 0);
+            const float *src = p.initial_states + row * p.initial_states_batch_stride + h * p.initial_states_h_stride + state_at;
+            #pragma unroll
+            for (int j = 0; j < 32; ++j) S[j] = from && 32 * part + j < dk && col < dv ? src[(int64_t)j * dv] : 0.f;
+        }
+        // this warp's part of an operand is in tensor memory
+        auto ready = [&](uint32_t bar) {
+            tmem_wait_st();
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        GdrRecord *record = kKeep ? records + gdr_first_slot(p, seq, n) * heads + h : nullptr;
+        auto put_state = [&]() {
+            if (kKeep) {
+                #pragma unroll
+                for (int j = 0; j < 32; ++j) record->S0[32 * part + j][col] = S[j];
+            }
+            #pragma unroll
+            for (int b = 0; b < 4; ++b) split8_to_tmem<3>(S + 8 * b, mine + kFwdColS + 16 * part + 4 * b, 64, 128);
+            ready(bar_s);
+        };
+        if (chunks > 0) put_state();
+        T *out = reinterpret_cast<T *>(p.out) + seq.row * p.out_batch_stride + h * p.out_h_stride + col;
+        for (int c = 0; c < chunks; ++c) {
+            const int s = c % L::kStages;
+            const uint32_t par = c & 1;
+            unsigned char *stage = smem + s * St::kBytes;
+            gdr_wait(bar_full + 8 * s, (c / L::kStages) & 1, dead);
+            const GdrGates &gates = *reinterpret_cast<const GdrGates *>(stage + St::kGates);
+            T *V = reinterpret_cast<T *>(stage + St::kV) + 16 * part * kGdrMaxDim + col;
+            const int first = 16 * part;               // this thread's tokens: first .. first + 15
+            float R[16];
+            #pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const float4 b = *reinterpret_cast<const float4 *>(gates.beta + first + j);
+                R[j] = b.x * Elem<T>::to_f(V[j * kGdrMaxDim]); R[j + 1] = b.y * Elem<T>::to_f(V[(j + 1) * kGdrMaxDim]);
+                R[j + 2] = b.z * Elem<T>::to_f(V[(j + 2) * kGdrMaxDim]); R[j + 3] = b.w * Elem<T>::to_f(V[(j + 3) * kGdrMaxDim]);
+            }
+            gdr_wait(bar_x, par, dead);
+            __syncwarp();
+            fence_after_sync();
+            {             // R = beta V - beta e^G X
+                float x[16];
+                tmem_ld<16>(x, mine + kFwdColX + first);
+                tmem_wait_ld();
+                #pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(gates.minus_beta_from_start + first + j);
+                    const float2 u = fma2(make_float2(f.x, f.y), make_float2(x[j], x[j + 1]), make_float2(R[j], R[j + 1]));
+                    const float2 v = fma2(make_float2(f.z, f.w), make_float2(x[j + 2], x[j + 3]), make_float2(R[j + 2], R[j + 3]));
+                    x[j] = R[j] = u.x; x[j + 1] = R[j + 1] = u.y;
+                    x[j + 2] = R[j + 2] = v.x; x[j + 3] = R[j + 3] = v.y;
+                }
+                #pragma unroll
+                for (int j = 0; j < 16; j += 8) split8_to_tmem<PT>(x + j, mine + kFwdColR + first / 2 + j / 2, 32, 64);
+            }
+            ready(bar_r);
+            gdr_wait(bar_u, par, dead);
+            __syncwarp();
+            fence_after_sync();
+            {             // U and U''
+                float x[16];
+                tmem_ld<16>(x, mine + kFwdColX + first);
+                tmem_wait_ld();
+                #pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const float2 v = add2(make_float2(x[j], x[j + 1]), make_float2(R[j], R[j + 1]));
+                    x[j] = v.x; x[j + 1] = v.y;
+                }
+                if (kKeep) {
+                    #pragma unroll
+                    for (int j = 0; j < 16; ++j) record->U[first + j][col] = x[j];
+                    record += heads;
+                } else {
+                    #pragma unroll
+                    for (int j = 0; j < 16; j += 8) split8_to_tmem<PO>(x + j, mine + kFwdColU + first / 2 + j / 2, 32, 480 - kFwdColU);
+                }
+                #pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(gates.to_end + first + j);
+                    x[j] *= f.x; x[j + 1] *= f.y; x[j + 2] *= f.z; x[j + 3] *= f.w;
+                }
+                #pragma unroll
+                for (int j = 0; j < 16; j += 8) split8_to_tmem<3>(x + j, mine + kFwdColR + first / 2 + j / 2, 32, 64);
+            }
+            ready(bar_w);
+            const float whole = gates.from_start[kChunk - 1];
+            gdr_wait(bar_d, par, dead);
+            __syncwarp();
+            fence_after_sync();
+            #pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                float x[16];
+                tmem_ld<16>(x, mine + kFwdColDelta + 32 * part + 16 * b);
+                tmem_wait_ld();
+                #pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const float2 v = fma2(splat2(whole), make_float2(S[16 * b + j], S[16 * b + j + 1]), make_float2(x[j], x[j + 1]));
+                    S[16 * b + j] = v.x; S[16 * b + j + 1] = v.y;
+                }
+            }
+            // the output is taken out of tensor memory before the next chunk's products go there
+            if (!kKeep) {
+                gdr_wait(bar_o, par, dead);
+                __syncwarp();
+                fence_after_sync();
+                #pragma unroll
+                for (int b = 0; b < 16; b += 8) {
+                    float x[8], y[8];
+                    tmem_ld<8>(x, mine + kFwdColO + first + b);
+                    tmem_ld<8>(y, mine + kFwdColX + first + b);
+                    tmem_wait_ld();
+                    #pragma unroll
+                    for (int j = 0; j < 8; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(gates.from_start + first + b + j);
+                        x[j] = fmaf(f.x, x[j], y[j]); x[j + 1] = fmaf(f.y, x[j + 1], y[j + 1]);
+                        x[j + 2] = fmaf(f.z, x[j + 2], y[j + 2]); x[j + 3] = fmaf(f.w, x[j + 3], y[j + 3]);
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j) V[(b + j) * kGdrMaxDim] = Elem<T>::from_f(p.scale * x[j]);   // where this thread read its v
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_out);
+            fence_before_sync();
+            walk_sync<kWalkers>();                      // every thread has read its part of Delta
+            fence_after_sync();
+            if (c + 1 < chunks) put_state();
+        }
+        if (!kKeep && p.final_states != nullptr && row >= 0) {
+            float *dst = p.final_states + row * p.final_states_batch_stride + h * p.final_states_h_stride + state_at;
+            #pragma unroll
+            for (int j = 0; j < 32; ++j) if (32 * part + j < dk && col < dv) dst[(int64_t)j * dv] = S[j];
+        }
+        // tokens that belong to no sequence
+        if (!kKeep && p.cu_seqlens != nullptr && n + 1 >= sequences) {
+            for (int64_t t = seq.end + part; t < p.seqlen; t += 4)
+                if (col < dv) out[t * p.out_l_stride] = Elem<T>::from_f(0.f);
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 0) tmem_free512();
+}
+
+}  // namespace
+}  // namespace cc1d
