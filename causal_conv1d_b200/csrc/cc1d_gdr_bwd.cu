@@ -321,18 +321,21 @@ __global__ void __launch_bounds__(kWalkThreads, 1) gdr_bwd_walks_kernel(const __
 constexpr int kGradThreads = 512;
 
 // Tensor memory: lanes 0-63 the rows of q (and dO), lanes 64-127 those of k (and dB).
-constexpr uint32_t kColG = 0;      // 128: dO S0^T | dB S0^T, later M_P K | M_P^T Q + (M_A + M_A^T) K
+constexpr uint32_t kColG = 0;      // 128: dO S0^T | dB S0^T, later M_P K | M_A K
 constexpr uint32_t kColPa = 128;   // 64: dO U^T | dB U^T
 constexpr uint32_t kColQk = 192;   // 64: Q K^T | K K^T
-constexpr uint32_t kColU = 256;    // 128: - | U dS^T
+constexpr uint32_t kColU = 256;    // 128: - | U dS^T, later - | M_P^T Q + M_A^T K
 
 template <typename T> struct Grads {
     using S = GdrStage<T, true>;
     static constexpr int NP = S::kPieces;
     // three pieces in every type: the gradient of g, fp32 as a rule, is a difference of larger sums
     static constexpr int NB = 3;
-    static constexpr uint32_t kKq = 0, kA = NP * S::kKqPiece, kAPiece = 16384, kB = kA + NB * kAPiece, kBPiece = 192 * 128, kMPiece = 32768,
-                              kGates = kB + NB * kBPiece, kDots = kGates + 3072, kBars = kDots + 3 * 4 * 128 * 4, kBytes = kBars + 64 + 1024;
+    // dS has a place of its own where that fits (else that of [dO; dB], when their products are done)
+    static constexpr bool kOwnDs = NP == 1;
+    static constexpr uint32_t kKq = 0, kA = NP * S::kKqPiece, kAPiece = 16384, kB = kA + NB * kAPiece, kBPiece = 192 * 128,
+                              kDs = kOwnDs ? kB + NB * kBPiece : kA, kGates = kB + NB * kBPiece + (kOwnDs ? NB * kAPiece : 0),
+                              kDots = kGates + 3072, kBars = kDots + 3 * 4 * 128 * 4, kBytes = kBars + 64 + 1024;
     static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
 
@@ -358,28 +361,19 @@ template <typename T> __device__ __forceinline__ void store8(T *dst, const float
     *reinterpret_cast<uint4 *>(dst) = pack<T>(x);
     if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst + 4) = pack<T>(x + 4);
 }
-// one value into element (row, column) of a tile of 128-row panels, kPieces pieces
-template <int kPieces> __device__ __forceinline__ void put1(float x, unsigned char *tile, int row, int column) {
-    const uint32_t at = tile_at(row, column >> 3, 16384) + (column & 7) * 2;
-    #pragma unroll
-    for (int k = 0; k < kPieces; ++k) {
-        const __nv_bfloat16 v = __float2bfloat16_rn(x);
-        *reinterpret_cast<__nv_bfloat16 *>(tile + at + k * 32768) = v;
-        x -= __bfloat162float(v);
-    }
-}
-
 // One CTA: one chunk of one key head, the value heads of its group one after the other (so dq and dk are
 // summed in registers in a fixed order).  With the rows [dO; dB] and [Q; K] stacked to 128:
 //   [dO; dB] [S0; U]^T -> dO S0^T, dB S0^T, dP = dO U^T, -dA = dB U^T      [Q; K] K^T      U dS^T
 //   M_P = scale dP e^{Gi - Gj} (j <= i), M_A = beta dA e^{Gi - Gj} (j < i)
 //   dQ = scale e^G dO S0^T + M_P K
-//   dK = -beta e^G dB S0^T + e^{G_C - G} U dS^T + M_P^T Q + (M_A + M_A^T) K
+//   dK = -beta e^G dB S0^T + e^{G_C - G} U dS^T + M_A K + [M_P; M_A]^T [Q; K]
 //   dbeta = dB.V - e^G k.(dB S0^T) + sum_j t_ij,  t = dA (k_i.k_j) e^{Gi - Gj}
-//   dG = q.dQ - k.(M_P^T Q + (M_A + M_A^T) K) - beta e^G k.(dB S0^T) - k.(e^{G_C - G} U dS^T) + 2 beta sum_j t_ij
-//        (what q and k see of G they see through their own products; the sum over j of t_ij is k.(M_A K), which
-//        counts with the other sign), and at the chunk's end + sum k.(e^{G_C - G} U dS^T) + e^{G_C} <S0, dS>;
+//   dG = q.dQ - beta e^G k.(dB S0^T) + beta sum_j t_ij - k.(e^{G_C - G} U dS^T) - k.([M_P; M_A]^T [Q; K])
+//        (what q and k see of G they see through their own products, with the sign of their place in e^{Gi - Gj}), and
+//        at the chunk's end + sum k.(e^{G_C - G} U dS^T) + e^{G_C} <S0, dS>;
 //   dg is its sum from the chunk's end.
+// [M_P; M_A] is one tile of shared memory: rows as the contraction's results for the products with K, and
+// (read with its rows as the contraction) its own transpose for those with [Q; K].
 template <typename T, int kSteps>
 __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, const GdrRecord *records) {
     using L = Grads<T>;
@@ -441,41 +435,75 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
         const T *dout = reinterpret_cast<const T *>(b.dout) + seq.row * b.dout_batch_stride + h * b.dout_h_stride;
         const T *v = reinterpret_cast<const T *>(p.v) + seq.row * p.v_batch_stride + h * p.v_h_stride;
         float state_dot = 0.f, value_dot = 0.f;
-        for (int q = 0; q < panels; ++q) {
-            // [dO; dB] and [S0; U], 64 of the dim_v
-            const int row = tid >> 3, c16 = tid & 7, at = 64 * q + 8 * c16;
-            const int64_t t = t0 + row;
+        // a panel: 64 of the dim_v; this thread: 8 of them, of token `row` and of the rows `row` and 64 + `row` of the states
+        const int row = tid >> 3, c16 = tid & 7;
+        const int64_t t = t0 + row;
+        uint4 do_raw[sizeof(T) / 2], v_raw[sizeof(T) / 2];
+        float d_b[8], u[8], s0[2][8], ds[2][8];
+        auto ask = [&](int at) {
             const bool ok = t < seq.end && at < dv;
-            float x[8], y[8], s0[2][8], ds[2][8];
+            load_row<T>(dout + t * b.dout_l_stride + at, ok, do_raw);
+            load_row<T>(v + t * p.v_l_stride + at, ok, v_raw);
+            get8(d_b, &record.dB[row][at]);
+            get8(u, &record.U[row][at]);
             #pragma unroll
             for (int r = 0; r < 2; ++r) get8(s0[r], &record.S0[row + 64 * r][at]);
-            get8_of<T>(x, dout + t * b.dout_l_stride + at, ok);
+        };
+        auto ask_ds = [&](int at) {
+            #pragma unroll
+            for (int r = 0; r < 2; ++r) get8(ds[r], &record.dS[row + 64 * r][at]);
+        };
+        ask(8 * c16);
+        ask_ds(8 * c16);
+        for (int q = 0; q < panels; ++q) {
+            const int at = 64 * q + 8 * c16;
+            float x[8], y[8];
+            unpack<T>(do_raw[0], x); unpack<T>(v_raw[0], y);
+            if constexpr (sizeof(T) == 4) { unpack<T>(do_raw[1], x + 4); unpack<T>(v_raw[1], y + 4); }
             put8<NB>(x, base + L::kA + tile_at(row, c16, 0), L::kAPiece);
-            get8(x, &record.dB[row][at]);
-            put8<NB>(x, base + L::kA + tile_at(64 + row, c16, 0), L::kAPiece);
-            get8_of<T>(y, v + t * p.v_l_stride + at, ok);
+            put8<NB>(d_b, base + L::kA + tile_at(64 + row, c16, 0), L::kAPiece);
             #pragma unroll
-            for (int j = 0; j < 8; ++j) { value_dot = fmaf(x[j], y[j], value_dot); x[j] *= gates.beta[row]; }
-            if (ok) store8<T>(reinterpret_cast<T *>(b.dv) + ((seq.row * p.seqlen + t) * heads + h) * dv + at, x);
-            get8(x, &record.U[row][at]);
-            put8<NB>(x, base + L::kB + tile_at(128 + row, c16, 0), L::kBPiece);
+            for (int j = 0; j < 8; ++j) { value_dot = fmaf(d_b[j], y[j], value_dot); x[j] = gates.beta[row] * d_b[j]; }
+            if (t < seq.end && at < dv) store8<T>(reinterpret_cast<T *>(b.dv) + ((seq.row * p.seqlen + t) * heads + h) * dv + at, x);
+            put8<NB>(u, base + L::kB + tile_at(128 + row, c16, 0), L::kBPiece);
             #pragma unroll
-            for (int r = 0; r < 2; ++r) put8<NB>(s0[r], base + L::kB + tile_at(row + 64 * r, c16, 0), L::kBPiece);
+            for (int r = 0; r < 2; ++r) {
+                put8<NB>(s0[r], base + L::kB + tile_at(row + 64 * r, c16, 0), L::kBPiece);
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) state_dot = fmaf(s0[r][j], ds[r][j], state_dot);
+                if constexpr (L::kOwnDs) put8<NB>(ds[r], base + L::kDs + tile_at(row + 64 * r, c16, 0), L::kAPiece);
+            }
+            if (q + 1 < panels) {        // the next panel's loads pass under this one's products
+                ask(at + 64);
+                if (L::kOwnDs) ask_ds(at + 64);
+            }
+            const auto state_product = [&]() {
+                constexpr uint32_t id = mma_desc(128, 128, false, false);
+                // rows 64-191 of [S0; U]: the upper half of the result is U dS^T, the lower one is not used
+                const uint64_t up = smem_desc(base + L::kB + 64 * 128), d = smem_desc(base + L::kDs);
+                bool more = q > 0;
+                #pragma unroll
+                for (int o = NB - 1; o >= 0; --o) {
+                    #pragma unroll
+                    for (int m = 0; m <= o; ++m) {
+                        #pragma unroll
+                        for (int s = 0; s < 4; ++s) mma_ss(kColU, desc_add(up, m * L::kBPiece + 32 * s), desc_add(d, (o - m) * L::kAPiece + 32 * s), id, again(more));
+                    }
+                }
+            };
             smem_written();
             if (warp == 0) {
                 if (elect_one()) {
                     fence_after_sync();
-                                        constexpr uint32_t id = mma_desc(128, 192, false, false), idq = mma_desc(128, 64, false, false);
+                    constexpr uint32_t id = mma_desc(128, 192, false, false), idq = mma_desc(128, 64, false, false);
                     const uint64_t a = smem_desc(base + L::kA), bb = smem_desc(base + L::kB), kq = smem_desc(base + L::kKq);
                     bool more = q > 0;
                     #pragma unroll
                     for (int o = NB - 1; o >= 0; --o) {
                         #pragma unroll
                         for (int m = 0; m <= o; ++m) {
-                            const int k = o - m;
-                            if (m >= NB || k >= NB) continue;
                             #pragma unroll
-                            for (int s = 0; s < 4; ++s) mma_ss(kColG, desc_add(a, m * L::kAPiece + 32 * s), desc_add(bb, k * L::kBPiece + 32 * s), id, again(more));
+                            for (int s = 0; s < 4; ++s) mma_ss(kColG, desc_add(a, m * L::kAPiece + 32 * s), desc_add(bb, (o - m) * L::kBPiece + 32 * s), id, again(more));
                         }
                     }
                     if (q == 0 && h == hk * group) {
@@ -484,53 +512,41 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
                         for (int o = 2; o >= 0; --o) {
                             #pragma unroll
                             for (int m = 0; m <= o; ++m) {
-                                const int k = o - m;
-                                if (m >= NP || k >= NP) continue;
+                                if (m >= NP || o - m >= NP) continue;
                                 #pragma unroll
                                 for (int s = 0; s < kSteps; ++s) {
                                     const uint32_t off = (s >> 2) * S::kPanel + (s & 3) * 32;
-                                    mma_ss(kColQk, desc_add(kq, m * S::kKqPiece + off), desc_add(kq, k * S::kKqPiece + 64 * 128 + off), idq, again(more));
+                                    mma_ss(kColQk, desc_add(kq, m * S::kKqPiece + off), desc_add(kq, (o - m) * S::kKqPiece + 64 * 128 + off), idq, again(more));
                                 }
                             }
                         }
                     }
+                    if constexpr (L::kOwnDs) state_product();
                     mma_commit(bar);
                 }
                 __syncwarp();
             }
-            #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                get8(ds[r], &record.dS[row + 64 * r][at]);
+            wait_mma();
+            if constexpr (!L::kOwnDs) {
                 #pragma unroll
-                for (int j = 0; j < 8; ++j) state_dot = fmaf(s0[r][j], ds[r][j], state_dot);
-            }
-            wait_mma();
-            #pragma unroll
-            for (int r = 0; r < 2; ++r) put8<NB>(ds[r], base + L::kA + tile_at(row + 64 * r, c16, 0), L::kAPiece);
-            smem_written();
-            if (warp == 0) {
-                if (elect_one()) {
-                    fence_after_sync();
-                    bool more;
-                    constexpr uint32_t id = mma_desc(128, 128, false, false);
-                    // rows 64-191 of [S0; U]: the upper half of the result is U dS^T, the lower one is not used
-                    const uint64_t u = smem_desc(base + L::kB + 64 * 128), d = smem_desc(base + L::kA);
-                    more = q > 0;
-                    #pragma unroll
-                    for (int o = NB - 1; o >= 0; --o) {
-                        #pragma unroll
-                        for (int m = 0; m <= o; ++m) {
-                            const int k = o - m;
-                            if (m >= NB || k >= NB) continue;
-                            #pragma unroll
-                            for (int s = 0; s < 4; ++s) mma_ss(kColU, desc_add(u, m * L::kBPiece + 32 * s), desc_add(d, k * L::kAPiece + 32 * s), id, again(more));
-                        }
+                for (int r = 0; r < 2; ++r) put8<NB>(ds[r], base + L::kDs + tile_at(row + 64 * r, c16, 0), L::kAPiece);
+                if (q + 1 < panels) ask_ds(at + 64);
+                smem_written();
+                if (warp == 0) {
+                    if (elect_one()) {
+                        fence_after_sync();
+                        state_product();
+                        mma_commit(bar);
                     }
-                    mma_commit(bar);
+                    __syncwarp();
                 }
-                __syncwarp();
+                wait_mma();
             }
-            wait_mma();
+        }
+        if (h + 1 < (hk + 1) * group) {
+            // the next head's record into L2, two lines a thread (in registers it would spill)
+            const char *next = reinterpret_cast<const char *>(&records[slot * heads + h + 1]);
+            for (uint32_t at = tid * 128; at < sizeof(GdrRecord); at += kGradThreads * 128) asm volatile("prefetch.global.L2 [%0];" :: "l"(next + at));
         }
         // row sums whose threads are not those of the rows below
         #pragma unroll
@@ -540,63 +556,38 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
         if ((lane & 7) == 0) dots[2][1][tid >> 3] = value_dot;
         if (lane == 0) dots[2][0][warp] = state_dot;
 
-        unsigned char *tile = smem + L::kA;                // M: rows 0-63 [0 | M_P], rows 64-127 [M_P^T | M_A + M_A^T]
-        {
+        {   // [M_P; M_A], 64 columns
             const int j0 = 16 * part, block = i >> 4;
             const float2 gi = gates.g[i];
-            const float beta = gates.beta[i];
+            const float factor = is_k ? -gates.beta[i] : p.scale;
             const bool steep = gates.steep != 0;
-            float sum = 0.f;
+            float sum = 0.f, x[16];
+            #pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = 0.f;
             if (j0 <= first + 31) {
-                float x[16], y[16];
+                float y[16];
                 tmem_ld<16>(x, mine + kColPa + j0);
                 tmem_ld<16>(y, mine + kColQk + j0);
                 tmem_wait_ld();
                 const float *f = (16 * block > j0 ? gates.column[block - 1] : gates.same) + j0;
-                const float row = gates.row[i];
+                const float row_fade = gates.row[i];
+                const int last = is_k ? i - 1 : i;
                 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const float fade = j0 + 16 <= first || !steep ? row * f[j] : gdr_fade(gi, gates.g[j0 + j]);
-                    x[j] *= fade;
-                    if (is_k) {
-                        x[j] = j0 + j < i ? -x[j] : 0.f;
-                        sum = fmaf(x[j], y[j], sum);
-                        x[j] *= beta;
-                    } else {
-                        x[j] = j0 + j <= i ? p.scale * x[j] : 0.f;
-                    }
+                    const float fade = j0 + 16 <= first || !steep ? row_fade * f[j] : gdr_fade(gi, gates.g[j0 + j]);
+                    x[j] = j0 + j <= last ? x[j] * fade : 0.f;
+                    sum = fmaf(-x[j], y[j], sum);      // of the rows of k: dA (k_i.k_j) e^{Gi - Gj}
+                    x[j] *= factor;
                 }
-                if (!is_k) {
-                    float lo[8], hi[8];
-                    #pragma unroll
-                    for (int j = 0; j < 8; ++j) { lo[j] = x[j]; hi[j] = x[8 + j]; }
-                    put8<NB>(lo, base + L::kA + tile_at(i, 8 + j0 / 8, 16384), L::kMPiece);
-                    put8<NB>(hi, base + L::kA + tile_at(i, 9 + j0 / 8, 16384), L::kMPiece);
-                    #pragma unroll
-                    for (int j = 0; j < 16; ++j) put1<NB>(x[j], tile, 64 + j0 + j, i);
-                } else {
-                    #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if (j0 + j <= i) {
-                            put1<NB>(x[j], tile, 64 + i, 64 + j0 + j);
-                            if (j0 + j < i) put1<NB>(x[j], tile, 64 + j0 + j, 64 + i);
-                        }
-                    }
-                }
-            } else if (!is_k) {                            // above the diagonal
-                const float zero[8] = {};
-                put8<NB>(zero, base + L::kA + tile_at(i, 8 + j0 / 8, 16384), L::kMPiece);
-                put8<NB>(zero, base + L::kA + tile_at(i, 9 + j0 / 8, 16384), L::kMPiece);
+            }
+            #pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float z[8];
                 #pragma unroll
-                for (int j = 0; j < 16; ++j) put1<NB>(0.f, tile, 64 + j0 + j, i);
+                for (int j = 0; j < 8; ++j) z[j] = x[8 * e + j];
+                put8<NB>(z, base + L::kA + tile_at((is_k ? 64 : 0) + i, j0 / 8 + e, 0), L::kAPiece);
             }
-            if (!is_k) {                                   // the zeros of rows 0-63
-                const float zero[8] = {};
-                put8<NB>(zero, base + L::kA + tile_at(i, j0 / 8, 16384), L::kMPiece);
-                put8<NB>(zero, base + L::kA + tile_at(i, 1 + j0 / 8, 16384), L::kMPiece);
-            } else {
-                dots[1][part][i] = sum;
-            }
+            if (is_k) dots[1][part][i] = sum;
         }
         float mineq[32];                                   // this head's dq or dk: token i, dim_k 32 * part ..
         float dot_g = 0.f, dot_u = 0.f;
@@ -635,18 +626,28 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
         if (warp == 0) {
             if (elect_one()) {
                 fence_after_sync();
-                                constexpr uint32_t id = mma_desc(128, 128, false, true);
-                const uint64_t m0 = smem_desc(base + L::kA), qk = smem_desc(base + L::kKq, S::kPanel);
+                                constexpr uint32_t id = mma_desc(128, 128, false, true), idt = mma_desc(128, 128, true, true);
+                const uint64_t tile = smem_desc(base + L::kA), k_mn = smem_desc(base + L::kKq + 64 * 128, S::kPanel), qk = smem_desc(base + L::kKq, S::kPanel);
                 bool more = false;
                 #pragma unroll
                 for (int o = NB - 1; o >= 0; --o) {
                     #pragma unroll
                     for (int m = 0; m <= o; ++m) {
-                        const int k = o - m;
-                        if (m >= NB || k >= NP) continue;
+                        if (o - m >= NP) continue;
                         #pragma unroll
-                        for (int s = 0; s < 8; ++s)
-                            mma_ss(kColG, desc_add(m0, m * L::kMPiece + (s >> 2) * 16384 + (s & 3) * 32), desc_add(qk, k * S::kKqPiece + 2048 * s), id, again(more));
+                        for (int s = 0; s < 4; ++s) mma_ss(kColG, desc_add(tile, m * L::kAPiece + 32 * s), desc_add(k_mn, (o - m) * S::kKqPiece + 2048 * s), id, again(more));
+                    }
+                }
+                // the transpose of the tile as lanes 64-127; lanes 0-63 take what lies in K and Q's place, and are not used
+                const uint64_t turned = smem_desc(base + L::kKq, L::kA - L::kKq);
+                more = false;
+                #pragma unroll
+                for (int o = NB - 1; o >= 0; --o) {
+                    #pragma unroll
+                    for (int m = 0; m <= o; ++m) {
+                        if (o - m >= NP) continue;
+                        #pragma unroll
+                        for (int s = 0; s < 8; ++s) mma_ss(kColU, desc_add(turned, m * L::kAPiece + 2048 * s), desc_add(qk, (o - m) * S::kKqPiece + 2048 * s), idt, again(more));
                     }
                 }
                 mma_commit(bar);
@@ -657,15 +658,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
         float dot = 0.f;
         #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float x[8], own[8];
+            float x[8], y[8], own[8];
             tmem_ld<8>(x, mine + kColG + 32 * part + 8 * e);
+            tmem_ld<8>(y, mine + kColU + 32 * part + 8 * e);
             tmem_wait_ld();
             own8(own, e);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float sum = x[j] + mineq[8 * e + j];
-                dot = fmaf(own[j], is_k ? x[j] : sum, dot);
-                total[8 * e + j] += sum;
+                dot = fmaf(own[j], is_k ? y[j] : sum, dot);
+                total[8 * e + j] += is_k ? sum + y[j] : sum;
             }
         }
         fence_before_sync();
@@ -684,7 +686,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
                 u += uk;
                 const float seen = -gates.from_start[k] * g2;      // -e^G k.(dB S0^T)
                 db[e] = dots[2][1][k] + seen + ts;
-                d[e] = (qd - kd) - uk + gates.beta[k] * (seen + 2.f * ts);
+                d[e] = (qd - kd) - uk + gates.beta[k] * (seen + ts);
             }
             #pragma unroll
             for (int m = 16; m >= 1; m >>= 1) { u += __shfl_xor_sync(kFullMask, u, m); s += __shfl_xor_sync(kFullMask, s, m); }
