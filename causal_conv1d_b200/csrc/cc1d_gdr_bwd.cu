@@ -34,8 +34,9 @@ template <typename T> struct Back {
 //   dS <- e^{G_C} dS + scale (e^G Q)^T dO - (beta e^G K)^T dB
 // Same division of work and same precision as the forward walk; P^T dO and Q^T E do not wait for the
 // walk and run beside its arithmetic.
-template <typename T, int kSteps>
-__device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const unsigned char *images, GdrRecord *records, int block) {
+// kSum: a segment from zeros, its last gradient only.
+template <typename T, int kSteps, bool kSum>
+__device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const unsigned char *images, GdrRecord *records, const GdrSegments &segs, int64_t block) {
     using L = Back<T>;
     using St = GdrStage<T, true>;
     constexpr int NP = St::kPieces, PO = St::kOut, PT = St::kSolve;
@@ -48,6 +49,13 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
     volatile int *dead = reinterpret_cast<volatile int *>(smem + L::kBars + 96);
     uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 100);
     const int tid = threadIdx.x, warp = __shfl_sync(kFullMask, tid >> 5, 0), lane = tid & 31;
+    pdl_wait();
+    const int heads = (int)p.heads_v, h = (int)(block % heads), sequences = (int)gdr_sequences(p);
+    GdrPart w;
+    if (!gdr_find_part(p, segs, block / heads, w) || (kSum && w.first)) return;
+    const GdrSeq seq = w.seq;
+    const int n = w.n, chunks = w.chunks, dk = (int)p.dim_k, dv = (int)p.dim_v;
+    const int64_t first_slot = w.slot;
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) { mbar_init(bar_full + 8 * s, kFeeders + 1); mbar_init(bar_empty + 8 * s, kWalkers / 32); }
         mbar_init(bar_x, 1); mbar_init(bar_u, 1); mbar_init(bar_d, 1);
@@ -55,19 +63,10 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
         *dead = 0;
         fence_mbar_init();
     }
-    pdl_wait();
     if (warp == 0) tmem_alloc512(smem_u32(slot));
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-
-    const int heads = (int)p.heads_v, h = block % heads, n = block / heads;
-    const int sequences = (int)gdr_sequences(p);
-    GdrSeq seq = {0, 0, 0};
-    if (n < sequences) seq = gdr_sequence(p, n);
-    const int chunks = (seq.end - seq.begin + kChunk - 1) / kChunk;
-    const int dk = (int)p.dim_k, dv = (int)p.dim_v;
-    const int64_t first_slot = n < sequences ? gdr_first_slot(p, seq, n) : 0;
 
     if (warp == kWalkers / 32) {
         for (int i = 0; i < chunks; ++i) {
@@ -190,7 +189,8 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
         float S[32];
         #pragma unroll
         for (int j = 0; j < 32; ++j)
-            S[j] = b.dfinal_states != nullptr && n < sequences && 32 * part + j < dk && col < dv ? b.dfinal_states[state_at + (int64_t)j * dv] : 0.f;
+            S[j] = kSum ? 0.f : !w.last ? w.segment[h].end[32 * part + j][col]
+                 : b.dfinal_states != nullptr && n < sequences && 32 * part + j < dk && col < dv ? b.dfinal_states[state_at + (int64_t)j * dv] : 0.f;
         auto ready = [&](uint32_t bar) {
             tmem_wait_st();
             fence_before_sync();
@@ -199,8 +199,10 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
         };
         GdrRecord *record = records + (first_slot + chunks - 1) * heads + h;
         auto put_state = [&]() {
-            #pragma unroll
-            for (int j = 0; j < 32; ++j) record->dS[32 * part + j][col] = S[j];
+            if (!kSum) {
+                #pragma unroll
+                for (int j = 0; j < 32; ++j) record->dS[32 * part + j][col] = S[j];
+            }
             #pragma unroll
             for (int i = 0; i < 4; ++i) split8_to_tmem<3>(S + 8 * i, mine + kColS + 16 * part + 4 * i, 64, 128);
             ready(bar_s);
@@ -257,7 +259,7 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
                 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     x[k] += R[j + k];
-                    record->dB[first + j + k][col] = x[k];
+                    if (!kSum) record->dB[first + j + k][col] = x[k];
                     x[k] *= gates.minus_beta_from_start[first + j + k];
                 }
                 split8_to_tmem<3>(x, mine + kColF + first / 2 + j / 2, 32, 64);
@@ -283,14 +285,18 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
             fence_after_sync();
             if (i + 1 < chunks) put_state();
         }
-        if (b.dinitial_states != nullptr && n < sequences) {
+        if (kSum) {
+            #pragma unroll
+            for (int j = 0; j < 32; ++j) w.segment[h].back[32 * part + j][col] = S[j];
+        }
+        if (!kSum && w.first && b.dinitial_states != nullptr && n < sequences) {
             const bool from = p.initial_states != nullptr && gdr_state_row(p, n) >= 0 && (p.has_initial_state == nullptr || p.has_initial_state[n] != 0);
             #pragma unroll
             for (int j = 0; j < 32; ++j)
                 if (32 * part + j < dk && col < dv) b.dinitial_states[state_at + (int64_t)j * dv] = from ? S[j] : 0.f;
         }
         // tokens that belong to no sequence
-        if (p.cu_seqlens != nullptr && n + 1 >= sequences) {
+        if (!kSum && w.last && p.cu_seqlens != nullptr && n + 1 >= sequences) {
             const int group = heads / (int)p.heads_k;
             for (int64_t t = seq.end + part; t < p.seqlen; t += 4) {
                 if (col < dv) reinterpret_cast<T *>(b.dv)[(t * heads + h) * dv + col] = Elem<T>::from_f(0.f);
@@ -311,10 +317,21 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
 }
 
 template <typename T, int kSteps>
-__global__ void __launch_bounds__(kWalkThreads, 1) gdr_bwd_walks_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, GdrRecord *records, int walks) {
-    const int block = blockIdx.x;
-    if (block < walks) walk_back<T, kSteps>(b, images, records, block);
-    else walk_forward<T, kSteps, true>(b.fwd, images, records, block - walks);
+__global__ void __launch_bounds__(kWalkThreads, 1) gdr_bwd_walks_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, GdrRecord *records, const GdrSegments segs, unsigned walks) {
+    if (blockIdx.x < walks) walk_back<T, kSteps, false>(b, images, records, segs, blockIdx.x);
+    else walk_forward<T, kSteps, kKeep, true>(b.fwd, images, records, segs, blockIdx.x - walks, false);
+}
+
+// a third of the CTAs each: the gradient's walk from zeros, the state's, M
+template <typename T, int kSteps>
+__global__ void __launch_bounds__(kWalkThreads, 1) gdr_bwd_summary_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, const GdrSegments segs, unsigned walks) {
+    if (blockIdx.x < walks) {
+        walk_back<T, kSteps, true>(b, images, nullptr, segs, blockIdx.x);
+    } else {
+        const unsigned block = blockIdx.x - walks;
+        const bool unit = block >= walks;
+        walk_forward<T, kSteps, kSummary, true>(b.fwd, images, nullptr, segs, unit ? block - walks : block, unit);
+    }
 }
 
 // ---- everything else, chunk by chunk --------------------------------------------------------------
@@ -723,24 +740,35 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
 
 static size_t images_bytes(const cc1d_gdr_params &p) { return (gdr_image_bytes(p, true) + 255) / 256 * 256; }
 
+static size_t records_bytes(const cc1d_gdr_params &p) { return (size_t)gdr_slots(p) * (size_t)p.heads_v * sizeof(GdrRecord); }
+
 size_t gdr_bwd_workspace_bytes(const cc1d_gdr_bwd_params &b) {
-    return images_bytes(b.fwd) + (size_t)gdr_slots(b.fwd) * (size_t)b.fwd.heads_v * sizeof(GdrRecord);
+    const int per = gdr_plan_segments(b.fwd, true);
+    return images_bytes(b.fwd) + records_bytes(b.fwd) + (per > 0 ? (size_t)gdr_segment_slots(b.fwd, per) * (size_t)b.fwd.heads_v * sizeof(GdrSegment) : 0);
 }
 
 int launch_gdr_bwd(const cc1d_gdr_bwd_params &b, cudaStream_t stream) {
     const cc1d_gdr_params &p = b.fwd;
     unsigned char *images = reinterpret_cast<unsigned char *>(b.workspace);
     GdrRecord *records = reinterpret_cast<GdrRecord *>(images + images_bytes(p));
-    const int rc = launch_gdr_prep(p, true, images, stream);
+    const GdrSegments segs = {reinterpret_cast<GdrSegment *>(images + images_bytes(p) + records_bytes(p)), gdr_plan_segments(p, true)};
+    const int64_t sequences = gdr_sequences(p), chunks = gdr_slots(p) * p.heads_k;
+    const int64_t walks = (segs.per > 0 ? gdr_segment_slots(p, segs.per) : sequences > 0 ? sequences : 1) * p.heads_v;
+    if (walks >= (1ll << 29) || chunks >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
+    int rc = launch_gdr_prep(p, true, images, stream);
     if (rc != CC1D_OK) return rc;
-    const int64_t sequences = gdr_sequences(p), walks = (sequences > 0 ? sequences : 1) * p.heads_v, chunks = gdr_slots(p) * p.heads_k;
-    if (walks >= (1ll << 30) || chunks >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
     CC1D_DISPATCH_ITYPE(p.itype, {
         CC1D_DISPATCH_BOOL(p.dim_k <= 64, kNarrow, {
             constexpr int kSteps = kNarrow ? 4 : 8;     // contraction steps of 16 over dim_k
             constexpr uint32_t kBytes = Back<T>::kBytes > Fwd<T, true>::kBytes ? Back<T>::kBytes : Fwd<T, true>::kBytes;
+            if (segs.per > 0) {
+                allow_dynamic_smem(reinterpret_cast<const void *>(gdr_bwd_summary_kernel<T, kSteps>), kBytes);
+                launch_k(gdr_bwd_summary_kernel<T, kSteps>, dim3((unsigned)(3 * walks)), dim3(kWalkThreads), kBytes, stream, b, (const unsigned char *)images, segs, (unsigned)walks);
+                rc = launch_gdr_join(p, segs, b.dfinal_states, true, stream);
+                if (rc != CC1D_OK) return rc;
+            }
             allow_dynamic_smem(reinterpret_cast<const void *>(gdr_bwd_walks_kernel<T, kSteps>), kBytes);
-            launch_k(gdr_bwd_walks_kernel<T, kSteps>, dim3((unsigned)(2 * walks)), dim3(kWalkThreads), kBytes, stream, b, (const unsigned char *)images, records, (int)walks);
+            launch_k(gdr_bwd_walks_kernel<T, kSteps>, dim3((unsigned)(2 * walks)), dim3(kWalkThreads), kBytes, stream, b, (const unsigned char *)images, records, segs, (unsigned)walks);
             allow_dynamic_smem(reinterpret_cast<const void *>(gdr_grads_kernel<T, kSteps>), Grads<T>::kBytes);
             if (chunks > 0)
                 launch_k(gdr_grads_kernel<T, kSteps>, dim3((unsigned)chunks), dim3(kGradThreads), Grads<T>::kBytes, stream, b, (const unsigned char *)images, (const GdrRecord *)records);

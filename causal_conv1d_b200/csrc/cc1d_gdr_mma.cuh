@@ -324,11 +324,11 @@ template <typename T, int kN> struct GdrRows {
 constexpr int kFeeders = 64;
 // The last two warps of the forward walk: chunk after chunk into the stages.
 // bar_full counts the threads and the one that announces the image.
-template <typename T, int kStages, bool kKeep>
+template <typename T, int kStages, bool kBack, bool kWithP>
 __device__ __forceinline__ void feed_walk(const GdrRows<T, kFeeders> &rows, const unsigned char *images, int64_t image_step, uint32_t smem, int begin, int chunks,
                                           uint32_t bar_full, uint32_t bar_empty, volatile int *dead, int tid) {
-    using S = GdrStage<T, kKeep>;
-    constexpr uint32_t kBytes = kKeep ? S::kP - S::kT : S::kImage;      // what is kept needs no P
+    using S = GdrStage<T, kBack>;
+    constexpr uint32_t kBytes = kWithP ? S::kImage : S::kP - S::kT;      // without an output P is not needed
     for (int c = 0; c < chunks; ++c) {
         const int s = c % kStages;
         const uint32_t stage = smem + s * S::kBytes, full = bar_full + 8 * s;
@@ -350,6 +350,71 @@ __device__ __forceinline__ void feed_walk(const GdrRows<T, kFeeders> &rows, cons
 struct GdrRecord {
     float S0[kGdrMaxDim][kGdrMaxDim], U[kChunk][kGdrMaxDim], dS[kGdrMaxDim][kGdrMaxDim], dB[kChunk][kGdrMaxDim];
 };
+// ---- long sequences of few heads ------------------------------------------------------------------
+// A walk is one chain of chunks; where there are too few of them for the SMs, sequences are cut into segments
+// of `per` chunks.  Through a segment the state goes as S -> M S + B: a first launch walks every segment from
+// zeros (B) and, with no values, from the identity (M); the gradient of the state goes back as dS -> M^T dS +
+// back.  A small kernel then carries the states from segment to segment, and the real walks start from those.
+// per == 0: no segments, a walk is a whole sequence.
+struct GdrSegment {
+    float M[kGdrMaxDim][kGdrMaxDim], Mt[kGdrMaxDim][kGdrMaxDim], B[kGdrMaxDim][kGdrMaxDim], back[kGdrMaxDim][kGdrMaxDim];
+    float start[kGdrMaxDim][kGdrMaxDim], end[kGdrMaxDim][kGdrMaxDim];     // the state it starts from; the gradient of the one it ends with
+};
+struct GdrSegments { GdrSegment *at; int per; };
+
+// Segments of sequence n take slots gdr_first_segment(n) .., at least one each (as with the chunks' slots).
+__host__ __device__ inline int64_t gdr_segment_slots(const cc1d_gdr_params &p, int per) { return gdr_slots(p) / per + gdr_sequences(p); }
+__device__ __forceinline__ int64_t gdr_first_segment(const cc1d_gdr_params &p, const GdrSeq &seq, int n, int per) { return gdr_first_slot(p, seq, n) / per + n; }
+
+// What one walk covers
+struct GdrPart {
+    GdrSeq seq;               // its tokens
+    int n, chunks;
+    int64_t slot;             // of its first chunk
+    GdrSegment *segment;      // [heads_v], or NULL: the whole sequence
+    bool first, last;         // of the sequence
+};
+__device__ __forceinline__ int gdr_chunks(const GdrSeq &seq) { return (seq.end - seq.begin + kChunk - 1) / kChunk; }
+
+// False: nothing to walk (the whole CTA leaves)
+__device__ __forceinline__ bool gdr_find_part(const cc1d_gdr_params &p, const GdrSegments &segs, int64_t slot, GdrPart &w) {
+    const int sequences = (int)gdr_sequences(p);
+    w.segment = nullptr;
+    w.first = w.last = true;
+    if (segs.per == 0) {
+        w.n = (int)slot;
+        w.seq = {0, 0, 0};
+        w.slot = 0;
+        if (w.n < sequences) {
+            w.seq = gdr_sequence(p, w.n);
+            w.slot = gdr_first_slot(p, w.seq, w.n);
+        }
+        w.chunks = gdr_chunks(w.seq);
+        return true;
+    }
+    int n = 0, last = sequences - 1;            // the last sequence whose first slot is not behind this one
+    while (n < last) {
+        const int mid = (n + last + 1) / 2;
+        if (gdr_first_segment(p, gdr_sequence(p, mid), mid, segs.per) <= slot) n = mid; else last = mid - 1;
+    }
+    w.n = n;
+    w.seq = gdr_sequence(p, n);
+    const int chunks = gdr_chunks(w.seq), count = max(1, (chunks + segs.per - 1) / segs.per);
+    const int64_t i = slot - gdr_first_segment(p, w.seq, n, segs.per);
+    if (i < 0 || i >= count) return false;
+    w.slot = gdr_first_slot(p, w.seq, n) + i * segs.per;
+    w.segment = segs.at + slot * p.heads_v;
+    w.first = i == 0;
+    w.last = i + 1 == count;
+    const int64_t begin = (int64_t)w.seq.begin + i * segs.per * kChunk;
+    w.seq.end = (int32_t)min((int64_t)w.seq.end, begin + (int64_t)segs.per * kChunk);
+    w.seq.begin = (int32_t)begin;
+    w.chunks = gdr_chunks(w.seq);
+    return true;
+}
+
+int gdr_plan_segments(const cc1d_gdr_params &p, bool back);          // chunks of a segment, or 0
+int launch_gdr_join(const cc1d_gdr_params &p, const GdrSegments &segs, const float *dfinal_states, bool back, cudaStream_t stream);
 size_t gdr_image_bytes(const cc1d_gdr_params &p, bool back);          // of all chunks
 int launch_gdr_prep(const cc1d_gdr_params &p, bool back, void *images, cudaStream_t stream);
 

@@ -358,7 +358,101 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
     }
 }
 
+// ---- segments ----------------------------------------------------------------------------------------
+constexpr int kJoinColumns = 16;
+
+// One CTA carries 16 of the dim_v columns of one sequence and value head from segment to segment, in fp32:
+// start of the next = M start + B, or, back, end of the one before = M^T end + back.  Thread: one row of the
+// result and half of the sum; the matrix is read in the layout whose rows lie along the threads.
+__global__ void __launch_bounds__(256) gdr_join_kernel(const __grid_constant__ cc1d_gdr_params p, const GdrSegments segs, const float *dfinal_states, bool back) {
+    __shared__ float4 cur[kGdrMaxDim][kJoinColumns / 4], half_sum[kGdrMaxDim][kJoinColumns / 4];
+    pdl_wait();
+    const int groups = (int)(p.dim_v + kJoinColumns - 1) / kJoinColumns, heads = (int)p.heads_v, dk = (int)p.dim_k, dv = (int)p.dim_v;
+    const bool to_back = back && (blockIdx.x & 1);            // back: both directions, every other CTA
+    const unsigned id = back ? blockIdx.x >> 1 : blockIdx.x;
+    const int col0 = (int)(id % groups) * kJoinColumns, h = (int)(id / groups) % heads, n = (int)(id / groups) / heads;
+    const GdrSeq seq = gdr_sequence(p, n);
+    const int chunks = gdr_chunks(seq), count = max(1, (chunks + segs.per - 1) / segs.per);
+    if (count == 1) return;
+    GdrSegment *at = segs.at + gdr_first_segment(p, seq, n, segs.per) * heads + h;
+    const int tid = threadIdx.x, row = tid & 127, half = tid >> 7;
+    float *flat = reinterpret_cast<float *>(&cur[row][0]);
+    if (half == 0) {
+        const float *src = nullptr;
+        if (to_back) {
+            if (dfinal_states != nullptr) src = dfinal_states + ((int64_t)n * heads + h) * dk * dv;
+        } else {
+            const int64_t r = gdr_state_row(p, n);
+            if (p.initial_states != nullptr && r >= 0 && (p.has_initial_state == nullptr || p.has_initial_state[n] != 0))
+                src = p.initial_states + r * p.initial_states_batch_stride + h * p.initial_states_h_stride;
+        }
+        for (int c = 0; c < kJoinColumns; ++c) flat[c] = src != nullptr && row < dk && col0 + c < dv ? src[(int64_t)row * dv + col0 + c] : 0.f;
+    }
+    __syncthreads();
+    for (int i = 0; i + 1 < count; ++i) {
+        GdrSegment &s = at[(int64_t)(to_back ? count - 1 - i : i) * heads];
+        const float(*m)[kGdrMaxDim] = to_back ? s.M : s.Mt;
+        float4 sum[kJoinColumns / 4];
+        #pragma unroll
+        for (int c = 0; c < kJoinColumns / 4; ++c)
+            sum[c] = half == 0 ? *reinterpret_cast<const float4 *>(&(to_back ? s.back : s.B)[row][col0 + 4 * c]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        #pragma unroll 8
+        for (int k = 64 * half; k < 64 * half + 64; ++k) {
+            const float f = m[k][row];
+            #pragma unroll
+            for (int c = 0; c < kJoinColumns / 4; ++c) {
+                const float4 v = cur[k][c];
+                sum[c].x = fmaf(f, v.x, sum[c].x); sum[c].y = fmaf(f, v.y, sum[c].y); sum[c].z = fmaf(f, v.z, sum[c].z); sum[c].w = fmaf(f, v.w, sum[c].w);
+            }
+        }
+        if (half == 1) {
+            #pragma unroll
+            for (int c = 0; c < kJoinColumns / 4; ++c) half_sum[row][c] = sum[c];
+        }
+        __syncthreads();
+        if (half == 0) {
+            GdrSegment &next = at[(int64_t)(to_back ? count - 2 - i : i + 1) * heads];
+            #pragma unroll
+            for (int c = 0; c < kJoinColumns / 4; ++c) {
+                const float4 v = half_sum[row][c];
+                sum[c].x += v.x; sum[c].y += v.y; sum[c].z += v.z; sum[c].w += v.w;
+                cur[row][c] = sum[c];
+                *reinterpret_cast<float4 *>(&(to_back ? next.end : next.start)[row][col0 + 4 * c]) = sum[c];
+            }
+        }
+        __syncthreads();
+    }
+}
+
 }  // namespace
+
+// Times in us of a walk's chunk and of a join's step (measured, bf16, 128 x 128), for sequences of the mean length.
+// Cut where that is expected to save a quarter: one sequence of 32768 tokens and 4 heads, for example, is one
+// wave of 37 segments a head instead of 4 chains of 512 chunks.
+int gdr_plan_segments(const cc1d_gdr_params &p, bool back) {
+    const int64_t n = gdr_sequences(p), slots = gdr_slots(p);
+    if (n == 0 || slots == 0) return 0;
+    const int64_t mean = (slots + n - 1) / n, sms = num_sms(), heads = n * p.heads_v;
+    if (heads >= sms || mean < 8) return 0;
+    const int walks = back ? 2 : 1, sums = back ? 3 : 2;
+    const auto waves = [&](int64_t ctas) { return (double)((ctas + sms - 1) / sms); };
+    const double chunk = back ? 4.6 : 4.0, sum_chunk = back ? 4.2 : 3.6, step = 3.0, launches = 8.0;
+    double best = 0.75 * waves(walks * heads) * (double)mean * chunk;
+    int per = 0;
+    for (int64_t count = 2; count <= 64 && count * 2 <= mean; ++count) {
+        const int64_t m = (mean + count - 1) / count, segments = (mean + m - 1) / m;
+        const double t = launches + waves(sums * heads * (segments - 1)) * (double)m * sum_chunk + step * (double)segments + waves(walks * heads * segments) * (double)m * chunk;
+        if (t < best) { best = t; per = (int)m; }
+    }
+    return per;
+}
+
+int launch_gdr_join(const cc1d_gdr_params &p, const GdrSegments &segs, const float *dfinal_states, bool back, cudaStream_t stream) {
+    const int64_t ctas = gdr_sequences(p) * p.heads_v * ((p.dim_v + kJoinColumns - 1) / kJoinColumns) * (back ? 2 : 1);
+    if (ctas >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
+    launch_k(gdr_join_kernel, dim3((unsigned)ctas), dim3(256), 0, stream, p, segs, dfinal_states, back);
+    return check_launch();
+}
 
 size_t gdr_image_bytes(const cc1d_gdr_params &p, bool back) {
     size_t one = 0;

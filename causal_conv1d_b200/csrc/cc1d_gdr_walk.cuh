@@ -17,8 +17,9 @@ constexpr uint32_t kFwdColX = 288;    // 64: S^T K^T, then R^T (T - I)^T, then U
 constexpr uint32_t kFwdColO = 352;    // 64: S^T Q^T
 __device__ __forceinline__ uint32_t col_u(int piece) { return piece < 2 ? kFwdColU + 32 * piece : 480; }
 
-template <typename T, bool kKeep> struct Fwd {
-    using S = GdrStage<T, kKeep>;
+enum GdrMode { kOutput, kKeep, kSummary };
+template <typename T, bool kBack> struct Fwd {
+    using S = GdrStage<T, kBack>;
     static constexpr int kStages = S::kPieces == 1 ? 2 : 1;
     static constexpr uint32_t kBars = kStages * S::kBytes, kBytes = kBars + 128 + 1024;
 };
@@ -32,10 +33,13 @@ template <typename T, bool kKeep> struct Fwd {
 // computes passes through shared memory.  S itself is kept and decayed in fp32 registers; only
 // its pieces are rewritten every chunk.
 // kKeep: the backward's walk, which leaves S and U of every chunk in its record instead of an output.
-template <typename T, int kSteps, bool kKeep>
-__device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const unsigned char *images, GdrRecord *records, int block) {
-    using L = Fwd<T, kKeep>;
-    using St = GdrStage<T, kKeep>;
+// kSummary: what a segment does to the state: from zeros its last state B, or (unit) without values from the
+// identity, dim_k columns instead of dim_v, its M.
+template <typename T, int kSteps, GdrMode kMode, bool kBack>
+__device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const unsigned char *images, GdrRecord *records, const GdrSegments &segs, int64_t block, bool unit) {
+    constexpr bool kOut = kMode == kOutput;
+    using L = Fwd<T, kBack>;
+    using St = GdrStage<T, kBack>;
     constexpr int NP = St::kPieces, PO = GdrType<T>::kOutPieces, PT = St::kSolve;
     extern __shared__ unsigned char raw[];
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -45,6 +49,14 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
     volatile int *dead = reinterpret_cast<volatile int *>(smem + L::kBars + 120);
     uint32_t *slot = reinterpret_cast<uint32_t *>(smem + L::kBars + 124);
     const int tid = threadIdx.x, warp = __shfl_sync(kFullMask, tid >> 5, 0), lane = tid & 31;
+    pdl_wait();
+    const int heads = (int)p.heads_v, h = (int)(block % heads), sequences = (int)gdr_sequences(p);
+    GdrPart w;
+    if (!gdr_find_part(p, segs, block / heads, w)) return;
+    // B of a last segment leads nowhere, nor does M of one that is alone (or, forwards, of a last one)
+    if (kMode == kSummary && (unit ? (kBack ? w.first && w.last : w.last) : w.last)) return;
+    const GdrSeq seq = w.seq;
+    const int n = w.n, chunks = w.chunks, dk = (int)p.dim_k, dv = kMode == kSummary && unit ? dk : (int)p.dim_v;
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) { mbar_init(bar_full + 8 * s, kFeeders + 1); mbar_init(bar_empty + 8 * s, 1); }
         mbar_init(bar_x, 1); mbar_init(bar_u, 1); mbar_init(bar_o, 1); mbar_init(bar_d, 1);
@@ -52,18 +64,10 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
         *dead = 0;
         fence_mbar_init();
     }
-    pdl_wait();
     if (warp == 0) tmem_alloc512(smem_u32(slot));
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-
-    const int heads = (int)p.heads_v, h = block % heads, n = block / heads;
-    const int sequences = (int)gdr_sequences(p);
-    GdrSeq seq = {0, 0, 0};
-    if (n < sequences) seq = gdr_sequence(p, n);
-    const int chunks = (seq.end - seq.begin + kChunk - 1) / kChunk;
-    const int dk = (int)p.dim_k, dv = (int)p.dim_v;
 
     if (warp == kWalkers / 32) {
         // issues the walk's products: a thread that issues is held up while earlier ones still run,
@@ -94,7 +98,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 mma_commit(bar_x);
                 more = false;
                 #pragma unroll
-                for (int o = kKeep ? -1 : PO - 1; o >= 0; --o) {
+                for (int o = kOut ? PO - 1 : -1; o >= 0; --o) {
                     #pragma unroll
                     for (int a = 0; a <= o; ++a) {
                         const int b = o - a;
@@ -142,7 +146,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 mma_commit(bar_d);
                 more = false;
                 #pragma unroll
-                for (int o = kKeep ? -1 : PO - 1; o >= 0; --o) {
+                for (int o = kOut ? PO - 1 : -1; o >= 0; --o) {
                     #pragma unroll
                     for (int a = 0; a <= o; ++a) {
                         const int b = o - a;
@@ -166,7 +170,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             gdr_wait(bar_out, c & 1, dead);
             __syncwarp();
             const int rows = min(kChunk, seq.end - seq.begin - c * kChunk);
-            if (!kKeep && at < dv) {
+            if (kOut && at < dv) {
                 #pragma unroll 8
                 for (int i = lane / kLanes; i < rows; i += kRows) {
                     const uint4 v = *reinterpret_cast<const uint4 *>(V + (i * kGdrMaxDim + at) * sizeof(T));
@@ -177,9 +181,10 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             if (lane == 0) mbar_arrive(bar_empty + 8 * (c % L::kStages));
         }
     } else if (warp > kWalkers / 32) {
-        const GdrRows<T, kFeeders> rows(p, seq, h, p.v, seq.row * p.v_batch_stride + h * p.v_h_stride, p.v_l_stride);
+        GdrRows<T, kFeeders> rows(p, seq, h, p.v, seq.row * p.v_batch_stride + h * p.v_h_stride, p.v_l_stride);
         const int64_t step = (int64_t)heads * St::kImage;
-        feed_walk<T, L::kStages, kKeep>(rows, images + gdr_first_slot(p, seq, n) * step + h * (int64_t)St::kImage, step, smem_u32(smem), seq.begin, chunks,
+        if (kMode == kSummary && unit) rows.dv = 0;
+        feed_walk<T, L::kStages, kBack, kOut>(rows, images + w.slot * step + h * (int64_t)St::kImage, step, smem_u32(smem), seq.begin, chunks,
                                         bar_full, bar_empty, dead, tid - kWalkers - 64);
     } else {
         const int quad = warp & 3, part = warp >> 2, col = quad * 32 + lane;   // part: a quarter of the dim_k and of the tokens
@@ -187,7 +192,13 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
         const int64_t row = n < sequences ? gdr_state_row(p, n) : -1;
         const int64_t state_at = (int64_t)(32 * part) * dv + col;
         float S[32];
-        {
+        if (kMode == kSummary) {
+            #pragma unroll
+            for (int j = 0; j < 32; ++j) S[j] = unit && 32 * part + j == col ? 1.f : 0.f;
+        } else if (!w.first) {
+            #pragma unroll
+            for (int j = 0; j < 32; ++j) S[j] = w.segment[h].start[32 * part + j][col];
+        } else {
             const bool from = p.initial_states != nullptr && row >= 0 && (p.has_initial_state == nullptr || p.has_initial_state[n] != 0);
             const float *src = p.initial_states + row * p.initial_states_batch_stride + h * p.initial_states_h_stride + state_at;
             #pragma unroll
@@ -200,9 +211,9 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        GdrRecord *record = kKeep ? records + gdr_first_slot(p, seq, n) * heads + h : nullptr;
+        GdrRecord *record = kMode == kKeep ? records + w.slot * heads + h : nullptr;
         auto put_state = [&]() {
-            if (kKeep) {
+            if (kMode == kKeep) {
                 #pragma unroll
                 for (int j = 0; j < 32; ++j) record->S0[32 * part + j][col] = S[j];
             }
@@ -258,11 +269,11 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     const float2 v = add2(make_float2(x[j], x[j + 1]), make_float2(R[j], R[j + 1]));
                     x[j] = v.x; x[j + 1] = v.y;
                 }
-                if (kKeep) {
+                if (kMode == kKeep) {
                     #pragma unroll
                     for (int j = 0; j < 16; ++j) record->U[first + j][col] = x[j];
                     record += heads;
-                } else {
+                } else if (kOut) {
                     #pragma unroll
                     for (int j = 0; j < 16; j += 8) split8_to_tmem<PO>(x + j, mine + kFwdColU + first / 2 + j / 2, 32, 480 - kFwdColU);
                 }
@@ -291,7 +302,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 }
             }
             // the output is taken out of tensor memory before the next chunk's products go there
-            if (!kKeep) {
+            if (kOut) {
                 gdr_wait(bar_o, par, dead);
                 __syncwarp();
                 fence_after_sync();
@@ -318,13 +329,25 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             fence_after_sync();
             if (c + 1 < chunks) put_state();
         }
-        if (!kKeep && p.final_states != nullptr && row >= 0) {
+        if (kMode == kSummary) {
+            GdrSegment &to = w.segment[h];
+            if (unit) {
+                #pragma unroll
+                for (int j = 0; j < 32; ++j) to.M[32 * part + j][col] = S[j];
+                #pragma unroll
+                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(&to.Mt[col][32 * part + j]) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+            } else {
+                #pragma unroll
+                for (int j = 0; j < 32; ++j) to.B[32 * part + j][col] = S[j];
+            }
+        }
+        if (kOut && w.last && p.final_states != nullptr && row >= 0) {
             float *dst = p.final_states + row * p.final_states_batch_stride + h * p.final_states_h_stride + state_at;
             #pragma unroll
             for (int j = 0; j < 32; ++j) if (32 * part + j < dk && col < dv) dst[(int64_t)j * dv] = S[j];
         }
         // tokens that belong to no sequence
-        if (!kKeep && p.cu_seqlens != nullptr && n + 1 >= sequences) {
+        if (kOut && w.last && p.cu_seqlens != nullptr && n + 1 >= sequences) {
             for (int64_t t = seq.end + part; t < p.seqlen; t += 4)
                 if (col < dv) out[t * p.out_l_stride] = Elem<T>::from_f(0.f);
         }

@@ -177,3 +177,13 @@ def test_strided_slices_of_a_conv_output():
     want = expect(q, k, v, g, beta, [T] * B, torch.zeros(B, hv, dk, dv), torch.ones(B, T, hv, dv), torch.zeros(B, hv, dk, dv), dk ** -0.5)
     gdr_ref.close(out.flatten(0, 1), want[0], TOL, "out", torch.bfloat16)
     gdr_ref.close(x.grad[..., 2 * hk * dk:].unflatten(-1, (hv, dv)).flatten(0, 1), want[2][2], TOL, "dv", torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype,slow", [("bf16", True), ("fp32", True), ("fp16", False)])
+def test_long_sequences_of_few_heads(dtype, slow):
+    """Cut into segments that are walked side by side: lengths that end inside, at and just behind a segment."""
+    check([2048, 1000, 0, 1, 1985], 1, 2, 64, 32, DT[dtype], True, 7, slow=slow, seed=1)
+
+
+def test_one_long_row():
+    check([2500], 1, 1, 128, 128, torch.bfloat16, False, slow=True, seed=2)

@@ -80,3 +80,10 @@ def test_many_sequences_more_than_resident():
 
 def test_slow_decay_long():
     check([3000], 1, 2, 128, 128, torch.bfloat16, slow=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("lens", [[4000], [64 * 40, 1, 64 * 17 + 1, 0, 900, 64 * 13 - 1]])
+def test_long_sequences_of_few_heads(dtype, lens):
+    """Cut into segments that are walked side by side, with states that last through all of them."""
+    check(lens, 1, 2, 96, 72, DT[dtype], 3, slow=True, seed=len(lens))
