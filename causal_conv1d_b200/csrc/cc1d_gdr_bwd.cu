@@ -25,7 +25,7 @@ template <typename T> struct Back {
     static constexpr int kStages = S::kPieces == 1 ? 2 : 1;
     static constexpr uint32_t kDoPiece = 16384, kDo = S::kPieces * S::kKqPiece, kT = kDo + S::kPieces * kDoPiece, kGates = kT + (S::kGates - S::kT),
                               kP = kT + (S::kP - S::kT), kStage = kT + S::kImage;
-    static constexpr uint32_t kBars = kStages * kStage, kBytes = kBars + 128 + 1024;
+    static constexpr uint32_t kBars = kStages * kStage, kBytes = kBars + 128 + sizeof(GdrPart) + 1024;
     static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
 
@@ -56,7 +56,10 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
     const GdrSeq seq = w.seq;
     const int n = w.n, chunks = w.chunks, dk = (int)p.dim_k, dv = (int)p.dim_v;
     const int64_t first_slot = w.slot;
+    // what the walkers need again at their end (kept in registers over the walk it makes them spill)
+    volatile GdrPart *kept = reinterpret_cast<volatile GdrPart *>(smem + L::kBars + 128);
     if (tid == 0) {
+        kept->n = w.n; kept->seq.end = w.seq.end; kept->segment = w.segment; kept->first = w.first; kept->last = w.last;
         for (int s = 0; s < 2; ++s) { mbar_init(bar_full + 8 * s, kFeeders + 1); mbar_init(bar_empty + 8 * s, kWalkers / 32); }
         mbar_init(bar_x, 1); mbar_init(bar_u, 1); mbar_init(bar_d, 1);
         mbar_init(bar_s, kWalkers / 32); mbar_init(bar_e, kWalkers / 32); mbar_init(bar_r, kWalkers / 32); mbar_init(bar_w, kWalkers / 32);
@@ -185,12 +188,14 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
     } else if (warp < kWalkers / 32) {
         const int quad = warp & 3, part = warp >> 2, col = quad * 32 + lane;   // part: a quarter of the dim_k and of the tokens
         const uint32_t mine = (uint32_t)(quad * 32) << 16;
-        const int64_t state_at = ((int64_t)n * heads + h) * dk * dv + (int64_t)(32 * part) * dv + col;
         float S[32];
-        #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            S[j] = kSum ? 0.f : !w.last ? w.segment[h].end[32 * part + j][col]
-                 : b.dfinal_states != nullptr && n < sequences && 32 * part + j < dk && col < dv ? b.dfinal_states[state_at + (int64_t)j * dv] : 0.f;
+        {
+            const int64_t state_at = ((int64_t)n * heads + h) * dk * dv + (int64_t)(32 * part) * dv + col;
+            #pragma unroll
+            for (int j = 0; j < 32; ++j)
+                S[j] = kSum ? 0.f : !w.last ? w.segment[h].end[32 * part + j][col]
+                     : b.dfinal_states != nullptr && n < sequences && 32 * part + j < dk && col < dv ? b.dfinal_states[state_at + (int64_t)j * dv] : 0.f;
+        }
         auto ready = [&](uint32_t bar) {
             tmem_wait_st();
             fence_before_sync();
@@ -285,28 +290,31 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
             fence_after_sync();
             if (i + 1 < chunks) put_state();
         }
+        const int head = (int)(block % heads), at = kept->n, all = (int)gdr_sequences(p);
         if (kSum) {
+            GdrSegment &to = kept->segment[head];
             #pragma unroll
-            for (int j = 0; j < 32; ++j) w.segment[h].back[32 * part + j][col] = S[j];
+            for (int j = 0; j < 32; ++j) to.back[32 * part + j][col] = S[j];
         }
-        if (!kSum && w.first && b.dinitial_states != nullptr && n < sequences) {
-            const bool from = p.initial_states != nullptr && gdr_state_row(p, n) >= 0 && (p.has_initial_state == nullptr || p.has_initial_state[n] != 0);
+        if (!kSum && kept->first && b.dinitial_states != nullptr && at < all) {
+            const int64_t state_at = ((int64_t)at * heads + head) * dk * dv + (int64_t)(32 * part) * dv + col;
+            const bool from = p.initial_states != nullptr && gdr_state_row(p, at) >= 0 && (p.has_initial_state == nullptr || p.has_initial_state[at] != 0);
             #pragma unroll
             for (int j = 0; j < 32; ++j)
                 if (32 * part + j < dk && col < dv) b.dinitial_states[state_at + (int64_t)j * dv] = from ? S[j] : 0.f;
         }
         // tokens that belong to no sequence
-        if (!kSum && w.last && p.cu_seqlens != nullptr && n + 1 >= sequences) {
+        if (!kSum && kept->last && p.cu_seqlens != nullptr && at + 1 >= all) {
             const int group = heads / (int)p.heads_k;
-            for (int64_t t = seq.end + part; t < p.seqlen; t += 4) {
-                if (col < dv) reinterpret_cast<T *>(b.dv)[(t * heads + h) * dv + col] = Elem<T>::from_f(0.f);
-                if (h % group == 0 && col < dk) {
-                    reinterpret_cast<T *>(b.dq)[(t * p.heads_k + h / group) * dk + col] = Elem<T>::from_f(0.f);
-                    reinterpret_cast<T *>(b.dk)[(t * p.heads_k + h / group) * dk + col] = Elem<T>::from_f(0.f);
+            for (int64_t t = kept->seq.end + part; t < p.seqlen; t += 4) {
+                if (col < dv) reinterpret_cast<T *>(b.dv)[(t * heads + head) * dv + col] = Elem<T>::from_f(0.f);
+                if (head % group == 0 && col < dk) {
+                    reinterpret_cast<T *>(b.dq)[(t * p.heads_k + head / group) * dk + col] = Elem<T>::from_f(0.f);
+                    reinterpret_cast<T *>(b.dk)[(t * p.heads_k + head / group) * dk + col] = Elem<T>::from_f(0.f);
                 }
                 if (col == 0) {
-                    store_any(b.dg, t * heads + h, p.gtype, 0.f);
-                    store_any(b.dbeta, t * heads + h, p.btype, 0.f);
+                    store_any(b.dg, t * heads + head, p.gtype, 0.f);
+                    store_any(b.dbeta, t * heads + head, p.btype, 0.f);
                 }
             }
         }

@@ -209,23 +209,24 @@ constexpr int kThreads = 128;
 
 template <typename T, bool kBack> struct Prep {
     using S = GdrStage<T, kBack>;
-    // the image takes the place of K and Q once their product is there; its gates lie beside them till then
-    static constexpr uint32_t kTiles = S::kPieces * S::kKqPiece, kImageTiles = S::kImage;
-    static constexpr uint32_t kInv = kTiles > kImageTiles ? kTiles : kImageTiles, kBars = kInv + kChunk * kLd * 4, kGates = kBars + 64, kBytes = kGates + 4096 + 1024;
+    // what is computed takes the place of K and Q once their product is there: A and its inverse that of T, P its own;
+    // the gates lie beside them till the end
+    static constexpr uint32_t kTiles = S::kPieces * S::kKqPiece, kGates = kTiles > S::kImage ? kTiles : S::kImage, kBars = kGates + 3072, kBytes = kBars + 64 + 1024;
+    static_assert(kChunk * kLd * 4 <= S::kP - S::kT, "A in the place of T and the image's gates");
 };
 
 // One CTA makes one chunk of one value head: K K^T and Q K^T by one MMA with the 128 rows [K; Q], then
 // warps 0, 1 the rows of A and warps 2, 3 those of P, the inverse, and the image out by one bulk copy.
-// A chain of short dependent steps: what fills the SM is that four CTAs (bf16) share it.
+// A chain of short dependent steps: what fills the SM is that five CTAs share it (bf16).
 template <typename T, int kSteps, bool kBack>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : sizeof(T) == 2 && GdrType<T>::kPieces == 1 ? 4 : 2)
+__global__ void __launch_bounds__(kThreads, 5)
 gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images) {
     using S = GdrStage<T, kBack>;
     using L = Prep<T, kBack>;
     constexpr int NP = S::kPieces;
     extern __shared__ unsigned char raw[];
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-    float *inv = reinterpret_cast<float *>(smem + L::kInv);
+    float *inv = reinterpret_cast<float *>(smem);
     GdrGates &gates = *reinterpret_cast<GdrGates *>(smem + L::kGates);
     const uint32_t base = smem_u32(smem), bar = base + L::kBars;
     volatile int *dead = reinterpret_cast<volatile int *>(smem + L::kBars + 8);
@@ -332,26 +333,31 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
     __syncthreads();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 64;" :: "r"(tmem) : "memory");
     invert_unit_lower(inv, warp, lane);
+    float x[2][16];
     #pragma unroll
     for (int half = 0; half < 2; ++half) {
         const int i = (tid >> 2) + 32 * half, j0 = (tid & 3) * 16;
-        float x[16];
         #pragma unroll
         for (int j = 0; j < 16; j += 4) {
             const float4 v = j0 <= i ? *reinterpret_cast<const float4 *>(inv + i * kLd + j0 + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
+            x[half][j] = v.x; x[half][j + 1] = v.y; x[half][j + 2] = v.z; x[half][j + 3] = v.w;
         }
+    }
+    __syncthreads();                   // the pieces of T go where the inverse lay
+    #pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int i = (tid >> 2) + 32 * half, j0 = (tid & 3) * 16;
         #pragma unroll
-        for (int j = 0; j < 16; ++j) if (j0 + j == i) x[j] = 0.f;      // T - I
+        for (int j = 0; j < 16; ++j) if (j0 + j == i) x[half][j] = 0.f;      // T - I
         #pragma unroll
-        for (int j = 0; j < 16; j += 8) store_pieces8<S::kSolve>(x + j, base + tile_at(i, (j0 + j) / 8, 0));
+        for (int j = 0; j < 16; j += 8) store_pieces8<S::kSolve>(x[half] + j, base + tile_at(i, (j0 + j) / 8, 0));
     }
     fence_proxy_async_smem();
     __syncthreads();
     if (tid == 0) {
         unsigned char *image = images + (slot * heads + h) * (int64_t)S::kImage;
         bulk_store(image, base, S::kSolve * 8192);
-        bulk_store(image + S::kSolve * 8192, base + L::kGates, 4096);
+        bulk_store(image + S::kSolve * 8192, base + L::kGates, 3072);
         bulk_store(image + (S::kP - S::kT), base + (S::kP - S::kT), S::kOut * 8192);
         bulk_commit();
         bulk_wait_read();

@@ -13,15 +13,16 @@ constexpr uint32_t kFwdColS = 0;      // 3 x 64: pieces of S^T, two dim_k per co
 constexpr uint32_t kFwdColDelta = 0;  //   128: U''^T K, and
 constexpr uint32_t kFwdColU = 128;    //   2 x 32: pieces of U^T (the third, fp32 inputs only, at 480)
 constexpr uint32_t kFwdColR = 192;    // 3 x 32: pieces of R^T, then of U''^T
-constexpr uint32_t kFwdColX = 288;    // 64: S^T K^T, then R^T (T - I)^T, then U^T P^T
+constexpr uint32_t kFwdColX = 288;    // 64: S^T K^T, then R^T (T - I)^T
 constexpr uint32_t kFwdColO = 352;    // 64: S^T Q^T
+constexpr uint32_t kFwdColY = 416;    // 64: U^T P^T
 __device__ __forceinline__ uint32_t col_u(int piece) { return piece < 2 ? kFwdColU + 32 * piece : 480; }
 
 enum GdrMode { kOutput, kKeep, kSummary };
 template <typename T, bool kBack> struct Fwd {
     using S = GdrStage<T, kBack>;
     static constexpr int kStages = S::kPieces == 1 ? 2 : 1;
-    static constexpr uint32_t kBars = kStages * S::kBytes, kBytes = kBars + 128 + 1024;
+    static constexpr uint32_t kBars = kStages * S::kBytes, kBytes = kBars + 128 + sizeof(GdrPart) + 1024;
 };
 
 // One CTA walks one sequence of one value head, chunk by chunk, with S^T (dim_v x dim_k) in the
@@ -57,7 +58,10 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
     if (kMode == kSummary && (unit ? (kBack ? w.first && w.last : w.last) : w.last)) return;
     const GdrSeq seq = w.seq;
     const int n = w.n, chunks = w.chunks, dk = (int)p.dim_k, dv = kMode == kSummary && unit ? dk : (int)p.dim_v;
+    // what the walkers need again at their end (kept in registers over the walk it makes them spill)
+    volatile GdrPart *kept = reinterpret_cast<volatile GdrPart *>(smem + L::kBars + 128);
     if (tid == 0) {
+        kept->n = w.n; kept->seq.end = w.seq.end; kept->segment = w.segment; kept->last = w.last;
         for (int s = 0; s < 2; ++s) { mbar_init(bar_full + 8 * s, kFeeders + 1); mbar_init(bar_empty + 8 * s, 1); }
         mbar_init(bar_x, 1); mbar_init(bar_u, 1); mbar_init(bar_o, 1); mbar_init(bar_d, 1);
         mbar_init(bar_s, kWalkers / 32); mbar_init(bar_r, kWalkers / 32); mbar_init(bar_w, kWalkers / 32); mbar_init(bar_out, kWalkers / 32);
@@ -96,7 +100,13 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     }
                 }
                 mma_commit(bar_x);
-                more = false;
+            }
+            __syncwarp();
+            if (kOut && c > 0) gdr_wait(bar_out, (c - 1) & 1, dead);      // the columns of S^T Q^T have been read
+            __syncwarp();
+            if (kOut && elect_one()) {
+                fence_after_sync();
+                bool more = false;
                 #pragma unroll
                 for (int o = kOut ? PO - 1 : -1; o >= 0; --o) {
                     #pragma unroll
@@ -152,7 +162,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                         const int b = o - a;
                         if (a >= PO || b >= PO) continue;
                         #pragma unroll
-                        for (int i = 0; i < 4; ++i) mma_ts(kFwdColX, col_u(a) + 8 * i, desc_add(kq, St::kP + b * 8192 + 32 * i), id, again(more));
+                        for (int i = 0; i < 4; ++i) mma_ts(kFwdColY, col_u(a) + 8 * i, desc_add(kq, St::kP + b * 8192 + 32 * i), id, again(more));
                     }
                 }
                 mma_commit(bar_o);
@@ -189,8 +199,6 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
     } else {
         const int quad = warp & 3, part = warp >> 2, col = quad * 32 + lane;   // part: a quarter of the dim_k and of the tokens
         const uint32_t mine = (uint32_t)(quad * 32) << 16;
-        const int64_t row = n < sequences ? gdr_state_row(p, n) : -1;
-        const int64_t state_at = (int64_t)(32 * part) * dv + col;
         float S[32];
         if (kMode == kSummary) {
             #pragma unroll
@@ -199,6 +207,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             #pragma unroll
             for (int j = 0; j < 32; ++j) S[j] = w.segment[h].start[32 * part + j][col];
         } else {
+            const int64_t row = n < sequences ? gdr_state_row(p, n) : -1, state_at = (int64_t)(32 * part) * dv + col;
             const bool from = p.initial_states != nullptr && row >= 0 && (p.has_initial_state == nullptr || p.has_initial_state[n] != 0);
             const float *src = p.initial_states + row * p.initial_states_batch_stride + h * p.initial_states_h_stride + state_at;
             #pragma unroll
@@ -222,7 +231,6 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             ready(bar_s);
         };
         if (chunks > 0) put_state();
-        T *out = reinterpret_cast<T *>(p.out) + seq.row * p.out_batch_stride + h * p.out_h_stride + col;
         for (int c = 0; c < chunks; ++c) {
             const int s = c % L::kStages;
             const uint32_t par = c & 1;
@@ -301,7 +309,11 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     S[16 * b + j] = v.x; S[16 * b + j + 1] = v.y;
                 }
             }
-            // the output is taken out of tensor memory before the next chunk's products go there
+            fence_before_sync();
+            walk_sync<kWalkers>();                      // every thread has read its part of Delta
+            fence_after_sync();
+            if (c + 1 < chunks) put_state();
+            // the output, while the next chunk's first product runs
             if (kOut) {
                 gdr_wait(bar_o, par, dead);
                 __syncwarp();
@@ -310,7 +322,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 for (int b = 0; b < 16; b += 8) {
                     float x[8], y[8];
                     tmem_ld<8>(x, mine + kFwdColO + first + b);
-                    tmem_ld<8>(y, mine + kFwdColX + first + b);
+                    tmem_ld<8>(y, mine + kFwdColY + first + b);
                     tmem_wait_ld();
                     #pragma unroll
                     for (int j = 0; j < 8; j += 4) {
@@ -322,15 +334,13 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     for (int j = 0; j < 8; ++j) V[(b + j) * kGdrMaxDim] = Elem<T>::from_f(p.scale * x[j]);   // where this thread read its v
                 }
             }
+            fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_out);
-            fence_before_sync();
-            walk_sync<kWalkers>();                      // every thread has read its part of Delta
-            fence_after_sync();
-            if (c + 1 < chunks) put_state();
         }
+        const int head = (int)(block % heads);
         if (kMode == kSummary) {
-            GdrSegment &to = w.segment[h];
+            GdrSegment &to = kept->segment[head];
             if (unit) {
                 #pragma unroll
                 for (int j = 0; j < 32; ++j) to.M[32 * part + j][col] = S[j];
@@ -341,15 +351,20 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 for (int j = 0; j < 32; ++j) to.B[32 * part + j][col] = S[j];
             }
         }
-        if (kOut && w.last && p.final_states != nullptr && row >= 0) {
-            float *dst = p.final_states + row * p.final_states_batch_stride + h * p.final_states_h_stride + state_at;
-            #pragma unroll
-            for (int j = 0; j < 32; ++j) if (32 * part + j < dk && col < dv) dst[(int64_t)j * dv] = S[j];
-        }
-        // tokens that belong to no sequence
-        if (kOut && w.last && p.cu_seqlens != nullptr && n + 1 >= sequences) {
-            for (int64_t t = seq.end + part; t < p.seqlen; t += 4)
-                if (col < dv) out[t * p.out_l_stride] = Elem<T>::from_f(0.f);
+        if (kOut && kept->last) {
+            const int at = kept->n, all = (int)gdr_sequences(p);
+            const int64_t row = at < all ? gdr_state_row(p, at) : -1;
+            if (p.final_states != nullptr && row >= 0) {
+                float *dst = p.final_states + row * p.final_states_batch_stride + head * p.final_states_h_stride + (int64_t)(32 * part) * dv + col;
+                #pragma unroll
+                for (int j = 0; j < 32; ++j) if (32 * part + j < dk && col < dv) dst[(int64_t)j * dv] = S[j];
+            }
+            // tokens that belong to no sequence
+            if (p.cu_seqlens != nullptr && at + 1 >= all) {
+                T *out = reinterpret_cast<T *>(p.out) + head * p.out_h_stride + col;
+                for (int64_t t = kept->seq.end + part; t < p.seqlen; t += 4)
+                    if (col < dv) out[t * p.out_l_stride] = Elem<T>::from_f(0.f);
+            }
         }
     }
     fence_before_sync();
