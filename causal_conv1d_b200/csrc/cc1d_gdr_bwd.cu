@@ -52,7 +52,7 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
     pdl_wait();
     const int heads = (int)p.heads_v, h = (int)(block % heads), sequences = (int)gdr_sequences(p);
     GdrPart w;
-    if (!gdr_find_part(p, segs, block / heads, w) || (kSum && w.first)) return;
+    if (!gdr_find_part(p, segs, segs.ranked ? gdr_ranked(p, (int)(block / heads), reinterpret_cast<int *>(smem)) : block / heads, w) || (kSum && w.first)) return;
     const GdrSeq seq = w.seq;
     const int n = w.n, chunks = w.chunks, dk = (int)p.dim_k, dv = (int)p.dim_v;
     const int64_t first_slot = w.slot;
@@ -325,9 +325,9 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
 }
 
 template <typename T, int kSteps>
-__global__ void __launch_bounds__(kWalkThreads, 1) gdr_bwd_walks_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, GdrRecord *records, const GdrSegments segs, unsigned walks) {
-    if (blockIdx.x < walks) walk_back<T, kSteps, false>(b, images, records, segs, blockIdx.x);
-    else walk_forward<T, kSteps, kKeep, true>(b.fwd, images, records, segs, blockIdx.x - walks, false);
+__global__ void __launch_bounds__(kWalkThreads, 1) gdr_bwd_walks_kernel(const __grid_constant__ cc1d_gdr_bwd_params b, const unsigned char *images, GdrRecord *records, const GdrSegments segs) {
+    if (blockIdx.x & 1) walk_forward<T, kSteps, kKeep, true>(b.fwd, images, records, segs, blockIdx.x >> 1, false);
+    else walk_back<T, kSteps, false>(b, images, records, segs, blockIdx.x >> 1);
 }
 
 // a third of the CTAs each: the gradient's walk from zeros, the state's, M
@@ -759,10 +759,11 @@ int launch_gdr_bwd(const cc1d_gdr_bwd_params &b, cudaStream_t stream) {
     const cc1d_gdr_params &p = b.fwd;
     unsigned char *images = reinterpret_cast<unsigned char *>(b.workspace);
     GdrRecord *records = reinterpret_cast<GdrRecord *>(images + images_bytes(p));
-    const GdrSegments segs = {reinterpret_cast<GdrSegment *>(images + images_bytes(p) + records_bytes(p)), gdr_plan_segments(p, true)};
+    GdrSegments segs = {reinterpret_cast<GdrSegment *>(images + images_bytes(p) + records_bytes(p)), gdr_plan_segments(p, true), false};
     const int64_t sequences = gdr_sequences(p), chunks = gdr_slots(p) * p.heads_k;
     const int64_t walks = (segs.per > 0 ? gdr_segment_slots(p, segs.per) : sequences > 0 ? sequences : 1) * p.heads_v;
     if (walks >= (1ll << 29) || chunks >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
+    segs.ranked = gdr_rank_walks(p, segs.per, 2 * walks);
     int rc = launch_gdr_prep(p, true, images, stream);
     if (rc != CC1D_OK) return rc;
     CC1D_DISPATCH_ITYPE(p.itype, {
@@ -776,7 +777,7 @@ int launch_gdr_bwd(const cc1d_gdr_bwd_params &b, cudaStream_t stream) {
                 if (rc != CC1D_OK) return rc;
             }
             allow_dynamic_smem(reinterpret_cast<const void *>(gdr_bwd_walks_kernel<T, kSteps>), kBytes);
-            launch_k(gdr_bwd_walks_kernel<T, kSteps>, dim3((unsigned)(2 * walks)), dim3(kWalkThreads), kBytes, stream, b, (const unsigned char *)images, records, segs, (unsigned)walks);
+            launch_k(gdr_bwd_walks_kernel<T, kSteps>, dim3((unsigned)(2 * walks)), dim3(kWalkThreads), kBytes, stream, b, (const unsigned char *)images, records, segs);
             allow_dynamic_smem(reinterpret_cast<const void *>(gdr_grads_kernel<T, kSteps>), Grads<T>::kBytes);
             if (chunks > 0)
                 launch_k(gdr_grads_kernel<T, kSteps>, dim3((unsigned)chunks), dim3(kGradThreads), Grads<T>::kBytes, stream, b, (const unsigned char *)images, (const GdrRecord *)records);

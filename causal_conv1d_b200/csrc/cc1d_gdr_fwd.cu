@@ -27,9 +27,10 @@ size_t gdr_fwd_workspace_bytes(const cc1d_gdr_params &p) {
 
 int launch_gdr_fwd(const cc1d_gdr_params &p, cudaStream_t stream) {
     unsigned char *images = reinterpret_cast<unsigned char *>(p.workspace);
-    const GdrSegments segs = {reinterpret_cast<GdrSegment *>(images + images_bytes(p)), gdr_plan_segments(p, false)};
+    GdrSegments segs = {reinterpret_cast<GdrSegment *>(images + images_bytes(p)), gdr_plan_segments(p, false), false};
     const int64_t sequences = gdr_sequences(p), walks = (segs.per > 0 ? gdr_segment_slots(p, segs.per) : sequences > 0 ? sequences : 1) * p.heads_v;
     if (walks >= (1ll << 30)) return CC1D_ERR_TOO_LARGE;
+    segs.ranked = gdr_rank_walks(p, segs.per, walks);
     int rc = launch_gdr_prep(p, false, images, stream);
     if (rc != CC1D_OK) return rc;
     CC1D_DISPATCH_ITYPE(p.itype, {

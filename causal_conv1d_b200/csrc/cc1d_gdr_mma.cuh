@@ -360,7 +360,7 @@ struct GdrSegment {
     float M[kGdrMaxDim][kGdrMaxDim], Mt[kGdrMaxDim][kGdrMaxDim], B[kGdrMaxDim][kGdrMaxDim], back[kGdrMaxDim][kGdrMaxDim];
     float start[kGdrMaxDim][kGdrMaxDim], end[kGdrMaxDim][kGdrMaxDim];     // the state it starts from; the gradient of the one it ends with
 };
-struct GdrSegments { GdrSegment *at; int per; };
+struct GdrSegments { GdrSegment *at; int per; bool ranked; };     // ranked: walks take the longest sequence first
 
 // Segments of sequence n take slots gdr_first_segment(n) .., at least one each (as with the chunks' slots).
 __host__ __device__ inline int64_t gdr_segment_slots(const cc1d_gdr_params &p, int per) { return gdr_slots(p) / per + gdr_sequences(p); }
@@ -375,6 +375,31 @@ struct GdrPart {
     bool first, last;         // of the sequence
 };
 __device__ __forceinline__ int gdr_chunks(const GdrSeq &seq) { return (seq.end - seq.begin + kChunk - 1) / kChunk; }
+
+// Sequences by falling length (the whole CTA; `scratch`: kGdrRanked + 1 ints of its shared memory, free again on
+// return): of walks that do not all fit the SMs at once the long ones should not start last.
+constexpr int kGdrRanked = 64;
+__device__ __forceinline__ int gdr_ranked(const cc1d_gdr_params &p, int rank, int *scratch) {
+    const int n = (int)p.nseq, i = threadIdx.x;
+    int mine = 0;
+    if (i < n) {
+        const GdrSeq seq = gdr_sequence(p, i);
+        scratch[i] = mine = seq.end - seq.begin;
+    }
+    __syncthreads();
+    if (i < n) {
+        int before = 0;
+        for (int j = 0; j < n; ++j) before += scratch[j] > mine || (scratch[j] == mine && j < i);
+        if (before == rank) scratch[kGdrRanked] = i;
+    }
+    __syncthreads();
+    const int at = scratch[kGdrRanked];
+    __syncthreads();
+    return at;
+}
+inline bool gdr_rank_walks(const cc1d_gdr_params &p, int per, int64_t ctas) {
+    return per == 0 && p.cu_seqlens != nullptr && p.nseq > 1 && p.nseq <= kGdrRanked && ctas > num_sms();
+}
 
 // False: nothing to walk (the whole CTA leaves)
 __device__ __forceinline__ bool gdr_find_part(const cc1d_gdr_params &p, const GdrSegments &segs, int64_t slot, GdrPart &w) {

@@ -53,7 +53,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
     pdl_wait();
     const int heads = (int)p.heads_v, h = (int)(block % heads), sequences = (int)gdr_sequences(p);
     GdrPart w;
-    if (!gdr_find_part(p, segs, block / heads, w)) return;
+    if (!gdr_find_part(p, segs, segs.ranked ? gdr_ranked(p, (int)(block / heads), reinterpret_cast<int *>(smem)) : block / heads, w)) return;
     // B of a last segment leads nowhere, nor does M of one that is alone (or, forwards, of a last one)
     if (kMode == kSummary && (unit ? (kBack ? w.first && w.last : w.last) : w.last)) return;
     const GdrSeq seq = w.seq;
