@@ -9,16 +9,24 @@ namespace cc1d {
 
 constexpr int kGdrMaxDim = 128;
 
-// exp(x) to about 2^-22: ex2.approx with the rounding of x * log2(e) put back as a first-order
-// term (the plain form would lose |x| * 2^-24).  Arguments below -200 (and -inf) give 0.
+// exp(x) to about one unit in the last place: x = n ln 2 + r with ln 2 = 2839 / 4096 + a rest (n times the first
+// part is exact), the Taylor series of exp(r) to r^7 / 7! (|r| <= 0.35: what is left out is 5e-9), and 2^n in two
+// factors so that it may leave the range.  ex2.approx's 2^-22 shows in the states: the decays of all chunks
+// multiply.  Below -176 (and at -inf) the result is 0, a NaN stays one.
 __device__ __forceinline__ float gdr_exp(float x) {
-    constexpr float kLog2e = 1.44269504088896341f, kLog2eLow = 1.92596299112661e-8f, kLn2 = 0.693147180559945309f;
-    x = x < -200.f ? -200.f : x;
-    const float hi = x * kLog2e;
-    const float lo = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -hi));
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
-    return fmaf(e, lo * kLn2, e);
+    x = x < -176.f ? -176.f : x > 176.f ? 176.f : x;
+    const float n = rintf(x * 1.44269504f);
+    const float r = fmaf(n, -3.194618494547e-05f, fmaf(n, -2839.f / 4096.f, x));
+    float p = 1.f / 5040.f;
+    p = fmaf(p, r, 1.f / 720.f);
+    p = fmaf(p, r, 1.f / 120.f);
+    p = fmaf(p, r, 1.f / 24.f);
+    p = fmaf(p, r, 1.f / 6.f);
+    p = fmaf(p, r, 0.5f);
+    p = fmaf(p, r, 1.f);
+    p = fmaf(p, r, 1.f);
+    const int i = (int)n, half = i >> 1;
+    return p * __uint_as_float((uint32_t)(half + 127) << 23) * __uint_as_float((uint32_t)(i - half + 127) << 23);
 }
 
 // A gate as it lies in memory, and its value: a conversion beside the load would wait for it
