@@ -445,27 +445,31 @@ struct GdrDims {
     int64_t batch, seqlen, heads_k, heads_v, dim_k, dim_v;
 };
 
-// q, k (batch, seqlen, heads_k, dim_k), v (batch, seqlen, heads_v, dim_v), g, beta (batch, seqlen, heads_v)
+// q, k (batch, seqlen, heads_k, dim_k), v (batch, seqlen, heads_v, dim_v), g, beta (batch, seqlen, heads_v); with
+// one token a row also without the seqlen dimension
 GdrDims gdr_inputs(cc1d_gdr_params &p, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
-                   const at::Tensor &beta, double scale) {
+                   const at::Tensor &beta, double scale, bool may_lack_seqlen = false) {
     need_cuda(q, "q"); need_cuda(k, "k"); need_cuda(v, "v"); need_cuda(g, "g"); need_cuda(beta, "beta");
-    TORCH_CHECK(q.dim() == 4 && v.dim() == 4, "expected q, k (batch, seqlen, heads_k, dim_k) and v (batch, seqlen, heads_v, dim_v)");
-    const GdrDims d{q.size(0), q.size(1), q.size(2), v.size(2), q.size(3), v.size(3)};
-    need_shape(k, {d.batch, d.seqlen, d.heads_k, d.dim_k}, "k");
-    need_shape(v, {d.batch, d.seqlen, d.heads_v, d.dim_v}, "v");
-    need_shape(g, {d.batch, d.seqlen, d.heads_v}, "g");
-    need_shape(beta, {d.batch, d.seqlen, d.heads_v}, "beta");
+    const bool one = may_lack_seqlen && q.dim() == 3;
+    TORCH_CHECK((q.dim() == 4 || one) && v.dim() == q.dim(), "expected q, k (batch, seqlen, heads_k, dim_k) and v (batch, seqlen, heads_v, dim_v)");
+    const int h = one ? 1 : 2;                // the dimension of the heads
+    const GdrDims d{q.size(0), one ? 1 : q.size(1), q.size(h), v.size(h), q.size(h + 1), v.size(h + 1)};
+    TORCH_CHECK(k.sizes() == q.sizes(), "k must have the shape of q, ", q.sizes(), ", got ", k.sizes());
+    TORCH_CHECK(v.size(0) == d.batch && (one || v.size(1) == d.seqlen), "v must have the batch and seqlen of q, got shape ", v.sizes());
+    for (const at::Tensor *t : {&g, &beta})
+        TORCH_CHECK(t->dim() == h + 1 && t->sizes() == v.sizes().slice(0, h + 1), "g and beta must have the shape of v without its last dimension, got ", t->sizes());
     TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
     for (const at::Tensor *t : {&k, &v, &g, &beta}) TORCH_CHECK(t->device() == q.device(), "q, k, v, g and beta must be on one device");
-    TORCH_CHECK(q.stride(3) == 1 && k.stride(3) == 1 && v.stride(3) == 1, "q, k and v must be contiguous along their last dimension");
+    TORCH_CHECK(q.stride(h + 1) == 1 && k.stride(h + 1) == 1 && v.stride(h + 1) == 1, "q, k and v must be contiguous along their last dimension");
     p.itype = dtype_code(q, "q"); p.gtype = dtype_code(g, "g"); p.btype = dtype_code(beta, "beta");
     p.scale = (float)scale;
     p.batch = d.batch; p.seqlen = d.seqlen; p.heads_k = d.heads_k; p.heads_v = d.heads_v; p.dim_k = d.dim_k; p.dim_v = d.dim_v;
-    p.q = q.data_ptr(); p.q_batch_stride = q.stride(0); p.q_l_stride = q.stride(1); p.q_h_stride = q.stride(2);
-    p.k = k.data_ptr(); p.k_batch_stride = k.stride(0); p.k_l_stride = k.stride(1); p.k_h_stride = k.stride(2);
-    p.v = v.data_ptr(); p.v_batch_stride = v.stride(0); p.v_l_stride = v.stride(1); p.v_h_stride = v.stride(2);
-    p.g = g.data_ptr(); p.g_batch_stride = g.stride(0); p.g_l_stride = g.stride(1); p.g_h_stride = g.stride(2);
-    p.beta = beta.data_ptr(); p.beta_batch_stride = beta.stride(0); p.beta_l_stride = beta.stride(1); p.beta_h_stride = beta.stride(2);
+    const auto step = [&](const at::Tensor &t) { return one ? 0 : t.stride(1); };
+    p.q = q.data_ptr(); p.q_batch_stride = q.stride(0); p.q_l_stride = step(q); p.q_h_stride = q.stride(h);
+    p.k = k.data_ptr(); p.k_batch_stride = k.stride(0); p.k_l_stride = step(k); p.k_h_stride = k.stride(h);
+    p.v = v.data_ptr(); p.v_batch_stride = v.stride(0); p.v_l_stride = step(v); p.v_h_stride = v.stride(h);
+    p.g = g.data_ptr(); p.g_batch_stride = g.stride(0); p.g_l_stride = step(g); p.g_h_stride = g.stride(h);
+    p.beta = beta.data_ptr(); p.beta_batch_stride = beta.stride(0); p.beta_l_stride = step(beta); p.beta_h_stride = beta.stride(h);
     return d;
 }
 
@@ -501,18 +505,20 @@ void gdr_indices(cc1d_gdr_params &p, const OptTensor &state_indices_, int64_t n,
 
 }  // namespace
 
-void gated_delta_rule_update(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
-                             const at::Tensor &beta, at::Tensor &state, const OptTensor &state_indices_, at::Tensor &out,
-                             double scale) {
+at::Tensor gated_delta_rule_update(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &g,
+                                   const at::Tensor &beta, at::Tensor &state, const OptTensor &state_indices_, double scale) {
     cc1d_gdr_params p = {};
-    const GdrDims d = gdr_inputs(p, q, k, v, g, beta, scale);
-    gdr_out(p, d, q, out);
+    const GdrDims d = gdr_inputs(p, q, k, v, g, beta, scale, true);
     gdr_state(state, d, q, "state");
     gdr_indices(p, state_indices_, d.batch, state.size(0), q);
     p.final_states = state.data_ptr<float>();
     p.final_states_batch_stride = state.stride(0); p.final_states_h_stride = state.stride(1);
     c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor out = at::empty(v.sizes(), v.options());
+    p.out = out.data_ptr();
+    p.out_h_stride = d.dim_v; p.out_l_stride = d.heads_v * d.dim_v; p.out_batch_stride = d.seqlen * p.out_l_stride;
     raise_on(cc1d_gdr_update(&p, at::cuda::getCurrentCUDAStream().stream()), "gated_delta_rule_update");
+    return out;
 }
 
 namespace {

@@ -121,13 +121,8 @@ def gated_delta_rule_update(
 
     out: (batch, heads_v, dim_v) or (batch, seqlen, heads_v, dim_v)
     """
-    squeeze = q.dim() == 3
-    if squeeze:
-        q, k, v, g, beta = (t.unsqueeze(1) for t in (q, k, v, g, beta))
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    _ext.gated_delta_rule_update(q, k, v, g, beta, state, state_indices, out,
-                                 q.shape[-1] ** -0.5 if scale is None else scale)
-    return out.squeeze(1) if squeeze else out
+    return _ext.gated_delta_rule_update(q, k, v, g, beta, state, state_indices,
+                                        q.shape[-1] ** -0.5 if scale is None else scale)
 
 
 def gated_delta_rule_varlen_fn(
