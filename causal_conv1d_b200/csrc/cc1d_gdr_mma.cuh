@@ -103,6 +103,17 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 }
 template <int kThreads> __device__ __forceinline__ void walk_sync() { asm volatile("bar.sync 1, %0;" :: "n"(kThreads) : "memory"); }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234e38f; }
+__device__ __forceinline__ bool all_finite(const float (&x)[16]) {
+    float2 m[2] = {};                          // 0 * x is 0 or NaN
+    #pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+        m[0] = fma2(make_float2(x[j], x[j + 1]), splat2(0.f), m[0]);
+        m[1] = fma2(make_float2(x[j + 2], x[j + 3]), splat2(0.f), m[1]);
+    }
+    return finite((m[0].x + m[0].y) + (m[1].x + m[1].y));
+}
+
 // ---- fp32 as a sum of bf16 pieces ---------------------------------------------------------------
 // x = x1 + x2 + x3 with x1 = bf16(x), x2 = bf16(x - x1), x3 = bf16(x - x1 - x2): 8 + 8 + 8
 // significant bits, so three pieces hold an fp32 and two leave 2^-17 of it.  The differences are
@@ -210,6 +221,7 @@ struct GdrGates {
     float from_start[kChunk], to_end[kChunk], beta[kChunk], minus_beta_from_start[kChunk];
     float row[kChunk], same[kChunk], column[3][48];
     int steep;
+    int bad;                          // first token whose row of T is not finite (64: none); such rows are left out
 };
 __device__ __forceinline__ float gdr_fade(float2 gi, float2 gj) { return gdr_exp((gi.x - gj.x) + (gi.y - gj.y)); }
 

@@ -50,7 +50,7 @@ __device__ __forceinline__ GateSums scan_gates(const GateRegs &r, const cc1d_gdr
 __device__ __forceinline__ void store_gates(GdrGates &s, const GateSums &r, int lane) {
     *reinterpret_cast<float4 *>(&s.g[2 * lane]) = r.G;
     *reinterpret_cast<float2 *>(&s.beta[2 * lane]) = r.beta;
-    if (lane == 0) s.steep = 0;
+    if (lane == 0) { s.steep = 0; s.bad = kChunk; }
 }
 // 128 threads, after store_gates: the exponentials
 __device__ __forceinline__ void expand_gates(GdrGates &s, int tid) {
@@ -320,6 +320,12 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
                 }
             }
             if (warp < 2) {
+                // an infinite or NaN entry would reach the rows before it through products with zeros; the walk
+                // finds the token itself (its R is not finite) and gives NaN to it and those behind
+                if (!all_finite(x)) {
+                    #pragma unroll
+                    for (int j = 0; j < 16; ++j) x[j] = finite(x[j]) ? x[j] : 0.f;
+                }
                 #pragma unroll
                 for (int j = 0; j < 16; j += 4)
                     *reinterpret_cast<float4 *>(inv + i * kLd + j0 + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
@@ -349,6 +355,11 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
         const int i = (tid >> 2) + 32 * half, j0 = (tid & 3) * 16;
         #pragma unroll
         for (int j = 0; j < 16; ++j) if (j0 + j == i) x[half][j] = 0.f;      // T - I
+        if (!all_finite(x[half])) {
+            atomicMin(&gates.bad, i);
+            #pragma unroll
+            for (int j = 0; j < 16; ++j) x[half][j] = finite(x[half][j]) ? x[half][j] : 0.f;
+        }
         #pragma unroll
         for (int j = 0; j < 16; j += 8) store_pieces8<S::kSolve>(x[half] + j, base + tile_at(i, (j0 + j) / 8, 0));
     }
@@ -393,6 +404,9 @@ __global__ void __launch_bounds__(256) gdr_join_kernel(const __grid_constant__ c
                 src = p.initial_states + r * p.initial_states_batch_stride + h * p.initial_states_h_stride;
         }
         for (int c = 0; c < kJoinColumns; ++c) flat[c] = src != nullptr && row < dk && col0 + c < dv ? src[(int64_t)row * dv + col0 + c] : 0.f;
+        if (!to_back) {
+            for (int c = 0; c < kJoinColumns; ++c) at->start[row][col0 + c] = flat[c];
+        }
     }
     __syncthreads();
     for (int i = 0; i + 1 < count; ++i) {

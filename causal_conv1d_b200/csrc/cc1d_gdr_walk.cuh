@@ -22,7 +22,8 @@ enum GdrMode { kOutput, kKeep, kSummary };
 template <typename T, bool kBack> struct Fwd {
     using S = GdrStage<T, kBack>;
     static constexpr int kStages = S::kPieces == 1 ? 2 : 1;
-    static constexpr uint32_t kBars = kStages * S::kBytes, kBytes = kBars + 128 + sizeof(GdrPart) + 1024;
+    static constexpr uint32_t kBars = kStages * S::kBytes, kPart = kBars + 128, kBad = kPart + 128, kBytes = kBad + 2 * kGdrMaxDim * 4 + 1024;
+    static_assert(sizeof(GdrPart) <= 128, "");
 };
 
 // One CTA walks one sequence of one value head, chunk by chunk, with S^T (dim_v x dim_k) in the
@@ -33,6 +34,9 @@ template <typename T, bool kBack> struct Fwd {
 // rows) in tensor memory and the right one (K, Q, T, P) in shared memory, so nothing that the walk
 // computes passes through shared memory.  S itself is kept and decayed in fp32 registers; only
 // its pieces are rewritten every chunk.
+// A token whose R is infinite or NaN in some column takes part as zero there (as do rows of T: GdrGates::bad), for a zero of T or P times NaN
+// would reach the tokens before it; `bad` holds the first such token of each column, and from it on the
+// outputs of the chunk and the state behind it are NaN in that column.
 // kKeep: the backward's walk, which leaves S and U of every chunk in its record instead of an output.
 // kSummary: what a segment does to the state: from zeros its last state B, or (unit) without values from the
 // identity, dim_k columns instead of dim_v, its M.
@@ -59,7 +63,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
     const GdrSeq seq = w.seq;
     const int n = w.n, chunks = w.chunks, dk = (int)p.dim_k, dv = kMode == kSummary && unit ? dk : (int)p.dim_v;
     // what the walkers need again at their end (kept in registers over the walk it makes them spill)
-    volatile GdrPart *kept = reinterpret_cast<volatile GdrPart *>(smem + L::kBars + 128);
+    volatile GdrPart *kept = reinterpret_cast<volatile GdrPart *>(smem + L::kPart);
     if (tid == 0) {
         kept->n = w.n; kept->seq.end = w.seq.end; kept->segment = w.segment; kept->last = w.last;
         for (int s = 0; s < 2; ++s) { mbar_init(bar_full + 8 * s, kFeeders + 1); mbar_init(bar_empty + 8 * s, 1); }
@@ -203,7 +207,8 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
         if (kMode == kSummary) {
             #pragma unroll
             for (int j = 0; j < 32; ++j) S[j] = unit && 32 * part + j == col ? 1.f : 0.f;
-        } else if (!w.first) {
+        } else if (!(w.first && w.last)) {
+            // (a first segment's too: its sequence's last one may already have written the state's row)
             #pragma unroll
             for (int j = 0; j < 32; ++j) S[j] = w.segment[h].start[32 * part + j][col];
         } else {
@@ -213,6 +218,19 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             #pragma unroll
             for (int j = 0; j < 32; ++j) S[j] = from && 32 * part + j < dk && col < dv ? src[(int64_t)j * dv] : 0.f;
         }
+        // first token of a chunk whose value is not finite, by column; chunks use the two rows in turn
+        int *bad = reinterpret_cast<int *>(smem + L::kBad) + col;
+        if (kOut && part < 2) bad[part * kGdrMaxDim] = kChunk;
+        if (kOut) walk_sync<kWalkers>();
+        auto only_finite = [&](float (&x)[16], int first, int par) {
+            if (!all_finite(x)) {
+                #pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (!finite(x[j])) { atomicMin(bad + par * kGdrMaxDim, first + j); x[j] = 0.f; }
+                }
+            }
+            __syncwarp();
+        };
         // this warp's part of an operand is in tensor memory
         auto ready = [&](uint32_t bar) {
             tmem_wait_st();
@@ -258,11 +276,11 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     const float4 f = *reinterpret_cast<const float4 *>(gates.minus_beta_from_start + first + j);
                     const float2 u = fma2(make_float2(f.x, f.y), make_float2(x[j], x[j + 1]), make_float2(R[j], R[j + 1]));
                     const float2 v = fma2(make_float2(f.z, f.w), make_float2(x[j + 2], x[j + 3]), make_float2(R[j + 2], R[j + 3]));
-                    x[j] = R[j] = u.x; x[j + 1] = R[j + 1] = u.y;
-                    x[j + 2] = R[j + 2] = v.x; x[j + 3] = R[j + 3] = v.y;
+                    R[j] = u.x; R[j + 1] = u.y; R[j + 2] = v.x; R[j + 3] = v.y;
                 }
+                if (kOut) only_finite(R, first, par);
                 #pragma unroll
-                for (int j = 0; j < 16; j += 8) split8_to_tmem<PT>(x + j, mine + kFwdColR + first / 2 + j / 2, 32, 64);
+                for (int j = 0; j < 16; j += 8) split8_to_tmem<PT>(R + j, mine + kFwdColR + first / 2 + j / 2, 32, 64);
             }
             ready(bar_r);
             gdr_wait(bar_u, par, dead);
@@ -295,6 +313,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             }
             ready(bar_w);
             const float whole = gates.from_start[kChunk - 1];
+            const int bad_row = kOut ? gates.bad : kChunk;
             gdr_wait(bar_d, par, dead);
             __syncwarp();
             fence_after_sync();
@@ -309,9 +328,16 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     S[16 * b + j] = v.x; S[16 * b + j + 1] = v.y;
                 }
             }
+            if (kOut && part == 0) bad[(par ^ 1) * kGdrMaxDim] = kChunk;      // (all are done with the chunk before)
             fence_before_sync();
             walk_sync<kWalkers>();                      // every thread has read its part of Delta
             fence_after_sync();
+            const int bad_from = kOut ? min(bad[par * kGdrMaxDim], bad_row) : kChunk;
+            if (kOut && bad_from < kChunk) {
+                #pragma unroll
+                for (int j = 0; j < 32; ++j) S[j] = __uint_as_float(0x7fc00000u);
+            }
+            __syncwarp();
             if (c + 1 < chunks) put_state();
             // the output, while the next chunk's first product runs
             if (kOut) {
@@ -331,7 +357,8 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                         x[j + 2] = fmaf(f.z, x[j + 2], y[j + 2]); x[j + 3] = fmaf(f.w, x[j + 3], y[j + 3]);
                     }
                     #pragma unroll
-                    for (int j = 0; j < 8; ++j) V[(b + j) * kGdrMaxDim] = Elem<T>::from_f(p.scale * x[j]);   // where this thread read its v
+                    for (int j = 0; j < 8; ++j)      // where this thread read its v
+                        V[(b + j) * kGdrMaxDim] = Elem<T>::from_f(first + b + j < bad_from ? p.scale * x[j] : __uint_as_float(0x7fc00000u));
                 }
             }
             fence_before_sync();

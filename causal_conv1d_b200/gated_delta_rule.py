@@ -34,11 +34,11 @@ class GatedDeltaRuleFn(torch.autograd.Function):
             cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
         scale = q.shape[-1] ** -0.5 if scale is None else scale
         out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        n = q.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
         final_state = None
         if return_final_state:
-            n = q.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
             final_state = torch.empty(n, v.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=v.device)
-        if initial_state is not None and final_state is not None and initial_state.shape[0] != final_state.shape[0]:
+        if initial_state is not None and initial_state.shape[0] != n:
             raise RuntimeError("initial_state must have one row per sequence")
         _ext.gated_delta_rule_fwd(q, k, v, g, beta, cu_seqlens, initial_state, final_state, None, None, out, scale)
         ctx.save_for_backward(q, k, v, g, beta, initial_state, cu_seqlens)

@@ -187,3 +187,29 @@ def test_long_sequences_of_few_heads(dtype, slow):
 
 def test_one_long_row():
     check([2500], 1, 1, 128, 128, torch.bfloat16, False, slow=True, seed=2)
+
+
+def test_gradients_around_forgotten_states():
+    """g = -inf and steep decays inside a chunk: finite gradients, those of the tokens behind as without the past."""
+    import causal_conv1d_b200 as cc
+    leaves = gdr_ref.inputs((1, 140), 1, 1, 64, 64, torch.float32, seed=5)
+    leaves[3][0, 30], leaves[3][0, 100], leaves[3][0, 70:80] = -1000.0, -70.0, -20.0
+    leaves = [t.requires_grad_() for t in leaves]
+    dout = torch.randn(1, 140, 1, 64, device="cuda")
+    got = torch.autograd.grad(cc.gated_delta_rule_fn(*leaves), leaves, dout)
+    S0 = torch.zeros(1, 1, 64, 64)
+    _, _, want = expect(*leaves, [140], S0, dout, S0, 64 ** -0.5)
+    for name, a, b in zip(NAMES, got, want):
+        gdr_ref.close(a.flatten(0, 1), b, TOL, name)
+
+
+def test_empty_batches_and_rows():
+    import causal_conv1d_b200 as cc
+    for B, T in ((0, 5), (2, 0)):
+        leaves = [t.requires_grad_() for t in gdr_ref.inputs((B, T), 1, 2, 32, 32, torch.bfloat16)]
+        S0 = torch.randn(B, 2, 32, 32, device="cuda").requires_grad_()
+        out, last = cc.gated_delta_rule_fn(*leaves, initial_state=S0, return_final_state=True)
+        assert out.shape == (B, T, 2, 32) and torch.equal(last, S0)
+        d = torch.randn_like(last)
+        got = torch.autograd.grad(last, leaves + [S0], d, allow_unused=True)
+        assert torch.equal(got[5], d)
