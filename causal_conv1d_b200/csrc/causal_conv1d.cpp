@@ -4,6 +4,7 @@
 // parameter blocks of include/cc1d.h and calls libcc1d.so on the current stream of the
 // tensors' device.  No kernels live here and there is no CPU path: a non-CUDA tensor is an
 // error.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -489,6 +490,10 @@ void gdr_state(const at::Tensor &t, const GdrDims &d, const at::Tensor &q, const
                 " must be (rows, heads_v, dim_k, dim_v)");
     TORCH_CHECK(t.stride(3) == 1 && t.stride(2) == d.dim_v, what, " must be contiguous along its last two dimensions");
 }
+// a state that is written: two rows or heads in one place would overwrite each other
+void no_overlap(const at::Tensor &t, const char *what) {
+    TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, what, " is written in place and must not be an expanded tensor");
+}
 
 void gdr_indices(cc1d_gdr_params &p, const OptTensor &state_indices_, int64_t n, int64_t rows, const at::Tensor &q) {
     p.state_rows = rows;
@@ -510,6 +515,7 @@ at::Tensor gated_delta_rule_update(const at::Tensor &q, const at::Tensor &k, con
     cc1d_gdr_params p = {};
     const GdrDims d = gdr_inputs(p, q, k, v, g, beta, scale, true);
     gdr_state(state, d, q, "state");
+    no_overlap(state, "state");
     gdr_indices(p, state_indices_, d.batch, state.size(0), q);
     p.final_states = state.data_ptr<float>();
     p.final_states_batch_stride = state.stride(0); p.final_states_h_stride = state.stride(1);
@@ -557,6 +563,7 @@ static void gdr_states(cc1d_gdr_params &p, const GdrDims &d, const at::Tensor &q
     if (final_states_.has_value()) {
         const at::Tensor &t = *final_states_;
         gdr_state(t, d, q, "final_states");
+        no_overlap(t, "final_states");
         TORCH_CHECK(rows < 0 || t.size(0) == rows, "initial_states and final_states differ in their number of rows");
         rows = t.size(0);
         p.final_states = t.data_ptr<float>();

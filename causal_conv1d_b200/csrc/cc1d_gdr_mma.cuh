@@ -247,7 +247,8 @@ template <typename T, bool kBack> struct GdrStage {
     static constexpr uint32_t kKq = 0, kV = kPieces * kKqPiece, kT = kV + kChunk * kGdrMaxDim * sizeof(T), kGates = kT + kSolve * 8192,
                               kP = kGates + 4096, kBytes = kP + kOut * 8192, kImage = kBytes - kT;
 };
-static_assert(sizeof(GdrGates) <= 3072, "gates of a chunk (4096 bytes of an image, for the alignment of P)");
+constexpr uint32_t kGateBytes = 3 * 1024;        // of the 4096 in an image, which align P
+static_assert(sizeof(GdrGates) <= kGateBytes, "gates of a chunk");
 
 // Chunks of sequence n in the workspace: slots gdr_first_slot(n) .. ; the slots of different sequences
 // never meet (a sequence of L tokens takes ceil(L / 64) of the at least floor(L / 64) + 1 there are).

@@ -76,8 +76,9 @@ __device__ __forceinline__ void expand_gates(GdrGates &s, int tid) {
 // ---- (I + A)^-1 of a unit lower triangular 64 x 64 matrix ------------------------------------
 // Block elimination: four 16 x 16 diagonal blocks column by column in fp32, then 16 -> 32 -> 64 with
 //   T21 = -(T22 A21) T11
-// on the TF32 tensor cores, every factor as two TF32 values (11 + 11 bits; three products).  The contraction index is taken in the order 0, 2, 4, 6, 1, 3, 5, 7 within a
-// step of 8: a product in accumulator layout is then the left factor of the next one as it is.
+// on the TF32 tensor cores, every factor as two TF32 values (11 + 11 bits; three products).  The
+// contraction index is taken in the order 0, 2, 4, 6, 1, 3, 5, 7 within a step of 8: a product in
+// accumulator layout is then the left factor of the next one as it is.
 // In place: a holds the strictly lower part and receives the lower part of the inverse, diagonal
 // included, with zeros above it inside the 16 x 16 diagonal blocks; the upper right 32 x 32 block is
 // scratch.  Rows are kLd floats.  128 threads; ends with a barrier.
@@ -211,7 +212,7 @@ template <typename T, bool kBack> struct Prep {
     using S = GdrStage<T, kBack>;
     // what is computed takes the place of K and Q once their product is there: A and its inverse that of T, P its own;
     // the gates lie beside them till the end
-    static constexpr uint32_t kTiles = S::kPieces * S::kKqPiece, kGates = kTiles > S::kImage ? kTiles : S::kImage, kBars = kGates + 3072, kBytes = kBars + 64 + 1024;
+    static constexpr uint32_t kTiles = S::kPieces * S::kKqPiece, kGates = kTiles > S::kImage ? kTiles : S::kImage, kBars = kGates + kGateBytes, kBytes = kBars + 64 + 1024;
     static_assert(kChunk * kLd * 4 <= S::kP - S::kT, "A in the place of T and the image's gates");
 };
 
@@ -255,12 +256,12 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-            bool more;
     const uint32_t tmem = *slot_at;
     if (warp == 1) {
         if (elect_one()) {
             constexpr uint32_t id = mma_desc(128, 64, false, false);
             const uint64_t kq = smem_desc(base);
+            bool more = false;
             more = false;
             #pragma unroll
             for (int o = 2; o >= 0; --o) {
@@ -368,7 +369,7 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
     if (tid == 0) {
         unsigned char *image = images + (slot * heads + h) * (int64_t)S::kImage;
         bulk_store(image, base, S::kSolve * 8192);
-        bulk_store(image + S::kSolve * 8192, base + L::kGates, 3072);
+        bulk_store(image + S::kSolve * 8192, base + L::kGates, kGateBytes);
         bulk_store(image + (S::kP - S::kT), base + (S::kP - S::kT), S::kOut * 8192);
         bulk_commit();
         bulk_wait_read();

@@ -23,7 +23,7 @@ template <typename T, bool kBack> struct Fwd {
     using S = GdrStage<T, kBack>;
     static constexpr int kStages = S::kPieces == 1 ? 2 : 1;
     static constexpr uint32_t kBars = kStages * S::kBytes, kPart = kBars + 128, kBad = kPart + 128, kBytes = kBad + 2 * kGdrMaxDim * 4 + 1024;
-    static_assert(sizeof(GdrPart) <= 128, "");
+    static_assert(sizeof(GdrPart) <= 128, "place between the barriers and the first bad tokens");
 };
 
 // One CTA walks one sequence of one value head, chunk by chunk, with S^T (dim_v x dim_k) in the

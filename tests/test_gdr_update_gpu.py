@@ -139,3 +139,18 @@ def test_refusals():
         cc.gated_delta_rule_update(q[..., :60], k[..., :60], v, g, beta, state[:, :, :60].contiguous())
     with pytest.raises(RuntimeError, match="multiple of the number of key heads"):
         cc.gated_delta_rule_update(q, k, v[:, :, :3], g[..., :3], beta[..., :3], state[:, :3].contiguous())
+
+
+def test_refuses_a_state_whose_rows_are_one_place():
+    import causal_conv1d_b200 as cc
+    q, k, v, g, beta = gdr_ref.inputs((2, 1), 2, 4, 64, 64, torch.bfloat16)
+    shared = torch.zeros(1, 4, 64, 64, device="cuda").expand(2, 4, 64, 64)
+    with pytest.raises(RuntimeError, match="expanded"):
+        cc.gated_delta_rule_update(q, k, v, g, beta, shared)
+    packed, cu = [t[:, 0] for t in (q, k, v, g, beta)], torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="expanded"):
+        cc.gated_delta_rule_varlen_fn(*packed, cu_seqlens=cu, states=shared)
+    # read only, it is a state that all sequences share
+    one = cc.gated_delta_rule_varlen_fn(*packed, cu_seqlens=cu, states=shared, update_states=False)
+    own = cc.gated_delta_rule_varlen_fn(*packed, cu_seqlens=cu, states=shared.contiguous(), update_states=False)
+    assert torch.equal(one, own)
