@@ -105,6 +105,21 @@ bool make_channel_last_tensor_map(CUtensorMap *map, int dtype, const void *base,
     return rc == CUDA_SUCCESS;
 }
 
+// 8-bit codes, dense (batch, seqlen, dim); dim a multiple of 16
+bool make_codes_tensor_map(CUtensorMap *map, const uint8_t *base, int64_t dim, int64_t seqlen, int64_t batch, int box_channels) {
+    const TensorMapEncodeFn encode = tensor_map_encoder();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)seqlen, (cuuint64_t)(batch < 1 ? 1 : batch)};
+    const cuuint64_t strides[2] = {(cuuint64_t)dim, (cuuint64_t)dim * (cuuint64_t)seqlen};
+    const cuuint32_t box[3] = {(cuuint32_t)box_channels, (cuuint32_t)kTmaRows, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    if (dim % 16 || (reinterpret_cast<uintptr_t>(base) & 15) != 0) return false;
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(base), dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS;
+}
+
 bool make_channel_first_tensor_map(CUtensorMap *map, int dtype, const void *base, int64_t seqlen, int64_t dim,
                                    int64_t batch, int64_t c_stride, int64_t batch_stride, int box_tokens, int box_channels) {
     const TensorMapEncodeFn encode = tensor_map_encoder();
@@ -226,8 +241,8 @@ const char *cc1d_status_str(int status) {
 
 }  // extern "C"
 
-// cc1d_fwd; channel-first rows that fwd_keeps_codes() also leave x in `codes`
-int cc1d::cc1d_fwd_keeping(const cc1d_fwd_params *p, const cc1d_codes *codes, cc1d_stream_t stream) {
+// cc1d_fwd, which leaves x in `codes` too where its kernel can (*kept)
+int cc1d::cc1d_fwd_keeping(const cc1d_fwd_params *p, const cc1d_codes *codes, bool *kept, cc1d_stream_t stream) {
     if (p == nullptr) return CC1D_ERR_NULL;
     bool cl = false;
     int rc = check_conv_common(p->itype, p->wtype, p->width, p->batch, p->dim, p->seqlen, p->x,
@@ -247,12 +262,15 @@ int cc1d::cc1d_fwd_keeping(const cc1d_fwd_params *p, const cc1d_codes *codes, cc
     cc1d_fwd_params q = *p;
     if (q.batch <= 1) q.x_batch_stride = q.out_batch_stride = q.initial_states_batch_stride = q.final_states_batch_stride = 0;
     if (q.width == 2) q.initial_states_l_stride = q.final_states_l_stride = 0;
-    return cl ? launch_fwd_channel_last(q, s) : launch_fwd_channel_first(q, s, codes != nullptr && fwd_keeps_codes(q) ? codes : nullptr);
+    if (cl) return launch_fwd_channel_last(q, s, codes, kept);
+    if (codes == nullptr || !fwd_keeps_codes(q)) return launch_fwd_channel_first(q, s);
+    *kept = true;
+    return launch_fwd_channel_first(q, s, codes);
 }
 
 extern "C" {
 
-int cc1d_fwd(const cc1d_fwd_params *p, cc1d_stream_t stream) { return cc1d_fwd_keeping(p, nullptr, stream); }
+int cc1d_fwd(const cc1d_fwd_params *p, cc1d_stream_t stream) { return cc1d_fwd_keeping(p, nullptr, nullptr, stream); }
 
 static int check_bwd(const cc1d_bwd_params *p, bool *cl) {
     if (p == nullptr) return CC1D_ERR_NULL;
@@ -312,7 +330,7 @@ static int run_bwd(const cc1d_bwd_params *p, bool cl, cc1d_stream_t stream, cons
         q.initial_states_batch_stride = q.dfinal_states_batch_stride = q.dinitial_states_batch_stride = 0;
     }
     if (q.width == 2) q.initial_states_l_stride = q.dfinal_states_l_stride = q.dinitial_states_l_stride = 0;
-    return cl ? launch_bwd_channel_last(q, s) : launch_bwd_channel_first(q, s, codes);
+    return cl ? launch_bwd_channel_last(q, s, codes) : launch_bwd_channel_first(q, s, codes);
 }
 
 int cc1d_bwd(const cc1d_bwd_params *p, cc1d_stream_t stream) {
@@ -333,8 +351,11 @@ int cc1d::cc1d_bwd_check(const cc1d_bwd_params *p) {
 }
 
 int cc1d::cc1d_bwd_reading(const cc1d_bwd_params *p, const cc1d_codes *codes, cc1d_stream_t stream) {
-    const int rc = cc1d_bwd_check(p);
-    return rc != CC1D_OK ? rc : run_bwd(p, false, stream, codes);
+    bool cl = false;
+    const int rc = check_bwd(p, &cl);
+    if (rc != CC1D_OK) return rc;
+    if (p->workspace == nullptr || p->workspace_bytes < cc1d_bwd_workspace_bytes(p)) return CC1D_ERR_WORKSPACE;
+    return run_bwd(p, cl, stream, codes);
 }
 
 // Scratch of cc1d_bwd_noalloc: part of the library image, so no allocation is ever needed.

@@ -961,6 +961,8 @@ struct BwdClArgs {
     int wtype;
     int tpt;
     uint32_t ncols, ncolblk, ngroups;
+    const uint8_t *codes, *scales;   // x in 8 bits (kCodes), dense (batch, seqlen, dim) and its groups
+    uint32_t groups;                 // scales per token
 };
 
 #ifndef CC1D_BWD_CL_ROWS
@@ -1277,10 +1279,11 @@ __global__ void __launch_bounds__(32 * kBwdClRows, CC1D_BWD_CL_MINBLK) bwd_cl_ke
 #endif
 constexpr int kBwdTmaStages = CC1D_BWD_TMA_STAGES;
 
-template <typename T> struct BwdTma {
+template <typename T, bool kCodes = false> struct BwdTma {
     static constexpr int kRowBytes = 32 * kBwdClC * (int)sizeof(T);      // one token of a warp's strip
     static constexpr int kBoxBytes = kTmaRows * kRowBytes;
-    static constexpr int kStageBytes = 2 * kBoxBytes;                     // x box, then dout box
+    static constexpr int kXRowBytes = kCodes ? 32 * kBwdClC : kRowBytes, kXBytes = kTmaRows * kXRowBytes;
+    static constexpr int kStageBytes = kXBytes + kBoxBytes;               // x box, then dout box
     static constexpr size_t kSmem = (size_t)kBwdClRows * kBwdTmaStages * kStageBytes + (size_t)kBwdClRows * kBwdTmaStages * 8;
 };
 
@@ -1295,14 +1298,19 @@ template <> __device__ __forceinline__ uint2 lds_raw<uint2>(uint32_t addr) {
 // kDoutCf: dout is stored channel-first ((batch, dim, seqlen) with seqlen stride 1) although x and dx are
 // channel-last: its box arrives as [32 * C channels][kTmaRows tokens] (16 bytes per channel), a thread
 // reads the C rows of its channels once per stage and picks token r out of them with byte permutes.
-template <typename T, int W, bool kSilu, bool kSeqIdx, bool kDoutCf>
+// kCodes: x arrives as its 8-bit codes (4 bytes a lane and token); the scales of a stage, kTmaRows tokens of
+// 4 groups, are one byte a lane, asked for a stage ahead like the sequence ids.  (1,5376,8192) bf16 with seq_idx,
+// forward and backward: 150 us, 167 with x restored by a kernel of its own first.
+template <typename T, int W, bool kSilu, bool kSeqIdx, bool kDoutCf, bool kCodes>
 __global__ void __launch_bounds__(32 * kBwdClRows, CC1D_BWD_CL_MINBLK)
 bwd_cl_tma_kernel(const BwdClArgs a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap dmap) {
     pdl_wait();
     constexpr int C = kBwdClC;
     constexpr int kAcc = (W + 1) * C;
     constexpr bool kTanh = kSilu && UseTanhSilu<T>::value;
-    constexpr int kRowBytes = BwdTma<T>::kRowBytes, kBoxBytes = BwdTma<T>::kBoxBytes, kStageBytes = BwdTma<T>::kStageBytes;
+    using B = BwdTma<T, kCodes>;
+    constexpr int kRowBytes = B::kRowBytes, kXBytes = B::kXBytes, kStageBytes = B::kStageBytes;
+    static_assert(!kCodes || (sizeof(T) == 2 && !kDoutCf && C * 8 == kCodeGroup && kTmaRows * 4 == 32), "a lane has 4 codes, 8 lanes a group");
     using R = Raw<T, C>;
     __shared__ __align__(16) float s_red[(kBwdClRows - 1) * 32 * kAcc];
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -1344,8 +1352,8 @@ bwd_cl_tma_kernel(const BwdClArgs a, const __grid_constant__ CUtensorMap xmap, c
                 if (s < nst) {
                     mbar_expect_tx(bars + 8 * s, kStageBytes);
                     tma_load_3d(ring + s * kStageBytes, &xmap, c0, t0 + s * kTmaRows, (int)b, bars + 8 * s);
-                    if (kDoutCf) tma_load_3d(ring + s * kStageBytes + kBoxBytes, &dmap, t0 + s * kTmaRows, c0, (int)b, bars + 8 * s);
-                    else tma_load_3d(ring + s * kStageBytes + kBoxBytes, &dmap, c0, t0 + s * kTmaRows, (int)b, bars + 8 * s);
+                    if (kDoutCf) tma_load_3d(ring + s * kStageBytes + kXBytes, &dmap, t0 + s * kTmaRows, c0, (int)b, bars + 8 * s);
+                    else tma_load_3d(ring + s * kStageBytes + kXBytes, &dmap, c0, t0 + s * kTmaRows, (int)b, bars + 8 * s);
                 }
             }
         }
@@ -1368,7 +1376,15 @@ bwd_cl_tma_kernel(const BwdClArgs a, const __grid_constant__ CUtensorMap xmap, c
             zero_raw(r);
             swin[k] = -1;
             if (p >= 0) {
-                if (lane_ok) ld_cached_raw(r, xptr - (W - 1 - k) * xs);
+                if constexpr (kCodes) {
+                    if (lane_ok) {
+                        const uint64_t t = (uint64_t)b * (uint64_t)L + p;
+                        r = expand4<T>(*reinterpret_cast<const uint32_t *>(a.codes + t * (uint64_t)a.dim + (uint64_t)col * C),
+                                       scale_value(a.scales[t * a.groups + col / (kCodeGroup / C)]));
+                    }
+                } else if (lane_ok) {
+                    ld_cached_raw(r, xptr - (W - 1 - k) * xs);
+                }
                 if (kSeqIdx) swin[k] = sp[k - (W - 1)];
             } else if (a.init != nullptr && lane_ok) {
                 ld_cached_raw(r, reinterpret_cast<const T *>(a.init) + b * a.i_bs + (p + (W - 1)) * a.i_ls + (int64_t)col * C);
@@ -1397,24 +1413,42 @@ bwd_cl_tma_kernel(const BwdClArgs a, const __grid_constant__ CUtensorMap xmap, c
         // stage; -2 beyond the sequence (matches nothing)
         const int myrow = tx & (kTmaRows - 1);
         int next_id = (kSeqIdx && myrow < n_ld) ? sp[myrow] : -2;
+        // scales likewise: lane l holds that of row l / 4 and of the strip's group l % 4 (0 past the end: codes are 0 there)
+        const uint32_t my_group = cb * 4 + (tx & 3);
+        const uint8_t *scales = kCodes ? a.scales + ((uint64_t)b * (uint64_t)L + t0 + (tx >> 2)) * a.groups + my_group : nullptr;
+        const auto ask_scale = [&](int base) -> uint32_t {
+            return kCodes && my_group < a.groups && base + (tx >> 2) < n_ld ? scales[(int64_t)base * a.groups] : 0u;
+        };
+        uint32_t next_scale = ask_scale(0);
 
         for (int st = 0; st < nst; ++st) {
             const int s = st % kBwdTmaStages;
             const int base = st * kTmaRows;
             const int my_id = next_id;
             next_id = (kSeqIdx && base + kTmaRows + myrow < n_ld) ? sp[kTmaRows + myrow] : -2;
+            const uint32_t my_scale = next_scale;
+            if (kCodes) next_scale = ask_scale(base + kTmaRows);
             // the warp decides together (the votes and shuffles below need all 32 lanes)
             if (!__all_sync(kFullMask, mbar_wait(bars + 8 * s, (uint32_t)(st / kBwdTmaStages) & 1u))) {
                 g_tma_wait_expired = 1;     // never expected; stop consuming, still join the block reduction
                 break;
             }
-            const uint32_t xsrc = ring + s * kStageBytes + tx * (C * (int)sizeof(T));
-            const uint32_t dsrc = xsrc + kBoxBytes;
+            const uint32_t xsrc = ring + s * kStageBytes + tx * (kCodes ? C : C * (int)sizeof(T));
+            const uint32_t dsrc = ring + s * kStageBytes + kXBytes + tx * (C * (int)sizeof(T));
+            const auto x_row = [&](int r) -> R {
+                if constexpr (kCodes) {
+                    uint32_t c;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(c) : "r"(xsrc + r * B::kXRowBytes));
+                    return expand4<T>(c, scale_value(__shfl_sync(kFullMask, my_scale, 4 * r + (tx >> 3))));
+                } else {
+                    return lds_raw<R>(xsrc + r * kRowBytes);
+                }
+            };
             // channel-first dout: the thread's C channel rows of this stage, kTmaRows tokens each
             uint4 dch[C];
             if (kDoutCf) {
                 #pragma unroll
-                for (int j = 0; j < C; ++j) dch[j] = lds128(ring + s * kStageBytes + kBoxBytes + (tx * C + j) * 16);
+                for (int j = 0; j < C; ++j) dch[j] = lds128(ring + s * kStageBytes + kXBytes + (tx * C + j) * 16);
             }
             auto dout_row = [&](int r) -> R {
                 if constexpr (kDoutCf) {
@@ -1447,7 +1481,7 @@ bwd_cl_tma_kernel(const BwdClArgs a, const __grid_constant__ CUtensorMap xmap, c
             if (plain) {
                 #pragma unroll
                 for (int r = 0; r < kTmaRows; ++r) {
-                    const R xr = lds_raw<R>(xsrc + r * kRowBytes), dr = dout_row(r);
+                    const R xr = x_row(r), dr = dout_row(r);
                     bwd_cl_position_impl<T, W, C, kSilu, false, kTanh>(
                         xr, dr, 0, true, lane_ok, false, xwin, gwin, swin, wv, wy, bv, dw, nullptr, 0, optr + r * os, nullptr);
                 }
@@ -1457,7 +1491,7 @@ bwd_cl_tma_kernel(const BwdClArgs a, const __grid_constant__ CUtensorMap xmap, c
                 #pragma unroll 1
                 for (int r = 0; r < kTmaRows; ++r) {
                     const int sid = kSeqIdx ? __shfl_sync(kFullMask, my_id, r) : 0;
-                    const R xr = lds_raw<R>(xsrc + r * kRowBytes), dr = dout_row(r);
+                    const R xr = x_row(r), dr = dout_row(r);
                     bwd_cl_position_impl<T, W, C, kSilu, kSeqIdx, kTanh>(
                         xr, dr, sid, true, lane_ok, false, xwin, gwin, swin, wv, wy, bv, dw, nullptr, 0, optr + r * os, nullptr);
                 }
@@ -1467,7 +1501,7 @@ bwd_cl_tma_kernel(const BwdClArgs a, const __grid_constant__ CUtensorMap xmap, c
                     const int i = base + r;               // position t0 + i
                     const int sid = kSeqIdx ? __shfl_sync(kFullMask, my_id, r) : 0;
                     if (i < n_ext) {
-                        const R xr = lds_raw<R>(xsrc + r * kRowBytes), dr = dout_row(r);
+                        const R xr = x_row(r), dr = dout_row(r);
                         const int q = t0 + i - (W - 1);   // dx position produced now
                         const bool st_dx = i >= W - 1 && lane_ok;
                         const bool st_di = q < 0 && want_dinit;
@@ -1485,8 +1519,8 @@ bwd_cl_tma_kernel(const BwdClArgs a, const __grid_constant__ CUtensorMap xmap, c
                 fence_proxy_async_smem();
                 mbar_expect_tx(bars + 8 * s, kStageBytes);
                 tma_load_3d(ring + s * kStageBytes, &xmap, c0, t0 + (st + kBwdTmaStages) * kTmaRows, (int)b, bars + 8 * s);
-                if (kDoutCf) tma_load_3d(ring + s * kStageBytes + kBoxBytes, &dmap, t0 + (st + kBwdTmaStages) * kTmaRows, c0, (int)b, bars + 8 * s);
-                else tma_load_3d(ring + s * kStageBytes + kBoxBytes, &dmap, c0, t0 + (st + kBwdTmaStages) * kTmaRows, (int)b, bars + 8 * s);
+                if (kDoutCf) tma_load_3d(ring + s * kStageBytes + kXBytes, &dmap, t0 + (st + kBwdTmaStages) * kTmaRows, c0, (int)b, bars + 8 * s);
+                else tma_load_3d(ring + s * kStageBytes + kXBytes, &dmap, c0, t0 + (st + kBwdTmaStages) * kTmaRows, (int)b, bars + 8 * s);
             }
         }
     }
@@ -1556,7 +1590,15 @@ size_t bwd_workspace_bytes_channel_last(const cc1d_bwd_params &p) {
     return (size_t)((uint64_t)p.batch * pl.ngroups * (uint64_t)p.dim * (uint64_t)(p.width + 1) * sizeof(float));
 }
 
-int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream) {
+// 16-bit types and a dout in x's layout, where tensor maps can describe both
+bool bwd_cl_reads_codes(const cc1d_bwd_params &p) {
+    const int64_t most = 1ll << 39;       // a map's strides end at 2^40 bytes
+    return p.itype != CC1D_F32 && p.dim % 16 == 0 && p.dim < (1ll << 31) && p.seqlen < (1ll << 31) - 4096 && p.batch < (1ll << 31) &&
+           p.dim * p.seqlen < most && p.dout_c_stride == 1 && p.dout_l_stride > 0 && p.dout_l_stride % 8 == 0 && p.dout_l_stride < (1ll << 31) &&
+           p.dout_l_stride * p.seqlen < most && (p.batch <= 1 || (p.dout_batch_stride > 0 && p.dout_batch_stride % 8 == 0 && p.dout_batch_stride < most));
+}
+
+int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream, const cc1d_codes *codes) {
     const int C = kBwdClC;
     // token positions are 32-bit integers in the kernels (chunk starts plus a halo must not wrap)
     if (p.seqlen >= (1ll << 31) - 4096 || p.dim >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
@@ -1574,7 +1616,7 @@ int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream) {
     if (bwd_workspace_bytes_channel_last(p) > p.workspace_bytes) return CC1D_ERR_WORKSPACE;
     if (!is_aligned16(p.workspace)) return CC1D_ERR_ALIGN;
 
-    BwdClArgs a;
+    BwdClArgs a = {};
     a.x = p.x; a.dout = p.dout; a.dx = p.dx; a.weight = p.weight; a.bias = p.bias; a.seq_idx = p.seq_idx;
     a.init = p.initial_states; a.dfin = p.dfinal_states; a.dinit = p.dinitial_states;
     a.ws = reinterpret_cast<float *>(p.workspace);
@@ -1593,15 +1635,27 @@ int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream) {
         // fp32 stages are twice as large (2 CTAs per SM instead of 3): still 3 % ahead of the register-prefetch
         // kernel; a channel-first dout is read in place for 16-bit types only
         if ((p.itype != CC1D_F32 || !dout_cf) && p.seqlen < (1ll << 31) - 16 && p.batch < (1ll << 31) &&
-            make_channel_last_tensor_map(&xmap, p.itype, p.x, p.dim, p.seqlen, p.batch, p.x_l_stride, p.x_batch_stride, row_bytes) &&
+            (codes != nullptr ? make_codes_tensor_map(&xmap, codes->codes, p.dim, p.seqlen, p.batch, 32 * kBwdClC)
+                              : make_channel_last_tensor_map(&xmap, p.itype, p.x, p.dim, p.seqlen, p.batch, p.x_l_stride, p.x_batch_stride, row_bytes)) &&
             (dout_cf ? make_channel_first_tensor_map(&dmap, p.itype, p.dout, p.seqlen, p.dim, p.batch, p.dout_c_stride,
                                                      p.dout_batch_stride, kTmaRows, 32 * kBwdClC)
                      : make_channel_last_tensor_map(&dmap, p.itype, p.dout, p.dim, p.seqlen, p.batch, p.dout_l_stride,
                                                     p.dout_batch_stride, row_bytes))) {
-            if (p.itype == CC1D_F32) {
+            if (codes != nullptr) {
+                a.codes = codes->codes; a.scales = codes->scales;
+                a.groups = (uint32_t)((p.dim + kCodeGroup - 1) / kCodeGroup);
+                CC1D_DISPATCH_BOOL(p.itype == CC1D_BF16, kBf16, {
+                    using T = std::conditional_t<kBf16, __nv_bfloat16, __half>;
+                    CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(p.seq_idx != nullptr, kSeqIdx, {
+                        auto kernel = bwd_cl_tma_kernel<T, W, kSilu, kSeqIdx, false, true>;
+                        allow_dynamic_smem(reinterpret_cast<const void *>(kernel), BwdTma<T, true>::kSmem);
+                        launch_k(kernel, dim3((unsigned)ctas), dim3(32 * kBwdClRows), BwdTma<T, true>::kSmem, stream, a, xmap, dmap);
+                    });););
+                });
+            } else if (p.itype == CC1D_F32) {
                 using T = float;
                 CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(p.seq_idx != nullptr, kSeqIdx, {
-                        auto kernel = bwd_cl_tma_kernel<T, W, kSilu, kSeqIdx, false>;
+                        auto kernel = bwd_cl_tma_kernel<T, W, kSilu, kSeqIdx, false, false>;
                         allow_dynamic_smem(reinterpret_cast<const void *>(kernel), BwdTma<T>::kSmem);
                         launch_k(kernel, dim3((unsigned)ctas), dim3(32 * kBwdClRows), BwdTma<T>::kSmem, stream, a, xmap, dmap);
                     });););
@@ -1609,7 +1663,7 @@ int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream) {
                 using T = __nv_bfloat16;
                 CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(p.seq_idx != nullptr, kSeqIdx,
                     CC1D_DISPATCH_BOOL(dout_cf, kDoutCf, {
-                        auto kernel = bwd_cl_tma_kernel<T, W, kSilu, kSeqIdx, kDoutCf>;
+                        auto kernel = bwd_cl_tma_kernel<T, W, kSilu, kSeqIdx, kDoutCf, false>;
                         allow_dynamic_smem(reinterpret_cast<const void *>(kernel), BwdTma<T>::kSmem);
                         launch_k(kernel, dim3((unsigned)ctas), dim3(32 * kBwdClRows), BwdTma<T>::kSmem, stream, a, xmap, dmap);
                     }););););
@@ -1617,7 +1671,7 @@ int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream) {
                 using T = __half;
                 CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu, CC1D_DISPATCH_BOOL(p.seq_idx != nullptr, kSeqIdx,
                     CC1D_DISPATCH_BOOL(dout_cf, kDoutCf, {
-                        auto kernel = bwd_cl_tma_kernel<T, W, kSilu, kSeqIdx, kDoutCf>;
+                        auto kernel = bwd_cl_tma_kernel<T, W, kSilu, kSeqIdx, kDoutCf, false>;
                         allow_dynamic_smem(reinterpret_cast<const void *>(kernel), BwdTma<T>::kSmem);
                         launch_k(kernel, dim3((unsigned)ctas), dim3(32 * kBwdClRows), BwdTma<T>::kSmem, stream, a, xmap, dmap);
                     }););););
@@ -1625,8 +1679,8 @@ int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream) {
             launched = true;
         }
 #endif
-        // a channel-first dout is only served by the TMA kernel (16-bit types, a tensor map the driver accepts)
-        if (!launched && dout_cf) return CC1D_ERR_STRIDE;
+        // a channel-first dout and codes are only served by the TMA kernel (16-bit types, tensor maps the driver accepts)
+        if (!launched && (dout_cf || codes != nullptr)) return CC1D_ERR_STRIDE;
         if (!launched) {
             CC1D_DISPATCH_ITYPE(p.itype, CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu,
                 CC1D_DISPATCH_BOOL(p.seq_idx != nullptr, kSeqIdx, {

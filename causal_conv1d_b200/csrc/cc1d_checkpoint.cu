@@ -161,8 +161,9 @@ int cc1d_fwd_e4m3(const cc1d_fwd_params *p, const cc1d_codes *to, cc1d_stream_t 
     if (p == nullptr || to == nullptr) return CC1D_ERR_NULL;
     if (!is_aligned16(to->codes)) return CC1D_ERR_ALIGN;
     if (p->batch > 0 && p->dim > 0 && p->seqlen > 0 && (to->codes == nullptr || to->scales == nullptr)) return CC1D_ERR_NULL;
-    const int rc = cc1d_fwd_keeping(p, to, stream);
-    if (rc != CC1D_OK || (!channel_last(p->x_c_stride, p->x_l_stride) && fwd_keeps_codes(*p))) return rc;
+    bool kept = false;
+    const int rc = cc1d_fwd_keeping(p, to, &kept, stream);
+    if (rc != CC1D_OK || kept) return rc;
     return cc1d_checkpoint_e4m3(p, to, stream);
 }
 
@@ -176,9 +177,13 @@ static cc1d_bwd_params with_dense_x(const cc1d_bwd_params &p, const void *x) {
     return q;
 }
 
+static bool reads_codes(const cc1d_bwd_params &p) {
+    return channel_last(p.x_c_stride, p.x_l_stride) ? bwd_cl_reads_codes(p) : bwd_reads_codes(p);
+}
+
 size_t cc1d_bwd_e4m3_restore_bytes(const cc1d_bwd_params *p) {
     if (p == nullptr || p->batch < 0 || p->dim < 0 || p->seqlen < 0) return 0;
-    if (!channel_last(p->x_c_stride, p->x_l_stride) && bwd_reads_codes(*p)) return 0;
+    if (reads_codes(*p)) return 0;
     return (size_t)p->batch * (size_t)p->dim * (size_t)p->seqlen * (size_t)elem_size(p->itype);
 }
 
@@ -187,7 +192,7 @@ int cc1d_bwd_e4m3(const cc1d_bwd_params *p, const cc1d_codes *from, void *restor
     const bool some = p->batch > 0 && p->dim > 0 && p->seqlen > 0;
     if (some && (from->codes == nullptr || from->scales == nullptr)) return CC1D_ERR_NULL;
     if (!is_aligned16(from->codes)) return CC1D_ERR_ALIGN;
-    if (!channel_last(p->x_c_stride, p->x_l_stride) && bwd_reads_codes(*p)) {
+    if (reads_codes(*p)) {
         const cc1d_bwd_params q = with_dense_x(*p, from->codes);
         return cc1d_bwd_reading(&q, from, stream);
     }

@@ -28,6 +28,26 @@ __device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d)
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return (uint32_t)lo | ((uint32_t)hi << 16);
 }
+// 4 neighbouring values of each of 8 lanes, a group -> this lane's codes, and the group's scale.  The bits of
+// a float without their sign are ordered like the values, with infinities above all numbers and NaN above
+// those, so the largest magnitude is an integer's (of 16-bit types two at a time).
+template <typename T> __device__ __forceinline__ uint32_t codes_of_group(const uint2 &v, uint32_t &s) {
+    uint32_t m = __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu);
+    #pragma unroll
+    for (int i = 1; i < 8; i <<= 1) m = __vmaxu2(m, __shfl_xor_sync(kFullMask, m, i));
+    s = code_scale(unpack_pair<T>(max(m & 0xffffu, m >> 16)).x);
+    const float inv = scale_inverse(s);
+    const float2 a = unpack_pair<T>(v.x), b = unpack_pair<T>(v.y);
+    return to_codes(a.x * inv, a.y * inv, b.x * inv, b.y * inv);
+}
+template <typename T> __device__ __forceinline__ uint32_t codes_of_group(const uint4 &v, uint32_t &s) {
+    uint32_t m = max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+    #pragma unroll
+    for (int i = 1; i < 8; i <<= 1) m = max(m, __shfl_xor_sync(kFullMask, m, i));
+    s = code_scale(__uint_as_float(m));
+    const float inv = scale_inverse(s);
+    return to_codes(__uint_as_float(v.x) * inv, __uint_as_float(v.y) * inv, __uint_as_float(v.z) * inv, __uint_as_float(v.w) * inv);
+}
 // 2 codes (the low 16 bits) times their scale
 __device__ __forceinline__ float2 from_codes(uint32_t codes, float scale) {
     uint32_t h;

@@ -377,6 +377,8 @@ struct FwdClArgs {
     uint32_t ncols;     // 16-byte channel vectors per token
     uint32_t ncolblk;   // CTAs along channels (32 vectors each)
     uint32_t ngroups;   // CTAs along seqlen per batch entry (kRows chunks each)
+    uint8_t *codes, *scales;   // x kept in 8 bits beside the output (kCodes), dense (batch, seqlen, dim) and its groups
+    uint32_t groups;           // scales per token
 };
 
 #ifndef CC1D_FWD_CL_TMA
@@ -560,6 +562,7 @@ template <typename T> struct FwdTma {
     static constexpr int kStageBytes = kTmaRows * kRowBytes;
     static constexpr size_t kSmem = (size_t)kTmaWarps * kTmaStages * kStageBytes + (size_t)kTmaWarps * kTmaStages * 8;
     static constexpr int kMinBlocks = sizeof(T) == 4 ? CC1D_FWD_TMA_MINBLK : CC1D_FWD_TMA_MINBLK_16BIT;
+    static constexpr int kMinBlocksCodes = sizeof(T) == 4 ? CC1D_FWD_TMA_MINBLK : 4;     // the codes' registers cost a CTA
 };
 template <typename R> __device__ __forceinline__ R fwd_lds(uint32_t addr);
 template <> __device__ __forceinline__ uint4 fwd_lds<uint4>(uint32_t addr) { return lds128(addr); }
@@ -569,8 +572,11 @@ template <> __device__ __forceinline__ uint2 fwd_lds<uint2>(uint32_t addr) {
     return v;
 }
 
-template <typename T, int W, bool kSilu, bool kSeqIdx>
-__global__ void __launch_bounds__(32 * kTmaWarps, FwdTma<T>::kMinBlocks)
+// kCodes: x is also left in 8 bits; a group is 8 lanes of one token, and what is past dim arrives as zeros.  More
+// arithmetic than the copy leaves room for: (1,5376,8192) bf16 with seq_idx 48 us, 32 without, 32 + 34 with a kernel of
+// its own for the codes.
+template <typename T, int W, bool kSilu, bool kSeqIdx, bool kCodes>
+__global__ void __launch_bounds__(32 * kTmaWarps, kCodes ? FwdTma<T>::kMinBlocksCodes : FwdTma<T>::kMinBlocks)
 fwd_cl_tma_kernel(const FwdClArgs a, const __grid_constant__ CUtensorMap xmap) {
     pdl_wait();
     constexpr int C = kFwdTmaC;
@@ -643,6 +649,19 @@ fwd_cl_tma_kernel(const FwdClArgs a, const __grid_constant__ CUtensorMap xmap) {
         }
     }
 
+    uint8_t *codes = kCodes ? a.codes + ((uint64_t)b * (uint64_t)L + t0) * (uint64_t)a.dim + (uint64_t)col * C : nullptr;
+    uint8_t *scales = kCodes ? a.scales + ((uint64_t)b * (uint64_t)L + t0) * a.groups + col / (kCodeGroup / C) : nullptr;
+    const auto keep = [&](const R &raw, int r) {
+        if constexpr (kCodes) {
+            uint32_t s;
+            const uint32_t c = codes_of_group<T>(raw, s);
+            if (lane_ok) {
+                *reinterpret_cast<uint32_t *>(codes + (int64_t)r * a.dim) = c;
+                if ((lane & (kCodeGroup / C - 1)) == 0) scales[(int64_t)r * a.groups] = (uint8_t)s;
+            }
+        }
+    };
+
     // sequence ids of a box are fetched one box ahead, so that their latency hides behind a box;
     // one id per lane: lane l holds the id of row l % kTmaRows (-2 past the chunk: matches nothing)
     const int myrow = lane & (kTmaRows - 1);
@@ -676,12 +695,14 @@ fwd_cl_tma_kernel(const FwdClArgs a, const __grid_constant__ CUtensorMap xmap) {
             #pragma unroll
             for (int r = 0; r < kTmaRows; ++r) {
                 const R raw = fwd_lds<R>(src + r * kTmaRowBytes);
+                keep(raw, r);
                 fwd_cl_token_impl<T, W, C, kSilu, false, kTanh>(raw, 0, win, sw, wv, bv, optr + r * os, lane_ok);
             }
         } else if (rows >= kTmaRows) {
             #pragma unroll
             for (int r = 0; r < kTmaRows; ++r) {
                 const R raw = fwd_lds<R>(src + r * kTmaRowBytes);
+                keep(raw, r);
                 fwd_cl_token_impl<T, W, C, kSilu, kSeqIdx, kTanh>(raw, sid[r], win, sw, wv, bv, optr + r * os, lane_ok);
             }
         } else {
@@ -689,12 +710,14 @@ fwd_cl_tma_kernel(const FwdClArgs a, const __grid_constant__ CUtensorMap xmap) {
             for (int r = 0; r < kTmaRows; ++r) {
                 if (r < rows) {
                     const R raw = fwd_lds<R>(src + r * kTmaRowBytes);
+                    keep(raw, r);
                     fwd_cl_token<T, W, C, kSilu, kSeqIdx, kTanh>(raw, sid[r], win, sw, wv, bv, optr + r * os, lane_ok);
                 }
             }
         }
         optr += kTmaRows * os;
         if (kSeqIdx) sp += kTmaRows;
+        if (kCodes) { codes += (int64_t)kTmaRows * a.dim; scales += (int64_t)kTmaRows * a.groups; }
         __syncwarp();                                   // every lane has consumed the box
         if (lane == 0 && st + kTmaStages < nst) {       // refill it
             fence_proxy_async_smem();
@@ -741,7 +764,7 @@ int pick_chunk_tokens(int64_t batch, int64_t ncolblk, int64_t seqlen, int warps_
     return best;
 }
 
-int launch_fwd_channel_last(const cc1d_fwd_params &p, cudaStream_t stream) {
+int launch_fwd_channel_last(const cc1d_fwd_params &p, cudaStream_t stream, const cc1d_codes *codes, bool *kept) {
     if (p.batch == 0 || p.dim == 0 || p.seqlen == 0) return CC1D_OK;
     // token positions are 32-bit integers in the kernels (chunk starts plus a halo must not wrap)
     if (p.seqlen >= (1ll << 31) - 4096 || p.dim >= (1ll << 31)) return CC1D_ERR_TOO_LARGE;
@@ -752,7 +775,7 @@ int launch_fwd_channel_last(const cc1d_fwd_params &p, cudaStream_t stream) {
     if (p.final_states && (!is_aligned16(p.final_states) || p.final_states_batch_stride % C ||
                            p.final_states_l_stride % C)) return CC1D_ERR_ALIGN;
     const int sms = num_sms();
-    FwdClArgs a;
+    FwdClArgs a = {};
     a.x = p.x; a.out = p.out; a.weight = p.weight; a.bias = p.bias; a.seq_idx = p.seq_idx;
     a.init = p.initial_states; a.fin = p.final_states;
     a.x_bs = p.x_batch_stride; a.x_ls = p.x_l_stride; a.o_bs = p.out_batch_stride; a.o_ls = p.out_l_stride;
@@ -798,12 +821,17 @@ int launch_fwd_channel_last(const cc1d_fwd_params &p, cudaStream_t stream) {
         t.ngroups = (uint32_t)((tchunks + kTmaWarps - 1) / kTmaWarps);
         const uint64_t tctas = (uint64_t)t.ncolblk * t.ngroups * (uint64_t)p.batch;
         if (tctas >= (1ull << 31)) return CC1D_ERR_TOO_LARGE;
+        if (codes != nullptr && p.dim % kFwdTmaC == 0) {
+            t.codes = codes->codes; t.scales = codes->scales;
+            t.groups = (uint32_t)((p.dim + kCodeGroup - 1) / kCodeGroup);
+            *kept = true;
+        }
         CC1D_DISPATCH_ITYPE(p.itype, CC1D_DISPATCH_WIDTH(p.width, CC1D_DISPATCH_BOOL(p.silu != 0, kSilu,
-            CC1D_DISPATCH_BOOL(p.seq_idx != nullptr, kSeqIdx, {
-                auto kernel = fwd_cl_tma_kernel<T, W, kSilu, kSeqIdx>;
+            CC1D_DISPATCH_BOOL(p.seq_idx != nullptr, kSeqIdx, CC1D_DISPATCH_BOOL(t.codes != nullptr, kCodes, {
+                auto kernel = fwd_cl_tma_kernel<T, W, kSilu, kSeqIdx, kCodes>;
                 allow_dynamic_smem(reinterpret_cast<const void *>(kernel), FwdTma<T>::kSmem);
                 launch_k(kernel, dim3((unsigned)tctas), dim3(32 * kTmaWarps), FwdTma<T>::kSmem, stream, t, xmap);
-            }););););
+            });););););
         return check_launch();
     }
 #endif

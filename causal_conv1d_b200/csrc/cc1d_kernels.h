@@ -33,20 +33,21 @@ inline int elem_size(int dtype) { return dtype == CC1D_F32 ? 4 : 2; }
 inline int vec_elems(int dtype) { return 16 / elem_size(dtype); }
 
 // The calls of include/cc1d.h with x kept in, or taken from, 8 bits (where the kernels can: see below)
-int cc1d_fwd_keeping(const cc1d_fwd_params *p, const cc1d_codes *codes, cc1d_stream_t stream);
+int cc1d_fwd_keeping(const cc1d_fwd_params *p, const cc1d_codes *codes, bool *kept, cc1d_stream_t stream);
 int cc1d_bwd_check(const cc1d_bwd_params *p);
 int cc1d_bwd_reading(const cc1d_bwd_params *p, const cc1d_codes *codes, cc1d_stream_t stream);
 
 uint64_t groups_per_unit(uint64_t rows, uint64_t groups_per_row);
 int launch_fwd_channel_first(const cc1d_fwd_params &p, cudaStream_t stream, const cc1d_codes *codes = nullptr);   // codes: only where fwd_keeps_codes
 bool fwd_keeps_codes(const cc1d_fwd_params &p);     // channel-first rows whose kernel can keep x in 8 bits on its way
-int launch_fwd_channel_last(const cc1d_fwd_params &p, cudaStream_t stream);
+int launch_fwd_channel_last(const cc1d_fwd_params &p, cudaStream_t stream, const cc1d_codes *codes = nullptr, bool *kept = nullptr);   // *kept: x is in `codes` too
 
 size_t bwd_workspace_bytes_channel_first(const cc1d_bwd_params &p);
 size_t bwd_workspace_bytes_channel_last(const cc1d_bwd_params &p);
 int launch_bwd_channel_first(const cc1d_bwd_params &p, cudaStream_t stream, const cc1d_codes *codes = nullptr);   // codes: only where bwd_reads_codes
 bool bwd_reads_codes(const cc1d_bwd_params &p);     // ... and whose backward can read x in 8 bits
-int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream);
+int launch_bwd_channel_last(const cc1d_bwd_params &p, cudaStream_t stream, const cc1d_codes *codes = nullptr);    // codes: only where bwd_cl_reads_codes
+bool bwd_cl_reads_codes(const cc1d_bwd_params &p);  // the same of channel-last rows
 
 size_t peer_allreduce_buffer_bytes(int world, int64_t count);
 int launch_peer_allreduce(const cc1d_peer_allreduce_params &p, cudaStream_t stream);

@@ -82,6 +82,7 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 // caller then uses the non-TMA kernel).
 bool make_channel_last_tensor_map(CUtensorMap *map, int dtype, const void *base, int64_t dim, int64_t seqlen,
                                   int64_t batch, int64_t l_stride, int64_t batch_stride, int row_bytes = kTmaRowBytes);
+bool make_codes_tensor_map(CUtensorMap *map, const uint8_t *base, int64_t dim, int64_t seqlen, int64_t batch, int box_channels);
 
 // Host: tensor map over a channel-first tensor (seqlen, dim, batch) with element strides
 // (1, c_stride, batch_stride) and a box of [box_tokens tokens, box_channels channels, 1]: the box

@@ -32,14 +32,14 @@ typedef struct cc1d_codes {
 int cc1d_checkpoint_e4m3(const cc1d_fwd_params *p, const cc1d_codes *to, cc1d_stream_t stream);
 int cc1d_restore_e4m3(const cc1d_fwd_params *p, void *x, const cc1d_codes *from, cc1d_stream_t stream);
 
-/* cc1d_fwd, and x kept: in one pass over x where the rows are 16-bit, channel-first, 32-byte aligned
- * and a multiple of 16 long, else by a second kernel. */
+/* cc1d_fwd, and x kept: in one pass over x where it is channel-last, or channel-first in 16 bits with rows 32-byte
+ * aligned and a multiple of 16 long, else by a second kernel. */
 int cc1d_fwd_e4m3(const cc1d_fwd_params *p, const cc1d_codes *to, cc1d_stream_t stream);
 
 /* cc1d_bwd with x taken from codes.  p->x itself is not read and may be NULL; x's strides say its
  * layout class.  `restored`: scratch of cc1d_bwd_e4m3_restore_bytes() bytes, 32-byte aligned; that is 0 where
- * the backward reads the codes as they are (the rows that cc1d_fwd_e4m3 does in one pass), else room for a
- * dense x. */
+ * the backward reads the codes as they are (16-bit types: channel-first rows as above, channel-last ones of a multiple of
+ * 16 channels beside a channel-last dout), else room for a dense x. */
 size_t cc1d_bwd_e4m3_restore_bytes(const cc1d_bwd_params *p);
 int cc1d_bwd_e4m3(const cc1d_bwd_params *p, const cc1d_codes *from, void *restored, cc1d_stream_t stream);
 

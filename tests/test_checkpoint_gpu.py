@@ -189,3 +189,31 @@ def test_in_front_of_the_delta_rule():
                             (got[2], want[2], 8 * 2 ** -8, "dg"), (got[3], want[3], 8 * 2 ** -8, "dbeta")]:
         a, b = a.detach().double().cpu(), b.detach()
         assert (a - b).norm() <= tol * b.norm(), (name, ((a - b).norm() / b.norm()).item())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,D,L,W,form", [(1, 48, 333, 4, "packed"), (2, 176, 40, 3, "states"), (1, 272, 1000, 4, "packed"), (3, 16, 9, 2, "states"),
+                                          (2, 64, 1, 4, "plain"), (2, 40, 130, 4, "packed"), (2, 160, 523, 4, "window")])
+def test_channel_last_in_its_own_kernels(dtype, B, D, L, W, form):
+    """Channel-last rows of whole and broken groups, read from the codes (40 channels: restored first): the bits of
+    the plain backward of the kept x."""
+    from causal_conv1d_b200 import causal_conv1d_fn
+    t = DT[dtype]
+    x = make(B, D, L, t, True, seed=L, spread=False).requires_grad_()
+    at = kept(x, True).to(t).cuda().mT.contiguous().mT.requires_grad_()
+    w, b = (torch.rand(D, W, device="cuda") - 0.5).requires_grad_(), (torch.rand(D, device="cuda") - 0.5).requires_grad_()
+    dout = torch.randn(B, L, 2 * D, device="cuda").to(t)[..., :D].mT if form == "window" else torch.randn(B, L, D, device="cuda").to(t).mT
+    kw, more = {}, ()
+    if form == "packed":
+        kw["seq_idx"] = torch.sort(torch.randint(0, 6, (B, L), device="cuda", dtype=torch.int32), dim=1).values
+    if form == "states":
+        init = torch.randn(B, W - 1, D, device="cuda").to(t).mT.requires_grad_()
+        kw["initial_states"], more = init, (init,)
+    for x_, checkpoint in ((x, "e4m3"), (at, None)):
+        out = causal_conv1d_fn(x_, w, b, activation="silu", checkpoint=checkpoint, **kw)
+        grads = torch.autograd.grad(out, (x_, w, b, *more), dout)
+        if checkpoint:
+            got, first = grads, out
+    assert torch.equal(first, causal_conv1d_fn(x, w, b, activation="silu", **kw))
+    for a, c in zip(got, grads):
+        assert torch.equal(a, c)
