@@ -573,7 +573,7 @@ template <> __device__ __forceinline__ uint2 fwd_lds<uint2>(uint32_t addr) {
 }
 
 // kCodes: x is also left in 8 bits; a group is 8 lanes of one token, and what is past dim arrives as zeros.  More
-// arithmetic than the copy leaves room for: (1,5376,8192) bf16 with seq_idx 48 us, 32 without, 32 + 34 with a kernel of
+// arithmetic than the copy leaves room for: (1,5376,8192) bf16 with seq_idx 51 us, 32 without, 32 + 34 with a kernel of
 // its own for the codes.
 template <typename T, int W, bool kSilu, bool kSeqIdx, bool kCodes>
 __global__ void __launch_bounds__(32 * kTmaWarps, kCodes ? FwdTma<T>::kMinBlocksCodes : FwdTma<T>::kMinBlocks)

@@ -393,6 +393,8 @@ template <typename T> __device__ __forceinline__ void store8(T *dst, const float
 //   dg is its sum from the chunk's end.
 // U dS^T has a barrier of its own: dS is split while the first product runs, and the next panel's [dO; dB] and
 // S0, or the tile below, are made while it runs itself (training step 2 x 4096 x 32 heads 1355 -> 1311 us).
+// Bound by its chain of phases: about 33,000 cycles a head and chunk (one CTA an SM, 215 KB), 12,500 of them
+// products; its record, 192 KB a head and chunk written by the walks and read here, is 1.5 TB/s.
 // [M_P; M_A] is one tile of shared memory: rows as the contraction's results for the products with K, and
 // (read with its rows as the contraction) its own transpose for those with [Q; K].
 template <typename T, int kSteps>

@@ -218,7 +218,9 @@ template <typename T, bool kBack> struct Prep {
 
 // One CTA makes one chunk of one value head: K K^T and Q K^T by one MMA with the 128 rows [K; Q], then
 // warps 0, 1 the rows of A and warps 2, 3 those of P, the inverse, and the image out by one bulk copy.
-// A chain of short dependent steps: what fills the SM is that five CTAs share it (bf16).
+// A chain of short dependent steps: what fills the SM is that five CTAs share it (bf16).  8192 chunks of
+// 128 x 128 take 142 us: 8,300 warp instructions a chunk at 49 % of the issue slots, the rest barriers, waits for
+// results and instruction fetches.  (In the walk itself the same steps took 13,000 cycles a chunk.)
 template <typename T, int kSteps, bool kBack>
 __global__ void __launch_bounds__(kThreads, 5)
 gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images) {

@@ -32,7 +32,11 @@ template <typename T, bool kBack> struct Fwd {
 //   O = scale (e^G Q S + P U)                  S <- e^{G_C} S + K^T U''
 // All five products run on tcgen05 with the transposed left factor (S^T, R^T, U^T, U''^T: 128 dim_v
 // rows) in tensor memory and the right one (K, Q, T, P) in shared memory, so nothing that the walk
-// computes passes through shared memory.  S itself is kept and decayed in fp32 registers; only
+// computes passes through shared memory.  What bounds it is the chain of a chunk, 7,500 cycles (4.0 us, bf16,
+// 128 x 128; 64 chunks of 128 heads and rows 258 us): S^T K^T -> R -> (T - I) R -> U -> K^T U'' -> S, each link a
+// product, a wait, and registers split into pieces and put back into tensor memory; 3,200 of them are products
+// (33 cycles an instruction of 64 columns, 66 of 128), and the rest fills 47 % of the issue slots.  One sequence
+// and head a CTA, so few heads leave SMs idle: cc1d_gdr_prep.cu cuts long sequences into segments then.  S itself is kept and decayed in fp32 registers; only
 // its pieces are rewritten every chunk.
 // A token whose R is infinite or NaN in some column takes part as zero there (as do rows of T: GdrGates::bad), for a zero of T or P times NaN
 // would reach the tokens before it; `bad` holds the first such token of each column, and from it on the

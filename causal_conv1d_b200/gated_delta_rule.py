@@ -10,6 +10,10 @@ Per sequence and value head, with a state S of (dim_k, dim_v) in float32 and a_t
     o_t = scale * S_t^T q_t
 
 Value head h uses key head h // (heads_v // heads_k).  dim_k and dim_v are multiples of 8 up to 128.
+g, the logarithm of the decay, is meant to be at most 0; sums of positive ones above 88 within 64 tokens leave
+float32.  A token that is not finite makes itself and those behind it in its sequence and head NaN, none before.
+A call takes its workspace from the caching allocator on the current stream, so calls on several streams, and
+captured graphs, have one each.
 """
 import torch
 from torch import Tensor
@@ -89,8 +93,8 @@ def gated_delta_rule_fn(
 
     out: (batch, seqlen, heads_v, dim_v); with return_final_state also (sequences, heads_v, dim_k, dim_v)
 
-    The backward computes the forward's states again; it needs about 230 KB of workspace for each 64
-    tokens of a value head while it runs. Sums are taken in a fixed order.
+    The backward computes the forward's states again; it needs about 236 KB of workspace (16-bit types;
+    244 KB for float32) for each 64 tokens of a value head while it runs. Sums are taken in a fixed order.
     """
     return GatedDeltaRuleFn.apply(q, k, v, g, beta, initial_state, return_final_state, cu_seqlens, scale)
 

@@ -20,9 +20,14 @@ extern "C" {
  *
  *   S_t = a_t S_{t-1} + k_t (beta_t (v_t - a_t S_{t-1}^T k_t))^T      o_t = scale * S_t^T q_t
  *
- * Value head h uses key head h / (heads_v / heads_k).  g = -inf forgets the state.  All sums and
- * the state are fp32 (the tensor-core products split every factor into bf16 pieces until what
- * is left is below fp32's own rounding).
+ * Value head h uses key head h / (heads_v / heads_k).  g = -inf forgets the state.  g is meant to be
+ * at most 0: where positive ones add up to more than 88 over 64 tokens, e^sum leaves fp32 and the
+ * tokens behind are NaN.  A token whose values are infinite or NaN gives NaN to itself and to those
+ * behind it in its sequence and head (in the dim_v columns it touches), to none before.
+ * All sums and the state are fp32.  The tensor-core products split their fp32 factors into bf16
+ * pieces: three (24 bits) of the state, of every factor of fp32 inputs and in the gradients of g
+ * and beta; two (2^-17) of the chunk's U, P and of the correction (T - I) R where the result is
+ * rounded to 16 bits or is a small part of its sum.
  *
  * Sequences: `batch` rows of `seqlen` tokens, or (cu_seqlens != NULL) batch == 1 and nseq packed
  * sequences, sequence s owning tokens [cu_seqlens[s], cu_seqlens[s+1]) of the seqlen tokens;
