@@ -141,14 +141,7 @@ def causal_conv1d_fwd_e4m3_function(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The forward, and x in 8 bits: codes uint8, dense in x's layout class ((batch, seqlen, dim) for a
     channel-last x), and the scales' biased exponents, one for each 32 codes of a row; eager only."""
-    batch, dim, seqlen = x.shape
-    rows = (batch, seqlen, dim) if x.stride(1) == 1 and x.stride(2) > 1 else (batch, dim, seqlen)
-    codes = torch.empty(rows, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(rows[0], rows[1], (rows[2] + 31) // 32, dtype=torch.uint8, device=x.device)
-    out = torch.empty_like(x)
-    _ext.causal_conv1d_fwd(x, weight, bias, seq_idx, initial_states, out, final_states_out, silu_activation,
-                           codes, scales)
-    return out, codes, scales
+    return _ext.causal_conv1d_fwd_e4m3(x, weight, bias, seq_idx, initial_states, final_states_out, silu_activation)
 
 
 def causal_conv1d_bwd_e4m3_function(
@@ -166,22 +159,8 @@ def causal_conv1d_bwd_e4m3_function(
     silu_activation: bool,
 ) -> tuple[torch.Tensor | None]:
     """``causal_conv1d_bwd_function`` with x (of ``dtype``) as ``causal_conv1d_fwd_e4m3_function`` kept it."""
-    dx = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-    if channel_last:
-        dx = dx.transpose(1, 2)
-    batch, dim, _ = dx.shape
-    dweight = torch.empty_like(weight, dtype=torch.float32)
-    dbias = torch.empty_like(bias, dtype=torch.float32) if bias is not None else None
-    dinitial_states = None
-    if return_dinitial_states:
-        dinitial_states = torch.empty(batch, weight.size(-1) - 1, dim, device=dx.device, dtype=dtype).transpose(1, 2)
-    # dx also stands for x: its shape, dtype and layout class
-    _ext.causal_conv1d_bwd(dx, weight, bias, dout, seq_idx, initial_states, dfinal_states, dx, dweight, dbias,
-                           dinitial_states, silu_activation, False, codes=codes, scales=scales)
-    dweight = dweight.type_as(weight)
-    if dbias is not None:
-        dbias = dbias.type_as(bias)
-    return dx, dweight, dbias, dinitial_states
+    return _ext.causal_conv1d_bwd_e4m3(codes, scales, dtype, channel_last, weight, bias, dout, seq_idx, initial_states,
+                                       dfinal_states, return_dinitial_states, silu_activation)
 
 
 def causal_conv1d_update_function(

@@ -10,6 +10,7 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <tuple>
 #include <vector>
 
 #include "cc1d.h"
@@ -267,6 +268,43 @@ void causal_conv1d_bwd(const at::Tensor &x, const at::Tensor &weight, const OptT
         rc = run();
     }
     raise_on(rc, "causal_conv1d_bwd");
+}
+
+// The forward and backward with x in 8 bits allocate what they return: from Python the seven tensors of a step
+// cost more than a small step itself.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> causal_conv1d_fwd_e4m3(const at::Tensor &x, const at::Tensor &weight, const OptTensor &bias_,
+                                                                      const OptTensor &seq_idx_, const OptTensor &initial_states_,
+                                                                      OptTensor final_states_out_, bool silu_activation) {
+    need_cuda(x, "x");
+    TORCH_CHECK(x.dim() == 3, "x must be (batch, dim, seqlen)");
+    const bool cl = x.stride(1) == 1 && x.stride(2) > 1;
+    const int64_t rows = x.size(cl ? 2 : 1), cols = x.size(cl ? 1 : 2);
+    const auto bytes = x.options().dtype(at::kByte);
+    at::Tensor codes = at::empty({x.size(0), rows, cols}, bytes), scales = at::empty({x.size(0), rows, (cols + 31) / 32}, bytes);
+    at::Tensor out = at::empty_like(x);
+    causal_conv1d_fwd(x, weight, bias_, seq_idx_, initial_states_, out, final_states_out_, silu_activation, codes, scales);
+    return {out, codes, scales};
+}
+
+std::tuple<at::Tensor, at::Tensor, OptTensor, OptTensor> causal_conv1d_bwd_e4m3(
+        const at::Tensor &codes, const at::Tensor &scales, at::ScalarType dtype, bool channel_last, const at::Tensor &weight, const OptTensor &bias_,
+        at::Tensor dout, const OptTensor &seq_idx_, const OptTensor &initial_states_, const OptTensor &dfinal_states_,
+        bool return_dinitial_states, bool silu_activation) {
+    need_cuda(codes, "codes");
+    TORCH_CHECK(codes.dim() == 3 && weight.dim() == 2, "codes must be (batch, rows, columns) and weight (dim, width)");
+    const auto options = codes.options().dtype(dtype);
+    at::Tensor dx = at::empty(codes.sizes(), options);
+    if (channel_last) dx = dx.transpose(1, 2);
+    at::Tensor dweight = at::empty(weight.sizes(), options.dtype(at::kFloat));
+    OptTensor dbias, dinitial_states;
+    if (bias_.has_value()) dbias = at::empty(bias_->sizes(), options.dtype(at::kFloat));
+    if (return_dinitial_states) dinitial_states = at::empty({codes.size(0), weight.size(1) - 1, dx.size(1)}, options).transpose(1, 2);
+    // dx also stands for x: its shape, dtype and layout class
+    causal_conv1d_bwd(dx, weight, bias_, dout, seq_idx_, initial_states_, dfinal_states_, dx, dweight, dbias, dinitial_states, silu_activation,
+                      false, {}, 0, 0, OptTensor(), 0, 0, OptTensor(), codes, scales);
+    dweight = dweight.to(weight.scalar_type());
+    if (dbias.has_value()) dbias = dbias->to(bias_->scalar_type());
+    return {dx, dweight, dbias, dinitial_states};
 }
 
 void causal_conv1d_update(const at::Tensor &x, const at::Tensor &conv_state, const at::Tensor &weight,
@@ -644,6 +682,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("accumulate") = true, py::arg("peer_ptrs") = std::vector<int64_t>(), py::arg("peer_rank") = 0,
           py::arg("peer_capacity") = 0, py::arg("peer_status") = py::none(), py::arg("peer_spin_limit") = 0,
           py::arg("phase") = 0, py::arg("workspace") = py::none(), py::arg("codes") = py::none(), py::arg("scales") = py::none());
+    m.def("causal_conv1d_fwd_e4m3", &causal_conv1d_fwd_e4m3, "Causal conv1d forward that keeps x in 8 bits");
+    m.def("causal_conv1d_bwd_e4m3", &causal_conv1d_bwd_e4m3, "Causal conv1d backward of an x kept in 8 bits");
     m.def("bwd_workspace_bytes", [](int64_t batch, int64_t dim, int64_t seqlen, int64_t width, int64_t elem_bytes, bool channel_last) {
         cc1d_bwd_params q = {};
         q.itype = elem_bytes == 4 ? CC1D_F32 : CC1D_BF16; q.wtype = CC1D_F32; q.width = (int32_t)width;

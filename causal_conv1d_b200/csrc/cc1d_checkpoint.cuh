@@ -10,12 +10,10 @@ constexpr int kCodeGroup = 32;     // neighbours that share a scale
 // Biased exponent of the least power of two s with most / s <= 448 = 1.75 * 2^8; 255 when most is
 // infinite or NaN, at least 1 (2^-126, below which 2^-s would leave the normal numbers).
 __device__ __forceinline__ uint32_t code_scale(float most) {
-    const uint32_t b = __float_as_uint(most), e = b >> 23;
-    if (e == 255u) return 255u;
-    const int s = (int)e - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return (uint32_t)(s < 1 ? 1 : s);
+    const uint32_t b = __float_as_uint(most);       // a mantissa above 1.75's carries into the exponent
+    return b >= 0x7f800000u ? 255u : (uint32_t)max((int)((b + 0x1fffffu) >> 23) - 8, 1);
 }
-__device__ __forceinline__ float scale_inverse(uint32_t s) { return __uint_as_float((s < 254u ? 254u - s : 0u) << 23); }
+__device__ __forceinline__ float scale_inverse(uint32_t s) { return __uint_as_float((uint32_t)max(254 - (int)s, 0) << 23); }
 __device__ __forceinline__ float scale_value(uint32_t s) { return __uint_as_float(s == 255u ? 0x7fc00000u : s << 23); }
 
 // A NaN has to come out of the maximum (max itself drops it)
@@ -28,25 +26,40 @@ __device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d)
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return (uint32_t)lo | ((uint32_t)hi << 16);
 }
-// 4 neighbouring values of each of 8 lanes, a group -> this lane's codes, and the group's scale.  The bits of
-// a float without their sign are ordered like the values, with infinities above all numbers and NaN above
-// those, so the largest magnitude is an integer's (of 16-bit types two at a time).
-template <typename T> __device__ __forceinline__ uint32_t codes_of_group(const uint2 &v, uint32_t &s) {
-    uint32_t m = __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu);
+// Largest magnitudes.  The bits of a float without their sign are ordered like the values, with infinities above
+// all numbers and NaN above those, so they are integers' maxima (of 16-bit types two at a time).
+__device__ __forceinline__ uint32_t most2(uint32_t a, uint32_t b) { return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu); }
+__device__ __forceinline__ uint32_t most2(const uint4 &v) { return __vmaxu2(most2(v.x, v.y), most2(v.z, v.w)); }
+template <typename T> __device__ __forceinline__ float most_of(uint32_t m) { return unpack_pair<T>(max(m & 0xffffu, m >> 16)).x; }
+
+template <typename T> __device__ __forceinline__ uint32_t codes_by(const uint2 &v, float inv) {
+    const float2 f = make_float2(inv, inv), a = mul2(unpack_pair<T>(v.x), f), b = mul2(unpack_pair<T>(v.y), f);
+    return to_codes(a.x, a.y, b.x, b.y);
+}
+template <typename T> __device__ __forceinline__ uint32_t codes_by(const uint4 &v, float inv) {
+    return to_codes(__uint_as_float(v.x) * inv, __uint_as_float(v.y) * inv, __uint_as_float(v.z) * inv, __uint_as_float(v.w) * inv);
+}
+// 4 neighbouring values of each of 8 lanes are a group: codes and scales of two groups (two tokens), whose
+// maxima go through the shuffles in one register where they are 16-bit
+template <typename T> __device__ __forceinline__ void codes_of_groups(const uint2 &u, const uint2 &v, uint32_t (&c)[2], uint32_t (&s)[2]) {
+    const uint32_t a = most2(u.x, u.y), b = most2(v.x, v.y);
+    uint32_t m = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
     #pragma unroll
     for (int i = 1; i < 8; i <<= 1) m = __vmaxu2(m, __shfl_xor_sync(kFullMask, m, i));
-    s = code_scale(unpack_pair<T>(max(m & 0xffffu, m >> 16)).x);
-    const float inv = scale_inverse(s);
-    const float2 a = unpack_pair<T>(v.x), b = unpack_pair<T>(v.y);
-    return to_codes(a.x * inv, a.y * inv, b.x * inv, b.y * inv);
+    const float2 most = unpack_pair<T>(m);
+    s[0] = code_scale(most.x); s[1] = code_scale(most.y);
+    c[0] = codes_by<T>(u, scale_inverse(s[0])); c[1] = codes_by<T>(v, scale_inverse(s[1]));
 }
-template <typename T> __device__ __forceinline__ uint32_t codes_of_group(const uint4 &v, uint32_t &s) {
-    uint32_t m = max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+template <typename T> __device__ __forceinline__ void codes_of_groups(const uint4 &u, const uint4 &v, uint32_t (&c)[2], uint32_t (&s)[2]) {
+    const uint4 w[2] = {u, v};
     #pragma unroll
-    for (int i = 1; i < 8; i <<= 1) m = max(m, __shfl_xor_sync(kFullMask, m, i));
-    s = code_scale(__uint_as_float(m));
-    const float inv = scale_inverse(s);
-    return to_codes(__uint_as_float(v.x) * inv, __uint_as_float(v.y) * inv, __uint_as_float(v.z) * inv, __uint_as_float(v.w) * inv);
+    for (int k = 0; k < 2; ++k) {
+        uint32_t m = max(max(w[k].x & 0x7fffffffu, w[k].y & 0x7fffffffu), max(w[k].z & 0x7fffffffu, w[k].w & 0x7fffffffu));
+        #pragma unroll
+        for (int i = 1; i < 8; i <<= 1) m = max(m, __shfl_xor_sync(kFullMask, m, i));
+        s[k] = code_scale(__uint_as_float(m));
+        c[k] = codes_by<T>(w[k], scale_inverse(s[k]));
+    }
 }
 // 2 codes (the low 16 bits) times their scale
 __device__ __forceinline__ float2 from_codes(uint32_t codes, float scale) {

@@ -206,10 +206,8 @@ __global__ void __launch_bounds__(CC1D_FWD_WIDE_THREADS, CC1D_FWD_WIDE_MINBLK) f
                     for (int i = 0; i < 8; ++i) xx[W - 1 + i] = make_float2(af[i], bf[i]);
                     if constexpr (kCodes) {
                         // a group is this lane's 16 elements and its neighbour's
-                        float most = 0.f;
-                        #pragma unroll
-                        for (int i = 0; i < 8; ++i) most = max_abs(max_abs(most, af[i]), bf[i]);
-                        most = max_abs(most, __shfl_xor_sync(kFullMask, most, 1));
+                        const uint32_t two = __vmaxu2(most2(xa[j]), most2(xb[j]));
+                        const float most = most_of<T>(__vmaxu2(two, __shfl_xor_sync(kFullMask, two, 1)));
                         const uint32_t s = code_scale(most), e = g * kGroupElems + j * kSlotElems + lane * 16;
                         const float2 inv = splat2(scale_inverse(s));
                         #pragma unroll
@@ -573,7 +571,7 @@ template <> __device__ __forceinline__ uint2 fwd_lds<uint2>(uint32_t addr) {
 }
 
 // kCodes: x is also left in 8 bits; a group is 8 lanes of one token, and what is past dim arrives as zeros.  More
-// arithmetic than the copy leaves room for: (1,5376,8192) bf16 with seq_idx 51 us, 32 without, 32 + 34 with a kernel of
+// arithmetic than the copy leaves room for: (1,5376,8192) bf16 with seq_idx 50 us, 32 without, 32 + 34 with a kernel of
 // its own for the codes.
 template <typename T, int W, bool kSilu, bool kSeqIdx, bool kCodes>
 __global__ void __launch_bounds__(32 * kTmaWarps, kCodes ? FwdTma<T>::kMinBlocksCodes : FwdTma<T>::kMinBlocks)
@@ -651,13 +649,19 @@ fwd_cl_tma_kernel(const FwdClArgs a, const __grid_constant__ CUtensorMap xmap) {
 
     uint8_t *codes = kCodes ? a.codes + ((uint64_t)b * (uint64_t)L + t0) * (uint64_t)a.dim + (uint64_t)col * C : nullptr;
     uint8_t *scales = kCodes ? a.scales + ((uint64_t)b * (uint64_t)L + t0) * a.groups + col / (kCodeGroup / C) : nullptr;
-    const auto keep = [&](const R &raw, int r) {
+    const bool first_of_group = lane_ok && (lane & (kCodeGroup / C - 1)) == 0;
+    // rows r and r + 1 of a box (the second only when it is there)
+    const auto keep = [&](const R &u, const R &v, int r, bool second) {
         if constexpr (kCodes) {
-            uint32_t s;
-            const uint32_t c = codes_of_group<T>(raw, s);
+            uint32_t c[2], s[2];
+            codes_of_groups<T>(u, v, c, s);
             if (lane_ok) {
-                *reinterpret_cast<uint32_t *>(codes + (int64_t)r * a.dim) = c;
-                if ((lane & (kCodeGroup / C - 1)) == 0) scales[(int64_t)r * a.groups] = (uint8_t)s;
+                *reinterpret_cast<uint32_t *>(codes + (int64_t)r * a.dim) = c[0];
+                if (second) *reinterpret_cast<uint32_t *>(codes + (int64_t)(r + 1) * a.dim) = c[1];
+            }
+            if (first_of_group) {
+                scales[(int64_t)r * a.groups] = (uint8_t)s[0];
+                if (second) scales[(int64_t)(r + 1) * a.groups] = (uint8_t)s[1];
             }
         }
     };
@@ -695,14 +699,14 @@ fwd_cl_tma_kernel(const FwdClArgs a, const __grid_constant__ CUtensorMap xmap) {
             #pragma unroll
             for (int r = 0; r < kTmaRows; ++r) {
                 const R raw = fwd_lds<R>(src + r * kTmaRowBytes);
-                keep(raw, r);
+                if (kCodes && (r & 1) == 0) keep(raw, fwd_lds<R>(src + (r + 1) * kTmaRowBytes), r, true);
                 fwd_cl_token_impl<T, W, C, kSilu, false, kTanh>(raw, 0, win, sw, wv, bv, optr + r * os, lane_ok);
             }
         } else if (rows >= kTmaRows) {
             #pragma unroll
             for (int r = 0; r < kTmaRows; ++r) {
                 const R raw = fwd_lds<R>(src + r * kTmaRowBytes);
-                keep(raw, r);
+                if (kCodes && (r & 1) == 0) keep(raw, fwd_lds<R>(src + (r + 1) * kTmaRowBytes), r, true);
                 fwd_cl_token_impl<T, W, C, kSilu, kSeqIdx, kTanh>(raw, sid[r], win, sw, wv, bv, optr + r * os, lane_ok);
             }
         } else {
@@ -710,7 +714,7 @@ fwd_cl_tma_kernel(const FwdClArgs a, const __grid_constant__ CUtensorMap xmap) {
             for (int r = 0; r < kTmaRows; ++r) {
                 if (r < rows) {
                     const R raw = fwd_lds<R>(src + r * kTmaRowBytes);
-                    keep(raw, r);
+                    if (kCodes && (r & 1) == 0) keep(raw, fwd_lds<R>(src + (r + 1) * kTmaRowBytes), r, r + 1 < rows);
                     fwd_cl_token<T, W, C, kSilu, kSeqIdx, kTanh>(raw, sid[r], win, sw, wv, bv, optr + r * os, lane_ok);
                 }
             }

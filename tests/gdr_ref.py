@@ -1,4 +1,4 @@
-"""The gated delta rule token by token in float64, the checker of the delta-rule tests."""
+"""The gated delta rule token by token in float64, what the delta-rule tests compare with."""
 import torch
 
 
