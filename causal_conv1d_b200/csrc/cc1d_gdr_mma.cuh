@@ -265,6 +265,7 @@ __device__ __forceinline__ bool gdr_find_chunk(const cc1d_gdr_params &p, int64_t
     if (p.cu_seqlens == nullptr) {
         n = (int)(slot / ((p.seqlen + kChunk - 1) / kChunk));
     } else {
+        if (p.nseq == 0) return false;         // all tokens are behind the last sequence
         int last = (int)p.nseq - 1;            // the last sequence whose first slot is not behind this one
         while (n < last) {
             const int mid = (n + last + 1) / 2;

@@ -213,3 +213,20 @@ def test_empty_batches_and_rows():
         d = torch.randn_like(last)
         got = torch.autograd.grad(last, leaves + [S0], d, allow_unused=True)
         assert torch.equal(got[5], d)
+
+
+@pytest.mark.parametrize("heads", [2, 160])
+def test_no_sequence_at_all(heads):
+    """cu_seqlens of one entry: every token is behind the last sequence, zero outputs and gradients."""
+    import causal_conv1d_b200 as cc
+    T = 200
+    leaves = [t.requires_grad_() for t in gdr_ref.inputs((1, T), heads // 2, heads, 32, 32, torch.bfloat16)]
+    cu = torch.full((1000,), T, dtype=torch.int32, device="cuda")[:1].zero_()      # what follows the entry is not read
+    out, last = cc.gated_delta_rule_fn(*leaves, return_final_state=True, cu_seqlens=cu)
+    assert last.shape == (0, heads, 32, 32) and not out.any()
+    for d in torch.autograd.grad(out, leaves, torch.ones_like(out)):
+        assert not d.any()
+    pool = torch.randn(3, heads, 32, 32, device="cuda")
+    kept = pool.clone()
+    out = cc.gated_delta_rule_varlen_fn(*(t.detach()[0] for t in leaves), cu_seqlens=cu, states=pool)
+    assert not out.any() and torch.equal(pool, kept)
