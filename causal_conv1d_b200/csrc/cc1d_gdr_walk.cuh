@@ -9,14 +9,20 @@ namespace {
 constexpr int kWalkers = 512, kWalkThreads = kWalkers + 64 + kFeeders;   // warps 0-15 walk the chunks, 16 issues their products, 17 stores, 18, 19 load
 
 // Columns of the walk's tensor memory (128 lanes = the dim_v rows of S^T, R^T, U^T, O^T).
-constexpr uint32_t kFwdColS = 0;      // 3 x 64: pieces of S^T, two dim_k per column; later in a chunk
+constexpr uint32_t kFwdColS = 0;      // 2 x 64: pieces of S^T, two dim_k per column (the third: col_s); later in a chunk
 constexpr uint32_t kFwdColDelta = 0;  //   128: U''^T K, and
-constexpr uint32_t kFwdColU = 128;    //   2 x 32: pieces of U^T (the third, fp32 inputs only, at 480)
+constexpr uint32_t kFwdColU = 128;    // 2 x 32: pieces of U^T (the third, fp32 inputs only, at 480)
 constexpr uint32_t kFwdColR = 192;    // 3 x 32: pieces of R^T, then of U''^T
 constexpr uint32_t kFwdColX = 288;    // 64: S^T K^T, then R^T (T - I)^T
 constexpr uint32_t kFwdColO = 352;    // 64: S^T Q^T
 constexpr uint32_t kFwdColY = 416;    // 64: U^T P^T
 __device__ __forceinline__ uint32_t col_u(int piece) { return piece < 2 ? kFwdColU + 32 * piece : 480; }
+// The third piece of S^T.  U^T P^T of the chunk before may still read U^T when the state is written, so not in U's
+// place: in that of R, which is written when S^T K^T is done.  Where S^T Q^T, done later, needs it too (fp32
+// inputs) it is in U's place, and the state is written when U^T P^T is done.
+template <int kOutPieces> __device__ __forceinline__ constexpr uint32_t col_s(int piece) {
+    return piece < 2 ? kFwdColS + 64 * piece : kOutPieces < 3 ? kFwdColR : kFwdColU;
+}
 
 enum GdrMode { kOutput, kKeep, kSummary };
 template <typename T, bool kBack> struct Fwd {
@@ -104,7 +110,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                         if (a >= 3 || b >= NP) continue;
                         #pragma unroll
                         for (int i = 0; i < kSteps; ++i)
-                            mma_ts(kFwdColX, kFwdColS + 64 * a + 8 * i, desc_add(kq, b * St::kKqPiece + (i >> 2) * St::kPanel + (i & 3) * 32), id, again(more));
+                            mma_ts(kFwdColX, col_s<PO>(a) + 8 * i, desc_add(kq, b * St::kKqPiece + (i >> 2) * St::kPanel + (i & 3) * 32), id, again(more));
                     }
                 }
                 mma_commit(bar_x);
@@ -123,7 +129,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                         if (a >= PO || b >= NP) continue;
                         #pragma unroll
                         for (int i = 0; i < kSteps; ++i)
-                            mma_ts(kFwdColO, kFwdColS + 64 * a + 8 * i, desc_add(kq, b * St::kKqPiece + 64 * 128 + (i >> 2) * St::kPanel + (i & 3) * 32), id, again(more));
+                            mma_ts(kFwdColO, col_s<PO>(a) + 8 * i, desc_add(kq, b * St::kKqPiece + 64 * 128 + (i >> 2) * St::kPanel + (i & 3) * 32), id, again(more));
                     }
                 }
             }
@@ -249,7 +255,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 for (int j = 0; j < 32; ++j) record->S0[32 * part + j][col] = S[j];
             }
             #pragma unroll
-            for (int b = 0; b < 4; ++b) split8_to_tmem<3>(S + 8 * b, mine + kFwdColS + 16 * part + 4 * b, 64, 128);
+            for (int b = 0; b < 4; ++b) split8_to_tmem<3>(S + 8 * b, mine + kFwdColS + 16 * part + 4 * b, 64, col_s<PO>(2) - kFwdColS);
             ready(bar_s);
         };
         if (chunks > 0) put_state();
@@ -342,6 +348,11 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 for (int j = 0; j < 32; ++j) S[j] = __uint_as_float(0x7fc00000u);
             }
             __syncwarp();
+            if (kOut && PO == 3) {
+                gdr_wait(bar_o, par, dead);             // U^T has been read (col_s)
+                __syncwarp();
+                fence_after_sync();
+            }
             if (c + 1 < chunks) put_state();
             // the output, while the next chunk's first product runs
             if (kOut) {
