@@ -193,8 +193,8 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
             const int64_t state_at = ((int64_t)n * heads + h) * dk * dv + (int64_t)(32 * part) * dv + col;
             #pragma unroll
             for (int j = 0; j < 32; ++j)
-                S[j] = kSum ? 0.f : !w.last ? w.segment[h].end[32 * part + j][col]
-                     : b.dfinal_states != nullptr && n < sequences && 32 * part + j < dk && col < dv ? b.dfinal_states[state_at + (int64_t)j * dv] : 0.f;
+                S[j] = kSum || 32 * part + j >= dk || col >= dv ? 0.f : !w.last ? w.segment[h].end[32 * part + j][col]
+                     : b.dfinal_states != nullptr && n < sequences ? b.dfinal_states[state_at + (int64_t)j * dv] : 0.f;
         }
         auto ready = [&](uint32_t bar) {
             tmem_wait_st();

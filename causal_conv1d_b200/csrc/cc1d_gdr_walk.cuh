@@ -218,9 +218,10 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             #pragma unroll
             for (int j = 0; j < 32; ++j) S[j] = unit && 32 * part + j == col ? 1.f : 0.f;
         } else if (!(w.first && w.last)) {
-            // (a first segment's too: its sequence's last one may already have written the state's row)
+            // (a first segment's too: its sequence's last one may already have written the state's row; what is past dim_v the
+            // join leaves as it lay in memory, and the gradients sum over all 128 columns)
             #pragma unroll
-            for (int j = 0; j < 32; ++j) S[j] = w.segment[h].start[32 * part + j][col];
+            for (int j = 0; j < 32; ++j) S[j] = 32 * part + j < dk && col < dv ? w.segment[h].start[32 * part + j][col] : 0.f;
         } else {
             const int64_t row = n < sequences ? gdr_state_row(p, n) : -1, state_at = (int64_t)(32 * part) * dv + col;
             const bool from = p.initial_states != nullptr && row >= 0 && (p.has_initial_state == nullptr || p.has_initial_state[n] != 0);

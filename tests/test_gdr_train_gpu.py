@@ -230,3 +230,19 @@ def test_no_sequence_at_all(heads):
     kept = pool.clone()
     out = cc.gated_delta_rule_varlen_fn(*(t.detach()[0] for t in leaves), cu_seqlens=cu, states=pool)
     assert not out.any() and torch.equal(pool, kept)
+
+
+def test_what_lies_in_the_workspace_does_not_matter():
+    """A long sequence of few heads, 72 columns, after memory full of NaN was given back to the allocator."""
+    import causal_conv1d_b200 as cc
+    leaves = [t.requires_grad_() for t in gdr_ref.inputs((1, 4000), 1, 2, 96, 72, torch.bfloat16, seed=3, slow=True)]
+    S0 = torch.randn(1, 2, 96, 72, device="cuda").requires_grad_()
+    first = None
+    for fill in (0.0, float("nan"), 1e30):
+        junk = [torch.full((1 << 25,), fill, device="cuda") for _ in range(4)]
+        del junk
+        out, last = cc.gated_delta_rule_fn(*leaves, initial_state=S0, return_final_state=True)
+        got = (out, last, *torch.autograd.grad((out, last), leaves + [S0], (torch.ones_like(out), torch.ones_like(last))))
+        first = first or got
+        for a, b in zip(got, first):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
