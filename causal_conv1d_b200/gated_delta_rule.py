@@ -25,7 +25,12 @@ def _rows(t: Tensor) -> Tensor:
     """t where the chunked kernels' 16-byte loads can read it, else a dense copy."""
     step = 16 // t.element_size()
     ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n <= 1 or s % step == 0 for n, s in zip(t.shape[:-1], t.stride()))
-    return t if ok else t.contiguous()
+    return t if ok else _dense_copy(t)
+
+
+def _dense_copy(t: Tensor) -> Tensor:
+    # (contiguous() returns a contiguous t itself, wherever in its storage that begins)
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 class GatedDeltaRuleFn(torch.autograd.Function):
@@ -33,7 +38,8 @@ class GatedDeltaRuleFn(torch.autograd.Function):
     def forward(ctx, q, k, v, g, beta, initial_state=None, return_final_state=False, cu_seqlens=None, scale=None):
         q, k, v = _rows(q), _rows(k), _rows(v)
         if initial_state is not None:
-            initial_state = initial_state.contiguous()
+            dense = initial_state.is_contiguous() and initial_state.data_ptr() % 16 == 0
+            initial_state = initial_state if dense else _dense_copy(initial_state)
         if cu_seqlens is not None:
             cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
         scale = q.shape[-1] ** -0.5 if scale is None else scale

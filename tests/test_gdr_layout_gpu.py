@@ -1,0 +1,53 @@
+"""Where the delta rule's tensors lie: storage offsets, and tokens that no sequence owns."""
+import pytest
+import torch
+
+import gdr_ref
+from conftest import DT
+
+pytestmark = pytest.mark.gpu
+
+
+def off_by_one(t):
+    """The same values, contiguous, one element behind a 16-byte boundary."""
+    there = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+    assert there.is_contiguous() and there.data_ptr() % 16 == t.element_size()
+    return there.copy_(t)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("which", ["q", "k", "v", "g", "beta", "initial_state", "dout", "dfinal_state"])
+def test_contiguous_tensors_off_a_16_byte_boundary(which, dtype):
+    import causal_conv1d_b200 as cc
+    names = ["q", "k", "v", "g", "beta", "initial_state", "dout", "dfinal_state"]
+    gen = torch.Generator().manual_seed(1)
+    state = lambda: torch.randn(2, 4, 64, 32, generator=gen).cuda()  # noqa: E731
+    args = dict(zip(names, (*gdr_ref.inputs((2, 70), 2, 4, 64, 32, DT[dtype]), state(), torch.randn(2, 70, 4, 32, generator=gen).to(DT[dtype]).cuda(), state())))
+
+    def run(a):
+        leaves = [a[n].detach().requires_grad_() for n in names[:6]]
+        out, last = cc.gated_delta_rule_fn(*leaves, return_final_state=True)
+        return (out, last, *torch.autograd.grad((out, last), leaves, (a["dout"], a["dfinal_state"])))
+
+    for a, b in zip(run({**args, which: off_by_one(args[which])}), run(args)):
+        assert torch.equal(a, b)
+
+
+def test_prefill_of_contiguous_tensors_off_a_16_byte_boundary():
+    import causal_conv1d_b200 as cc
+    args = [t[0] for t in gdr_ref.inputs((1, 70), 2, 4, 64, 32, torch.bfloat16)]
+    cu = torch.tensor([0, 70], dtype=torch.int32).cuda()
+    want = cc.gated_delta_rule_varlen_fn(*args, cu_seqlens=cu)
+    assert torch.equal(cc.gated_delta_rule_varlen_fn(*(off_by_one(t) for t in args), cu_seqlens=cu), want)
+
+
+def test_gradient_that_is_a_slice_of_a_flat_one():
+    """What the backward of torch.cat hands over starts wherever the output lay in the flat tensor."""
+    import causal_conv1d_b200 as cc
+    leaves = [t.requires_grad_() for t in gdr_ref.inputs((1, 70), 2, 4, 64, 32, torch.bfloat16)]
+    flat = torch.randn(1 + 70 * 4 * 32, device="cuda").bfloat16()
+    out = cc.gated_delta_rule_fn(*leaves)
+    got = torch.autograd.grad(torch.cat([torch.zeros_like(flat[:1]), out.flatten()]), leaves, flat)
+    out = cc.gated_delta_rule_fn(*leaves)
+    for a, b in zip(got, torch.autograd.grad(out, leaves, flat[1:].clone().view(out.shape))):
+        assert torch.equal(a, b)
