@@ -221,7 +221,7 @@ struct GdrGates {
     float from_start[kChunk], to_end[kChunk], beta[kChunk], minus_beta_from_start[kChunk];
     float row[kChunk], same[kChunk], column[3][48];
     int steep;
-    int bad;                          // first token whose row of T is not finite (64: none); such rows are left out
+    int bad;                          // first token whose row of A or T is not finite (64: none); such entries are left out
 };
 __device__ __forceinline__ float gdr_fade(float2 gi, float2 gj) { return gdr_exp((gi.x - gj.x) + (gi.y - gj.y)); }
 

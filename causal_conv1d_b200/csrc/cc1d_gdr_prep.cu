@@ -323,9 +323,10 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
                 }
             }
             if (warp < 2) {
-                // an infinite or NaN entry would reach the rows before it through products with zeros; the walk
-                // finds the token itself (its R is not finite) and gives NaN to it and those behind
+                // an infinite or NaN entry would reach the rows before it through products with zeros: its row is noted
+                // (the walk cannot see finite keys whose product overflows), and the walk gives NaN to it and those behind
                 if (!all_finite(x)) {
+                    atomicMin(&gates.bad, i);
                     #pragma unroll
                     for (int j = 0; j < 16; ++j) x[j] = finite(x[j]) ? x[j] : 0.f;
                 }

@@ -44,7 +44,7 @@ template <typename T, bool kBack> struct Fwd {
 // (33 cycles an instruction of 64 columns, 66 of 128), and the rest fills 47 % of the issue slots.  One sequence
 // and head a CTA, so few heads leave SMs idle: cc1d_gdr_prep.cu cuts long sequences into segments then.  S itself is kept and decayed in fp32 registers; only
 // its pieces are rewritten every chunk.
-// A token whose R is infinite or NaN in some column takes part as zero there (as do rows of T: GdrGates::bad), for a zero of T or P times NaN
+// A token whose R is infinite or NaN in some column takes part as zero there (as do entries of A and T: GdrGates::bad), for a zero of T or P times NaN
 // would reach the tokens before it; `bad` holds the first such token of each column, and from it on the
 // outputs of the chunk and the state behind it are NaN in that column.
 // kKeep: the backward's walk, which leaves S and U of every chunk in its record instead of an output.

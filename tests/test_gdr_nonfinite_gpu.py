@@ -1,0 +1,26 @@
+"""Infinities, NaN and overflow in the gated delta rule: which outputs and gradients they reach, and which stay as they are."""
+import pytest
+import torch
+
+import gdr_ref
+from conftest import DT
+
+pytestmark = pytest.mark.gpu
+
+
+def large_keys(k, at, head, size=1e20):
+    """Tokens at .. at + 3 with one direction of length `size`: at 1e20 their products with each other leave float32."""
+    k[..., at:at + 4, head, :] = size * k[..., at:at + 1, head, :].clone()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_keys_whose_products_overflow(dtype):
+    """k_i.k_j is infinite though k, v and the first product with the state are not."""
+    import causal_conv1d_b200 as cc
+    q, k, v, g, beta = gdr_ref.inputs((64,), 2, 2, 32, 32, DT[dtype], seed=12)
+    cu = torch.tensor([0, 64], dtype=torch.int32).cuda()
+    clean = cc.gated_delta_rule_varlen_fn(q, k, v, g, beta, cu_seqlens=cu)
+    large_keys(k, 30, 1)
+    got = cc.gated_delta_rule_varlen_fn(q, k, v, g, beta, cu_seqlens=cu)
+    assert torch.equal(got[:, 0], clean[:, 0]) and torch.equal(got[:30, 1], clean[:30, 1])
+    assert not torch.isfinite(got[31:, 1]).any()
