@@ -44,7 +44,7 @@ template <typename T, bool kBack> struct Fwd {
 // (33 cycles an instruction of 64 columns, 66 of 128), and the rest fills 47 % of the issue slots.  One sequence
 // and head a CTA, so few heads leave SMs idle: cc1d_gdr_prep.cu cuts long sequences into segments then.  S itself is kept and decayed in fp32 registers; only
 // its pieces are rewritten every chunk.
-// A token whose R is infinite or NaN in some column takes part as zero there (as do entries of A and T: GdrGates::bad), for a zero of T or P times NaN
+// A token whose R or U is infinite or NaN in some column takes part as zero there (as do entries of A and T: GdrGates::bad), for a zero of T or P times NaN
 // would reach the tokens before it; `bad` holds the first such token of each column, and from it on the
 // outputs of the chunk and the state behind it are NaN in that column.
 // kKeep: the backward's walk, which leaves S and U of every chunk in its record instead of an output.
@@ -306,6 +306,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     const float2 v = add2(make_float2(x[j], x[j + 1]), make_float2(R[j], R[j + 1]));
                     x[j] = v.x; x[j + 1] = v.y;
                 }
+                if (kOut) only_finite(x, first, par);     // (a finite R may overflow with T)
                 if (kMode == kKeep) {
                     #pragma unroll
                     for (int j = 0; j < 16; ++j) record->U[first + j][col] = x[j];

@@ -24,3 +24,18 @@ def test_keys_whose_products_overflow(dtype):
     got = cc.gated_delta_rule_varlen_fn(q, k, v, g, beta, cu_seqlens=cu)
     assert torch.equal(got[:, 0], clean[:, 0]) and torch.equal(got[:30, 1], clean[:30, 1])
     assert not torch.isfinite(got[31:, 1]).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_what_a_token_writes_overflows(dtype):
+    """Keys of 1e19 over a state of order one: T and R are finite, T R is not, and the tokens before keep their bits."""
+    import causal_conv1d_b200 as cc
+    q, k, v, g, beta = gdr_ref.inputs((64,), 2, 2, 32, 32, DT[dtype], seed=14, slow=True)
+    cu = torch.tensor([0, 64], dtype=torch.int32).cuda()
+    first = torch.randn(1, 2, 32, 32, generator=torch.Generator().manual_seed(15)).cuda()
+    run = lambda: cc.gated_delta_rule_varlen_fn(q, k, v, g, beta, cu_seqlens=cu, states=first, update_states=False)  # noqa: E731
+    clean = run()
+    large_keys(k, 30, 1, 1e19)
+    got = run()
+    assert torch.equal(got[:, 0], clean[:, 0]) and torch.equal(got[:30, 1], clean[:30, 1])
+    assert not torch.isfinite(got[32:, 1]).any()
