@@ -325,7 +325,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             }
             ready(bar_w);
             const float whole = gates.from_start[kChunk - 1];
-            const int bad_row = kOut ? gates.bad : kChunk;
+            const int bad_row = kMode == kKeep ? kChunk : gates.bad;
             gdr_wait(bar_d, par, dead);
             __syncwarp();
             fence_after_sync();
@@ -344,8 +344,8 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             fence_before_sync();
             walk_sync<kWalkers>();                      // every thread has read its part of Delta
             fence_after_sync();
-            const int bad_from = kOut ? min(bad[par * kGdrMaxDim], bad_row) : kChunk;
-            if (kOut && bad_from < kChunk) {
+            const int bad_from = kOut ? min(bad[par * kGdrMaxDim], bad_row) : bad_row;
+            if (kMode != kKeep && bad_from < kChunk) {
                 #pragma unroll
                 for (int j = 0; j < 32; ++j) S[j] = __uint_as_float(0x7fc00000u);
             }

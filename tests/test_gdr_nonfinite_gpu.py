@@ -39,3 +39,21 @@ def test_what_a_token_writes_overflows(dtype):
     got = run()
     assert torch.equal(got[:, 0], clean[:, 0]) and torch.equal(got[:30, 1], clean[:30, 1])
     assert not torch.isfinite(got[32:, 1]).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_overflow_passes_from_segment_to_segment(dtype):
+    """A long sequence of few heads is walked in segments: the ones behind the overflow know of it, and the last state."""
+    import causal_conv1d_b200 as cc
+    q, k, v, g, beta = gdr_ref.inputs((4000,), 2, 2, 64, 32, DT[dtype], seed=13, slow=True)
+    cu = torch.tensor([0, 4000], dtype=torch.int32).cuda()
+
+    def run(k):
+        states = torch.zeros(1, 2, 64, 32, device="cuda")
+        return cc.gated_delta_rule_varlen_fn(q, k, v, g, beta, cu_seqlens=cu, states=states), states
+
+    clean, state = run(k)
+    large_keys(k, 1000, 1)
+    got, last = run(k)
+    assert torch.equal(got[:, 0], clean[:, 0]) and torch.equal(got[:1000, 1], clean[:1000, 1]) and torch.equal(last[:, 0], state[:, 0])
+    assert not torch.isfinite(got[1001:, 1]).any() and not torch.isfinite(last[:, 1]).any()
