@@ -408,6 +408,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
     const uint32_t base = smem_u32(smem), bar = base + L::kBars, bar_state = bar + 8;
     const GdrGates &gates = *reinterpret_cast<const GdrGates *>(smem + L::kGates);
     float(*dots)[4][128] = reinterpret_cast<float(*)[4][128]>(smem + L::kDots);
+    // first token whose gradients of q, k, g and beta are NaN, of a head and of the group (a place that no sum takes)
+    int *bad = reinterpret_cast<int *>(&dots[2][2][0]);
     volatile int *dead = reinterpret_cast<volatile int *>(smem + L::kBars + 16);
     uint32_t *tmem_at = reinterpret_cast<uint32_t *>(smem + L::kBars + 20);
     const int tid = threadIdx.x, warp = __shfl_sync(kFullMask, tid >> 5, 0), lane = tid & 31;
@@ -459,6 +461,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
         if (tid < 192) {
             const uint4 *src = reinterpret_cast<const uint4 *>(images + (slot * heads + h) * (int64_t)S::kImage + S::kGates - S::kT);
             sts128(base + L::kGates + 16 * tid, src[tid]);
+        } else if (tid == 192) {
+            const int4 v = *reinterpret_cast<const int4 *>(record.bad);
+            bad[0] = min(min(v.x, v.y), min(v.z, v.w));
+            bad[1] = h == hk * group ? bad[0] : min(bad[0], bad[1]);
         }
         __syncthreads();
         const T *dout = reinterpret_cast<const T *>(b.dout) + seq.row * b.dout_batch_stride + h * b.dout_h_stride;
@@ -734,8 +740,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
                 const int64_t t = t0 + 2 * lane + e;
                 if (t < seq.end) {
                     const int64_t at = (seq.row * p.seqlen + t) * heads + h;
-                    store_any(b.dg, at, p.gtype, (e == 0 ? sum : sum - d[0]) + end);
-                    store_any(b.dbeta, at, p.btype, db[e]);
+                    const bool lost = 2 * lane + e >= bad[0];
+                    store_any(b.dg, at, p.gtype, lost ? __uint_as_float(0x7fc00000u) : (e == 0 ? sum : sum - d[0]) + end);
+                    store_any(b.dbeta, at, p.btype, lost ? __uint_as_float(0x7fc00000u) : db[e]);
                 }
             }
         }
@@ -743,6 +750,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
     }
     {
         const int64_t t = t0 + i;
+        if (i >= bad[1]) {
+            #pragma unroll
+            for (int j = 0; j < 32; ++j) total[j] = __uint_as_float(0x7fc00000u);
+        }
         T *dst = reinterpret_cast<T *>(is_k ? b.dk : b.dq) + ((seq.row * p.seqlen + t) * heads_k + hk) * dk + 32 * part;
         #pragma unroll
         for (int e = 0; e < 4; ++e)

@@ -363,6 +363,7 @@ __device__ __forceinline__ void feed_walk(const GdrRows<T, kFeeders> &rows, cons
 // it, U, the gradient of the state behind it, and the gradient dB of R.
 struct GdrRecord {
     float S0[kGdrMaxDim][kGdrMaxDim], U[kChunk][kGdrMaxDim], dS[kGdrMaxDim][kGdrMaxDim], dB[kChunk][kGdrMaxDim];
+    int bad[32];              // first token that is not finite in columns 32 i .. (64: none), i < 4; the rest keeps records 128-byte aligned
 };
 // ---- long sequences of few heads ------------------------------------------------------------------
 // A walk is one chain of chunks; where there are too few of them for the SMs, sequences are cut into segments

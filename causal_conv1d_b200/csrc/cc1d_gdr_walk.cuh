@@ -47,12 +47,13 @@ template <typename T, bool kBack> struct Fwd {
 // A token whose R or U is infinite or NaN in some column takes part as zero there (as do entries of A and T: GdrGates::bad), for a zero of T or P times NaN
 // would reach the tokens before it; `bad` holds the first such token of each column, and from it on the
 // outputs of the chunk and the state behind it are NaN in that column.
-// kKeep: the backward's walk, which leaves S and U of every chunk in its record instead of an output.
+// kKeep: the backward's walk, which leaves S, U and the first bad token of every chunk in its record instead of an
+// output.  The gradients of the tokens before that one do not depend on what stands in its place.
 // kSummary: what a segment does to the state: from zeros its last state B, or (unit) without values from the
 // identity, dim_k columns instead of dim_v, its M.
 template <typename T, int kSteps, GdrMode kMode, bool kBack>
 __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const unsigned char *images, GdrRecord *records, const GdrSegments &segs, int64_t block, bool unit) {
-    constexpr bool kOut = kMode == kOutput;
+    constexpr bool kOut = kMode == kOutput, kFinite = kMode != kSummary;
     using L = Fwd<T, kBack>;
     using St = GdrStage<T, kBack>;
     constexpr int NP = St::kPieces, PO = GdrType<T>::kOutPieces, PT = St::kSolve;
@@ -231,14 +232,18 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
         }
         // first token of a chunk whose value is not finite, by column; chunks use the two rows in turn
         int *bad = reinterpret_cast<int *>(smem + L::kBad) + col;
-        if (kOut && part < 2) bad[part * kGdrMaxDim] = kChunk;
-        if (kOut) walk_sync<kWalkers>();
-        auto only_finite = [&](float (&x)[16], int first, int par) {
+        if (kFinite && part < 2) bad[part * kGdrMaxDim] = kChunk;
+        if (kFinite) walk_sync<kWalkers>();
+        auto only_finite = [&](float (&x)[16], int first, int step, int par) {
             if (!all_finite(x)) {
+                uint32_t out = 0;
                 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    if (!finite(x[j])) { atomicMin(bad + par * kGdrMaxDim, first + j); x[j] = 0.f; }
+                    const bool ok = finite(x[j]);
+                    out |= ok ? 0u : 1u << j;
+                    x[j] = ok ? x[j] : 0.f;
                 }
+                if (out != 0) atomicMin(bad + par * kGdrMaxDim, first + step * (__ffs(out) - 1));
             }
             __syncwarp();
         };
@@ -289,7 +294,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     const float2 v = fma2(make_float2(f.z, f.w), make_float2(x[j + 2], x[j + 3]), make_float2(R[j + 2], R[j + 3]));
                     R[j] = u.x; R[j + 1] = u.y; R[j + 2] = v.x; R[j + 3] = v.y;
                 }
-                if (kOut) only_finite(R, first, par);
+                if (kFinite) only_finite(R, first, 1, par);
                 #pragma unroll
                 for (int j = 0; j < 16; j += 8) split8_to_tmem<PT>(R + j, mine + kFwdColR + first / 2 + j / 2, 32, 64);
             }
@@ -306,7 +311,8 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     const float2 v = add2(make_float2(x[j], x[j + 1]), make_float2(R[j], R[j + 1]));
                     x[j] = v.x; x[j + 1] = v.y;
                 }
-                if (kOut) only_finite(x, first, par);     // (a finite R may overflow with T)
+                // (a finite R may overflow with T; the gradients then have no token to begin with)
+                if (kFinite) only_finite(x, kOut ? first : 0, kOut ? 1 : 0, par);
                 if (kMode == kKeep) {
                     #pragma unroll
                     for (int j = 0; j < 16; ++j) record->U[first + j][col] = x[j];
@@ -325,7 +331,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
             }
             ready(bar_w);
             const float whole = gates.from_start[kChunk - 1];
-            const int bad_row = kMode == kKeep ? kChunk : gates.bad;
+            const int bad_row = gates.bad;
             gdr_wait(bar_d, par, dead);
             __syncwarp();
             fence_after_sync();
@@ -340,12 +346,12 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     S[16 * b + j] = v.x; S[16 * b + j + 1] = v.y;
                 }
             }
-            if (kOut && part == 0) bad[(par ^ 1) * kGdrMaxDim] = kChunk;      // (all are done with the chunk before)
+            if (kFinite && part == 0) bad[(par ^ 1) * kGdrMaxDim] = kChunk;      // (all are done with the chunk before)
             fence_before_sync();
             walk_sync<kWalkers>();                      // every thread has read its part of Delta
             fence_after_sync();
-            const int bad_from = kOut ? min(bad[par * kGdrMaxDim], bad_row) : bad_row;
-            if (kMode != kKeep && bad_from < kChunk) {
+            const int bad_from = kFinite ? min(bad[par * kGdrMaxDim], bad_row) : bad_row;
+            if (bad_from < kChunk) {
                 #pragma unroll
                 for (int j = 0; j < 32; ++j) S[j] = __uint_as_float(0x7fc00000u);
             }
@@ -356,6 +362,10 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 fence_after_sync();
             }
             if (c + 1 < chunks) put_state();
+            if (kMode == kKeep && part == 0) {
+                const int least = __reduce_min_sync(kFullMask, bad_from);
+                if (lane == 0) record[-heads].bad[quad] = least;      // (record: the next chunk's)
+            }
             // the output, while the next chunk's first product runs
             if (kOut) {
                 gdr_wait(bar_o, par, dead);

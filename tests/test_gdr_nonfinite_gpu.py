@@ -57,3 +57,52 @@ def test_overflow_passes_from_segment_to_segment(dtype):
     got, last = run(k)
     assert torch.equal(got[:, 0], clean[:, 0]) and torch.equal(got[:1000, 1], clean[:1000, 1]) and torch.equal(last[:, 0], state[:, 0])
     assert not torch.isfinite(got[1001:, 1]).any() and not torch.isfinite(last[:, 1]).any()
+
+
+NAMES = ["dq", "dk", "dv", "dg", "dbeta"]
+
+
+def gradients(leaves, S0, cu, dout, dfinal):
+    import causal_conv1d_b200 as cc
+    every = [t.detach().requires_grad_() for t in (*leaves, S0)]
+    out, last = cc.gated_delta_rule_fn(*every[:5], initial_state=every[5], return_final_state=True, cu_seqlens=cu)
+    return torch.autograd.grad((out, last), every, (dout, dfinal))
+
+
+def training(T, hk, hv, dtype, seed, tail_from=None):
+    """A sequence of T tokens and one of 20 behind it; tail_from: a padded end without an output's gradient."""
+    leaves = gdr_ref.inputs((1, T + 20), hk, hv, 64, 32, DT[dtype], seed=seed, slow=True)
+    gen = torch.Generator().manual_seed(seed)
+    S0, dfinal = (torch.randn(2, hv, 64, 32, generator=gen).cuda() for _ in range(2))
+    dout = torch.randn(1, T + 20, hv, 32, generator=gen).to(DT[dtype]).cuda()
+    if tail_from is not None:
+        dout[:, tail_from:T] = 0
+        dfinal[0] = 0
+    return leaves, S0, torch.tensor([0, T, T + 20], dtype=torch.int32).cuda(), dout, dfinal
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype,T,t,tail", [("bf16", 64, 30, False), ("fp32", 200, 64, False), ("fp16", 200, 127, True), ("bf16", 150, 100, True),
+                                            ("bf16", 90, 0, False), ("bf16", 2500, 1300, True)])
+def test_a_value_that_is_not_finite_leaves_the_gradients_before_it(value, dtype, T, t, tail):
+    """v of one token and column.  What the recurrence sends back (dS, dB) is made of q, k, g, beta and the outputs' gradients
+    alone, so neither dv nor the first state's gradient depends on v, nor does any gradient of a token before: they are those
+    of the run with a finite value there.  From the token on the gradients of q, k, g and beta are NaN.  2500 tokens are
+    walked in segments."""
+    leaves, *rest = training(T, 1, 2, dtype, T + t, t if tail else None)
+    clean = gradients(leaves, *rest)
+    leaves[2][0, t, 1, 5] = value
+    got = gradients(leaves, *rest)
+    for name, a, c in zip(NAMES, got, clean):
+        if name == "dv":
+            assert torch.equal(a, c)
+            continue
+        assert torch.equal(a[0, T:], c[0, T:]), f"{name}: another sequence"
+        if name in ("dg", "dbeta"):
+            assert torch.equal(a[..., 0], c[..., 0]), f"{name}: another head"
+            a, c = a[..., 1], c[..., 1]
+        # dg is a sum over the chunk's later tokens too, in which the value's part cancels: equal but for its roundings
+        # (at most 64 terms of the size of the largest: 64 * 2^-24 = 4e-6)
+        gdr_ref.close(a[0, :t], c[0, :t], 4e-6 if name == "dg" else 0, f"{name} before")
+        assert torch.isnan(a[0, t:T]).all(), f"{name}: from the token on"
+    assert torch.equal(got[5], clean[5])
