@@ -369,6 +369,13 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
     }
     fence_proxy_async_smem();
     __syncthreads();
+    if (kBack && gates.bad < kChunk) {
+        // what goes back through an entry that was left out is not finite either: with this factor dB of the chunk, and with it
+        // the gradient of every state before, is NaN (and the state behind, as it is in the forward)
+        if (tid < kChunk) gates.to_end[tid] = __uint_as_float(0x7fc00000u);
+        fence_proxy_async_smem();
+        __syncthreads();
+    }
     if (tid == 0) {
         unsigned char *image = images + (slot * heads + h) * (int64_t)S::kImage;
         bulk_store(image, base, S::kSolve * 8192);

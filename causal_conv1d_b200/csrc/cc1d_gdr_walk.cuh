@@ -234,7 +234,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
         int *bad = reinterpret_cast<int *>(smem + L::kBad) + col;
         if (kFinite && part < 2) bad[part * kGdrMaxDim] = kChunk;
         if (kFinite) walk_sync<kWalkers>();
-        auto only_finite = [&](float (&x)[16], int first, int step, int par) {
+        auto only_finite = [&](float (&x)[16], int first, int par) {
             if (!all_finite(x)) {
                 uint32_t out = 0;
                 #pragma unroll
@@ -243,7 +243,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     out |= ok ? 0u : 1u << j;
                     x[j] = ok ? x[j] : 0.f;
                 }
-                if (out != 0) atomicMin(bad + par * kGdrMaxDim, first + step * (__ffs(out) - 1));
+                if (out != 0) atomicMin(bad + par * kGdrMaxDim, first + __ffs(out) - 1);
             }
             __syncwarp();
         };
@@ -294,7 +294,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     const float2 v = fma2(make_float2(f.z, f.w), make_float2(x[j + 2], x[j + 3]), make_float2(R[j + 2], R[j + 3]));
                     R[j] = u.x; R[j + 1] = u.y; R[j + 2] = v.x; R[j + 3] = v.y;
                 }
-                if (kFinite) only_finite(R, first, 1, par);
+                if (kFinite) only_finite(R, first, par);
                 #pragma unroll
                 for (int j = 0; j < 16; j += 8) split8_to_tmem<PT>(R + j, mine + kFwdColR + first / 2 + j / 2, 32, 64);
             }
@@ -311,8 +311,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                     const float2 v = add2(make_float2(x[j], x[j + 1]), make_float2(R[j], R[j + 1]));
                     x[j] = v.x; x[j + 1] = v.y;
                 }
-                // (a finite R may overflow with T; the gradients then have no token to begin with)
-                if (kFinite) only_finite(x, kOut ? first : 0, kOut ? 1 : 0, par);
+                if (kFinite) only_finite(x, first, par);     // (a finite R may overflow with T)
                 if (kMode == kKeep) {
                     #pragma unroll
                     for (int j = 0; j < 16; ++j) record->U[first + j][col] = x[j];

@@ -106,3 +106,23 @@ def test_a_value_that_is_not_finite_leaves_the_gradients_before_it(value, dtype,
         gdr_ref.close(a[0, :t], c[0, :t], 4e-6 if name == "dg" else 0, f"{name} before")
         assert torch.isnan(a[0, t:T]).all(), f"{name}: from the token on"
     assert torch.equal(got[5], clean[5])
+
+
+@pytest.mark.parametrize("dtype,T,t", [("bf16", 64, 30), ("fp32", 200, 100), ("bf16", 2500, 1300)])
+def test_overflowed_keys_in_the_backward(dtype, T, t):
+    """Keys whose products leave float32: what goes back through them is not finite, where it does not pass them it is
+    as it was (dq of the tokens before, the other head, the other sequence)."""
+    leaves, *rest = training(T, 2, 2, dtype, T + t + 1)
+    clean = gradients(leaves, *rest)
+    large_keys(leaves[1], t, 1)
+    got = gradients(leaves, *rest)
+    for name, a, c in zip(NAMES, got, clean):
+        assert torch.equal(a[0, T:], c[0, T:]), f"{name}: another sequence"
+        assert torch.equal(a[0, :, 0], c[0, :, 0]), f"{name}: another head"
+        if name == "dq":
+            assert torch.equal(a[0, :t, 1], c[0, :t, 1])
+        else:
+            assert not torch.isfinite(a[0, :t, 1]).any(), f"{name} before"
+        if name != "dv":
+            assert not torch.isfinite(a[0, t + 1:T, 1]).any(), f"{name} behind"
+    assert torch.equal(got[5][0, 0], clean[5][0, 0]) and not torch.isfinite(got[5][0, 1]).any()
