@@ -59,7 +59,7 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
     // what the walkers need again at their end (kept in registers over the walk it makes them spill)
     volatile GdrPart *kept = reinterpret_cast<volatile GdrPart *>(smem + L::kBars + 128);
     if (tid == 0) {
-        kept->n = w.n; kept->seq.end = w.seq.end; kept->segment = w.segment; kept->first = w.first; kept->last = w.last;
+        kept->n = w.n; kept->seq.begin = w.seq.begin; kept->seq.end = w.seq.end; kept->segment = w.segment; kept->first = w.first; kept->last = w.last;
         for (int s = 0; s < 2; ++s) { mbar_init(bar_full + 8 * s, kFeeders + 1); mbar_init(bar_empty + 8 * s, kWalkers / 32); }
         mbar_init(bar_x, 1); mbar_init(bar_u, 1); mbar_init(bar_d, 1);
         mbar_init(bar_s, kWalkers / 32); mbar_init(bar_e, kWalkers / 32); mbar_init(bar_r, kWalkers / 32); mbar_init(bar_w, kWalkers / 32);
@@ -303,10 +303,9 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
             for (int j = 0; j < 32; ++j)
                 if (32 * part + j < dk && col < dv) b.dinitial_states[state_at + (int64_t)j * dv] = from ? S[j] : 0.f;
         }
-        // tokens that belong to no sequence
-        if (!kSum && kept->last && p.cu_seqlens != nullptr && at + 1 >= all) {
+        if (!kSum && p.cu_seqlens != nullptr) {
             const int group = heads / (int)p.heads_k;
-            for (int64_t t = kept->seq.end + part; t < p.seqlen; t += 4) {
+            unowned_tokens(p, kept, part, [&](int64_t t) {
                 if (col < dv) reinterpret_cast<T *>(b.dv)[(t * heads + head) * dv + col] = Elem<T>::from_f(0.f);
                 if (head % group == 0 && col < dk) {
                     reinterpret_cast<T *>(b.dq)[(t * p.heads_k + head / group) * dk + col] = Elem<T>::from_f(0.f);
@@ -316,7 +315,7 @@ __device__ __forceinline__ void walk_back(const cc1d_gdr_bwd_params &b, const un
                     store_any(b.dg, t * heads + head, p.gtype, 0.f);
                     store_any(b.dbeta, t * heads + head, p.btype, 0.f);
                 }
-            }
+            });
         }
     }
     fence_before_sync();

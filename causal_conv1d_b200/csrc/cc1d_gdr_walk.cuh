@@ -24,6 +24,17 @@ template <int kOutPieces> __device__ __forceinline__ constexpr uint32_t col_s(in
     return piece < 2 ? kFwdColS + 64 * piece : kOutPieces < 3 ? kFwdColR : kFwdColU;
 }
 
+// Tokens of a packed row that belong to no sequence, every fourth from `part` on: those before the first sequence, by the
+// walk that begins it, and those behind the last one, by the walk that ends it.
+template <typename F> __device__ __forceinline__ void unowned_tokens(const cc1d_gdr_params &p, const volatile GdrPart *w, int part, F &&f) {
+    if (w->n == 0 && w->first) {
+        for (int64_t t = part; t < w->seq.begin; t += 4) f(t);
+    }
+    if (w->n + 1 >= (int)gdr_sequences(p) && w->last) {
+        for (int64_t t = w->seq.end + part; t < p.seqlen; t += 4) f(t);
+    }
+}
+
 enum GdrMode { kOutput, kKeep, kSummary };
 template <typename T, bool kBack> struct Fwd {
     using S = GdrStage<T, kBack>;
@@ -76,7 +87,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
     // what the walkers need again at their end (kept in registers over the walk it makes them spill)
     volatile GdrPart *kept = reinterpret_cast<volatile GdrPart *>(smem + L::kPart);
     if (tid == 0) {
-        kept->n = w.n; kept->seq.end = w.seq.end; kept->segment = w.segment; kept->last = w.last;
+        kept->n = w.n; kept->seq.begin = w.seq.begin; kept->seq.end = w.seq.end; kept->segment = w.segment; kept->first = w.first; kept->last = w.last;
         for (int s = 0; s < 2; ++s) { mbar_init(bar_full + 8 * s, kFeeders + 1); mbar_init(bar_empty + 8 * s, 1); }
         mbar_init(bar_x, 1); mbar_init(bar_u, 1); mbar_init(bar_o, 1); mbar_init(bar_d, 1);
         mbar_init(bar_s, kWalkers / 32); mbar_init(bar_r, kWalkers / 32); mbar_init(bar_w, kWalkers / 32); mbar_init(bar_out, kWalkers / 32);
@@ -412,12 +423,10 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                 #pragma unroll
                 for (int j = 0; j < 32; ++j) if (32 * part + j < dk && col < dv) dst[(int64_t)j * dv] = S[j];
             }
-            // tokens that belong to no sequence
-            if (p.cu_seqlens != nullptr && at + 1 >= all) {
-                T *out = reinterpret_cast<T *>(p.out) + head * p.out_h_stride + col;
-                for (int64_t t = kept->seq.end + part; t < p.seqlen; t += 4)
-                    if (col < dv) out[t * p.out_l_stride] = Elem<T>::from_f(0.f);
-            }
+        }
+        if (kOut && p.cu_seqlens != nullptr) {
+            T *out = reinterpret_cast<T *>(p.out) + head * p.out_h_stride + col;
+            unowned_tokens(p, kept, part, [&](int64_t t) { if (col < dv) out[t * p.out_l_stride] = Elem<T>::from_f(0.f); });
         }
     }
     fence_before_sync();

@@ -94,7 +94,8 @@ def gated_delta_rule_fn(
         (-inf: the state is forgotten)
     initial_state: (sequences, heads_v, dim_k, dim_v) float32; zeros when None
     cu_seqlens: (nseq + 1,) int32: the one row of the batch holds nseq packed sequences, sequence s at
-        tokens cu_seqlens[s]:cu_seqlens[s+1]; tokens behind the last one have zero outputs and gradients
+        tokens cu_seqlens[s]:cu_seqlens[s+1]; tokens before the first and behind the last one have zero
+        outputs and gradients
     scale: factor of the output, dim_k ** -0.5 when None
 
     out: (batch, seqlen, heads_v, dim_v); with return_final_state also (sequences, heads_v, dim_k, dim_v)
@@ -157,7 +158,7 @@ def gated_delta_rule_varlen_fn(
         q, k: (total_tokens, heads_k, dim_k); sequence s owns rows cu_seqlens[s]:cu_seqlens[s+1]
         v: (total_tokens, heads_v, dim_v), dtype of q
         g, beta: (total_tokens, heads_v), float32, float16 or bfloat16; g: logarithm of the decay
-        cu_seqlens: (nseq + 1,) int32, non-decreasing from 0, its last entry at most total_tokens
+        cu_seqlens: (nseq + 1,) int32, non-decreasing, its last entry at most total_tokens
         states: (rows, heads_v, dim_k, dim_v) float32, dense in its last two dimensions, or None.
             Row r = state_indices[s] (s when state_indices is None) holds sequence s's state. An
             index that is negative or not below the number of rows: the sequence starts from
@@ -167,7 +168,7 @@ def gated_delta_rule_varlen_fn(
         update_states: write each sequence's last state back into its row of states (in place).
         scale: factor of the output, dim_k ** -0.5 when None
     Return:
-        out: (total_tokens, heads_v, dim_v); tokens at or after cu_seqlens[-1] are zero
+        out: (total_tokens, heads_v, dim_v); tokens before cu_seqlens[0], and at or after cu_seqlens[-1], are zero
     """
     q, k, v, g, beta = (t.unsqueeze(0) for t in (q, k, v, g, beta))
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)

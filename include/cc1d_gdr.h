@@ -31,8 +31,9 @@ extern "C" {
  *
  * Sequences: `batch` rows of `seqlen` tokens, or (cu_seqlens != NULL) batch == 1 and nseq packed
  * sequences, sequence s owning tokens [cu_seqlens[s], cu_seqlens[s+1]) of the seqlen tokens;
- * tokens at or after cu_seqlens[nseq] output zero.  cu_seqlens is non-decreasing from 0 and its
- * last entry is at most seqlen (entries outside are clamped to that range).
+ * tokens before cu_seqlens[0] and at or after cu_seqlens[nseq] get zero outputs and gradients.
+ * cu_seqlens is non-decreasing and its last entry is at most seqlen (entries outside [0, seqlen] are
+ * clamped).
  * State rows: r = state_indices ? state_indices[n] : n for sequence (row) n.  A row at or
  * above state_rows counts as a negative index.  No two sequences may name the same row of
  * final_states.

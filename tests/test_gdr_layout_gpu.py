@@ -51,3 +51,27 @@ def test_gradient_that_is_a_slice_of_a_flat_one():
     out = cc.gated_delta_rule_fn(*leaves)
     for a, b in zip(got, torch.autograd.grad(out, leaves, flat[1:].clone().view(out.shape))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("heads", [2, 160])
+@pytest.mark.parametrize("lens", [[70, 35], [1, 4000], [5, 0, 64], [130]])
+def test_tokens_before_the_first_sequence(lens, heads):
+    """cu_seqlens that does not start at 0: zero outputs and gradients there, as behind the last sequence; 2 heads of 4000 tokens
+    are walked in segments."""
+    import causal_conv1d_b200 as cc
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)[1:].cuda()            # lens[0] tokens in front
+    begin, end = int(cu[0]), int(cu[-1])
+    leaves = [t.requires_grad_() for t in gdr_ref.inputs((1, end + 9), heads // 2, heads, 32, 32, torch.bfloat16)]
+    junk = [torch.full((1 << 25,), float("nan"), device="cuda") for _ in range(4)]
+    del junk                                                                      # what torch.empty may hand out
+    out = cc.gated_delta_rule_fn(*leaves, cu_seqlens=cu)
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    for t in (out, *grads):
+        assert not t[:, :begin].any() and not t[:, end:].any()
+    part = [t.detach()[:, begin:end].clone().requires_grad_() for t in leaves]
+    if end > begin:
+        want = cc.gated_delta_rule_fn(*part, cu_seqlens=cu - begin)
+        for a, b in zip((out, *grads), (want, *torch.autograd.grad(want, part, torch.ones_like(want)))):
+            assert torch.equal(a[:, begin:end], b)
+    packed = cc.gated_delta_rule_varlen_fn(*(t.detach()[0] for t in leaves), cu_seqlens=cu)
+    assert torch.equal(packed, out[0])
