@@ -191,7 +191,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
                         for (int i = 0; i < 4; ++i) mma_ts(kFwdColY, col_u(a) + 8 * i, desc_add(kq, St::kP + b * 8192 + 32 * i), id, again(more));
                     }
                 }
-                mma_commit(bar_o);
+                if (kOut) mma_commit(bar_o);        // (an arrival that nothing waits for could come when the CTA is gone)
             }
             __syncwarp();
         }
