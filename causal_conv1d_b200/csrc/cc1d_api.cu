@@ -92,7 +92,8 @@ bool make_channel_last_tensor_map(CUtensorMap *map, int dtype, const void *base,
     if (encode == nullptr) return false;
     const int es = elem_size(dtype);
     if (batch < 1) batch = 1;
-    if (batch == 1 || batch_stride <= 0) batch_stride = l_stride * seqlen;   // unused extent: any legal stride
+    if (batch == 1) batch_stride = l_stride * seqlen;                        // unused extent: any legal stride
+    if (l_stride <= 0 || batch_stride <= 0) return false;                    // expanded tensors: by their strides, without a map
     const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)seqlen, (cuuint64_t)batch};
     const cuuint64_t strides[2] = {(cuuint64_t)l_stride * es, (cuuint64_t)batch_stride * es};   // bytes, dims 1..2
     const cuuint32_t box[3] = {(cuuint32_t)(row_bytes / es), (cuuint32_t)kTmaRows, 1};
@@ -126,7 +127,7 @@ bool make_channel_first_tensor_map(CUtensorMap *map, int dtype, const void *base
     if (encode == nullptr) return false;
     const int es = elem_size(dtype);
     if (batch < 1) batch = 1;
-    if (batch == 1 || batch_stride <= 0) batch_stride = c_stride * dim;      // unused extent: any legal stride
+    if (batch == 1) batch_stride = c_stride * dim;                           // unused extent: any legal stride
     if (c_stride <= 0 || batch_stride <= 0) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)seqlen, (cuuint64_t)dim, (cuuint64_t)batch};
     const cuuint64_t strides[2] = {(cuuint64_t)c_stride * es, (cuuint64_t)batch_stride * es};   // bytes, dims 1..2
