@@ -30,7 +30,7 @@ class CausalConv1dFn(torch.autograd.Function):
             raise NotImplementedError("activation must be None, silu, or swish")
         if checkpoint not in _CHECKPOINTS:
             raise NotImplementedError("checkpoint must be None or e4m3")
-        if not _unit_inner_stride(x):
+        if not _unit_inner_stride(x) or (x.stride(2) == 0 and x.shape[2] > 1):     # (0: one token expanded over the sequence)
             x = x.contiguous()
         if bias is not None:
             bias = bias.contiguous()

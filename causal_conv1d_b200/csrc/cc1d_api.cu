@@ -162,6 +162,7 @@ int check_conv_common(int itype, int wtype, int width, int64_t batch, int64_t di
     if (x_ls != 1 && x_cs != 1) return CC1D_ERR_STRIDE;
     if (!elem_aligned(x, itype) || !elem_aligned(weight, wtype)) return CC1D_ERR_ALIGN;
     *channel_last = x_cs == 1 && x_ls > 1;
+    if (!*channel_last && x_ls != 1 && seqlen > 1) return CC1D_ERR_STRIDE;      // one token expanded over the sequence
     if (*channel_last) {
         if (dim % 8 != 0) return CC1D_ERR_CL_DIM;
         if (x_ls % 8 != 0 || (batch > 1 && x_bs % 8 != 0)) return CC1D_ERR_CL_STRIDE;

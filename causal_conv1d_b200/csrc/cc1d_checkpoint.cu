@@ -111,6 +111,7 @@ int code_args(CodeArgs &a, int itype, int64_t batch, int64_t dim, int64_t seqlen
     if (cs != 1 && ls != 1) return CC1D_ERR_STRIDE;
     if (seqlen >= (1ll << 31) - 4096 || dim >= (1ll << 31) - 4096) return CC1D_ERR_TOO_LARGE;
     const bool cl = channel_last(cs, ls);
+    if (!cl && ls != 1 && seqlen > 1) return CC1D_ERR_STRIDE;
     a.x = x; a.restored = const_cast<void *>(x);
     a.codes = c->codes; a.scales = c->scales;
     a.inner = (uint32_t)(cl ? seqlen : dim); a.cols = (uint32_t)(cl ? dim : seqlen);
