@@ -110,7 +110,7 @@ def causal_conv1d_fn(x, weight, bias=None, seq_idx=None, initial_states=None, re
         x itself. The output is what it is without; the backward sees x rounded to 4 significant
         bits (relative error at most 2^-4), which reaches dweight and, with an activation, dx and
         dbias. Saves memory where nothing else keeps x; x in a group with an infinity or a NaN
-        comes back as NaN.
+        comes back as NaN. Runs eagerly: torch.compile leaves a break in its graph here.
 
     out: (batch, dim, seqlen)
     """

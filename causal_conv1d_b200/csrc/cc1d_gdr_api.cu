@@ -1,4 +1,4 @@
-// extern "C" entry points of the gated delta rule (include/cc1d.h): validation and hand-off.
+// extern "C" entry points of the gated delta rule (include/cc1d_gdr.h): validation and hand-off.
 #include "cc1d.h"
 #include "cc1d_gdr.cuh"
 #include "cc1d_kernels.h"

@@ -1,4 +1,4 @@
-// Decode step of the gated delta rule: cc1d_gdr_update (include/cc1d.h).
+// Decode step of the gated delta rule: cc1d_gdr_update (include/cc1d_gdr.h).
 #include "cc1d_gdr.cuh"
 
 namespace cc1d {
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, kLanes == 16 ? 4 : 6) gdr_update_ker
     #pragma unroll
     for (int i = 0; i < kIter; ++i) {
         const int r = row0 + i * kWarps * kRows;
-                if (col_ok && r < dk) __stcs(reinterpret_cast<float4 *>(state + (int64_t)r * dv), S[i]);
+        if (col_ok && r < dk) __stcs(reinterpret_cast<float4 *>(state + (int64_t)r * dv), S[i]);
     }
 }
 

@@ -22,8 +22,11 @@ extern "C" {
  *
  * Value head h uses key head h / (heads_v / heads_k).  g = -inf forgets the state.  g is meant to be
  * at most 0: where positive ones add up to more than 88 over 64 tokens, e^sum leaves fp32 and the
- * tokens behind are NaN.  A token whose values are infinite or NaN gives NaN to itself and to those
- * behind it in its sequence and head (in the dim_v columns it touches), to none before.
+ * tokens behind are NaN.  A token whose values are infinite or NaN, or whose products leave fp32, gives
+ * NaN to the outputs of itself and of those behind it in its sequence and head (in the dim_v columns it
+ * touches), to none before.  In the backward a v that is not finite gives NaN to the gradients of q, k, g
+ * and beta from its token on, to none before, and not to dv and dinitial_states; any other value that is
+ * not finite may give NaN to all gradients of its sequence and head.
  * All sums and the state are fp32.  The tensor-core products split their fp32 factors into bf16
  * pieces: three (24 bits) of the state, of every factor of fp32 inputs and in the gradients of g
  * and beta; two (2^-17) of the chunk's U, P and of the correction (T - I) R where the result is

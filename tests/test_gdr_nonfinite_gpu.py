@@ -126,3 +126,13 @@ def test_overflowed_keys_in_the_backward(dtype, T, t):
         if name != "dv":
             assert not torch.isfinite(a[0, t + 1:T, 1]).any(), f"{name} behind"
     assert torch.equal(got[5][0, 0], clean[5][0, 0]) and not torch.isfinite(got[5][0, 1]).any()
+
+
+def test_a_gate_of_minus_infinity_in_the_backward():
+    """-inf forgets the state like any gate that takes e^g to 0: finite gradients, the same bits."""
+    leaves, *rest = training(150, 1, 2, "bf16", 7)
+    leaves[3][0, [0, 30, 64, 100], 1] = -1000.0
+    want = gradients(leaves, *rest)
+    leaves[3][0, [0, 30, 64, 100], 1] = -torch.inf
+    for a, b in zip(gradients(leaves, *rest), want):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
