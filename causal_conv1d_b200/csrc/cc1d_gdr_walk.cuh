@@ -246,7 +246,7 @@ __device__ __forceinline__ void walk_forward(const cc1d_gdr_params &p, const uns
         if (kFinite && part < 2) bad[part * kGdrMaxDim] = kChunk;
         if (kFinite) walk_sync<kWalkers>();
         auto only_finite = [&](float (&x)[16], int first, int par) {
-            if (!all_finite(x)) {
+            if (__builtin_expect(!all_finite(x), 0)) {
                 uint32_t out = 0;
                 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
