@@ -457,10 +457,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdr_grads_kernel(const __grid
 
     for (int h = hk * group; h < (hk + 1) * group; ++h) {
         const GdrRecord &record = records[slot * heads + h];
-        if (tid < 192) {
+        if (tid < (int)kGateBytes / 16) {
             const uint4 *src = reinterpret_cast<const uint4 *>(images + (slot * heads + h) * (int64_t)S::kImage + S::kGates - S::kT);
             sts128(base + L::kGates + 16 * tid, src[tid]);
-        } else if (tid == 192) {
+        } else if (tid == kGradThreads - 1) {
             const int4 v = *reinterpret_cast<const int4 *>(record.bad);
             bad[0] = min(min(v.x, v.y), min(v.z, v.w));
             bad[1] = h == hk * group ? bad[0] : min(bad[0], bad[1]);

@@ -239,15 +239,17 @@ namespace cc1d {
 //          gradients, has all three)
 // T, P and the gates are one image in the workspace, made by gdr_prep_kernel for all chunks at
 // once (inside the walk their chain of short dependent steps, 13,000 cycles a chunk, held it up).
-// The product with T is taken as x + (T - I) x, x in fp32: two pieces of both (16-bit types) then leave
-// 2^-17 of the correction alone, not of x.
+// The product with T is taken as x + (T - I) x, x in fp32: two pieces of both (the forward of 16-bit types) then leave
+// 2^-17 of the correction alone, not of x.  The backward has three in every type: the gradients of g, of beta and of
+// the state are fp32 (64 x 64 states of order one: 2.6e-6 of the largest off with two pieces, 5e-7 with three; both walks of
+// 64 chunks 380 -> 404 us).
 template <typename T, bool kBack> struct GdrStage {
-    static constexpr int kPieces = GdrType<T>::kPieces, kOut = kBack ? 3 : GdrType<T>::kOutPieces, kSolve = GdrType<T>::kSolve;
+    static constexpr int kPieces = GdrType<T>::kPieces, kOut = kBack ? 3 : GdrType<T>::kOutPieces, kSolve = kBack ? 3 : GdrType<T>::kSolve;
     static constexpr uint32_t kPanel = 128 * 128, kKqPiece = 2 * kPanel;     // panel: 128 rows x 64 columns
     static constexpr uint32_t kKq = 0, kV = kPieces * kKqPiece, kT = kV + kChunk * kGdrMaxDim * sizeof(T), kGates = kT + kSolve * 8192,
                               kP = kGates + 4096, kBytes = kP + kOut * 8192, kImage = kBytes - kT;
 };
-constexpr uint32_t kGateBytes = 3 * 1024;        // of the 4096 in an image, which align P
+constexpr uint32_t kGateBytes = 2688;            // of the 4096 in an image, which align P (the preparation has them in shared memory besides: 3072 would cost it a CTA an SM)
 static_assert(sizeof(GdrGates) <= kGateBytes, "gates of a chunk");
 
 // Chunks of sequence n in the workspace: slots gdr_first_slot(n) .. ; the slots of different sequences

@@ -457,8 +457,8 @@ __global__ void __launch_bounds__(256) gdr_join_kernel(const __grid_constant__ c
 }  // namespace
 
 // Times in us of a walk's chunk and of a join's step (measured, bf16, 128 x 128), for sequences of the mean length;
-// `back`: of the backward's walks as launches of their own.  (In the one launch that they share now a chunk takes 5.9
-// to 6.4, so the rule cuts a little less often than it could; and one long sequence among many short ones is not cut.)
+// `back`: of the backward's walks as launches of their own.  (In the one launch that they share now a chunk takes 6.3
+// to 6.8, so the rule cuts a little less often than it could; and one long sequence among many short ones is not cut.)
 // Cut where that is expected to save a quarter: one sequence of 32768 tokens and 4 heads, for example, is one
 // wave of 37 segments a head instead of 4 chains of 512 chunks.
 int gdr_plan_segments(const cc1d_gdr_params &p, bool back) {

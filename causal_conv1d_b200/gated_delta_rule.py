@@ -103,9 +103,9 @@ def gated_delta_rule_fn(
 
     out: (batch, seqlen, heads_v, dim_v); with return_final_state also (sequences, heads_v, dim_k, dim_v)
 
-    The backward computes the forward's states again; it needs about 236 KB of workspace (16-bit types;
-    244 KB for float32) for each 64 tokens of a value head while it runs, whatever dim_k and dim_v are: 1 GB for
-    8192 tokens of 32 heads. Sums are taken in a fixed order.
+    The backward computes the forward's states again; it needs about 244 KB of workspace for each 64
+    tokens of a value head while it runs, whatever dim_k and dim_v are: 1 GB for 8192 tokens of 32 heads. Sums are
+    taken in a fixed order.
     """
     return GatedDeltaRuleFn.apply(q, k, v, g, beta, initial_state, return_final_state, cu_seqlens, scale)
 

@@ -28,9 +28,9 @@ extern "C" {
  * and beta from its token on, to none before, and not to dv and dinitial_states; any other value that is
  * not finite may give NaN to all gradients of its sequence and head.
  * All sums and the state are fp32.  The tensor-core products split their fp32 factors into bf16
- * pieces: three (24 bits) of the state, of every factor of fp32 inputs and in the gradients of g
- * and beta; two (2^-17) of the chunk's U, P and of the correction (T - I) R where the result is
- * rounded to 16 bits or is a small part of its sum.
+ * pieces: three (24 bits) of the state, of every factor of fp32 inputs and in the backward; two
+ * (2^-17) of the chunk's U, P and of the correction (T - I) R in the forward of 16-bit types, whose
+ * output is rounded to 16 bits (its last state is then off by up to 2e-6, of fp32 inputs by 2e-7).
  *
  * Sequences: `batch` rows of `seqlen` tokens, or (cu_seqlens != NULL) batch == 1 and nseq packed
  * sequences, sequence s owning tokens [cu_seqlens[s], cu_seqlens[s+1]) of the seqlen tokens;
