@@ -75,3 +75,24 @@ def test_tokens_before_the_first_sequence(lens, heads):
             assert torch.equal(a[:, begin:end], b)
     packed = cc.gated_delta_rule_varlen_fn(*(t.detach()[0] for t in leaves), cu_seqlens=cu)
     assert torch.equal(packed, out[0])
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "g", "beta", "dout"])
+@pytest.mark.parametrize("along", [0, 1, 2])
+def test_expanded_tensors(which, along):
+    """Rows, tokens or heads that share memory (stride 0): read where they lie."""
+    import causal_conv1d_b200 as cc
+    names = ["q", "k", "v", "g", "beta"]
+    args = dict(zip(names, gdr_ref.inputs((2, 70), 2, 4, 64, 32, torch.bfloat16, seed=along)))
+    args["dout"] = torch.randn(2, 70, 4, 32, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    t = args[which]
+    shared = t.narrow(along, 0, 1).expand(t.shape)
+
+    def run(a):
+        leaves = [a[n].detach().requires_grad_() for n in names]
+        out = cc.gated_delta_rule_fn(*leaves)
+        steps = cc.gated_delta_rule_update(*(x.detach()[:, :5] for x in leaves), torch.zeros(2, 4, 64, 32, device="cuda"))
+        return (out, steps, *torch.autograd.grad(out, leaves, a["dout"]))
+
+    for a, b in zip(run({**args, which: shared}), run({**args, which: shared.clone(memory_format=torch.contiguous_format)})):
+        assert torch.equal(a, b)
