@@ -323,11 +323,18 @@ gdr_prep_kernel(const __grid_constant__ cc1d_gdr_params p, unsigned char *images
             }
             if (warp < 2) {
                 // an infinite or NaN entry would reach the rows before it through products with zeros: its row is noted
-                // (the walk cannot see finite keys whose product overflows), and the walk gives NaN to it and those behind
-                if (!all_finite(x)) {
-                    atomicMin(&gates.bad, i);
+                // (the walk cannot see finite keys whose product overflows), and the walk gives NaN to it and those behind.
+                // Where the gates between leave nothing (e^-110 is 0) there is no entry, whatever the product; the last of
+                // them is the one that they leave most of.
+                if (__builtin_expect(!all_finite(x), 0)) {
+                    uint32_t out = 0;
                     #pragma unroll
-                    for (int j = 0; j < 16; ++j) x[j] = finite(x[j]) ? x[j] : 0.f;
+                    for (int j = 0; j < 16; ++j) {
+                        const bool ok = finite(x[j]);
+                        out |= ok ? 0u : 1u << j;
+                        x[j] = ok ? x[j] : 0.f;
+                    }
+                    if (out != 0 && !(gi.x - gates.g[j0 + 31 - __clz(out)].x < -110.f)) atomicMin(&gates.bad, i);
                 }
                 #pragma unroll
                 for (int j = 0; j < 16; j += 4)

@@ -136,3 +136,17 @@ def test_a_gate_of_minus_infinity_in_the_backward():
     leaves[3][0, [0, 30, 64, 100], 1] = -torch.inf
     for a, b in zip(gradients(leaves, *rest), want):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_overflowing_products_of_forgotten_tokens(dtype):
+    """Two keys of 1e20, the state forgotten in front of both: their product overflows and means nothing."""
+    import causal_conv1d_b200 as cc
+    q, k, v, g, beta = gdr_ref.inputs((60,), 1, 2, 32, 32, DT[dtype], seed=16, slow=True)
+    for t in (5, 40):
+        k[t] *= 1e20
+        g[t] = -torch.inf
+    got = cc.gated_delta_rule_varlen_fn(q, k, v, g, beta, cu_seqlens=torch.tensor([0, 60], dtype=torch.int32).cuda(), scale=1.0)
+    want, _ = gdr_ref.rule(*(t.double().cpu() for t in (q, k, v, g, beta)), torch.zeros(2, 32, 32, dtype=torch.float64), 1.0)
+    for part in (slice(0, 5), slice(5, 40), slice(40, 60)):
+        gdr_ref.close(got[part], want[part], 4e-5, "out", DT[dtype])
