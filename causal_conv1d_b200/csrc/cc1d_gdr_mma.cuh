@@ -249,7 +249,7 @@ template <typename T, bool kBack> struct GdrStage {
     static constexpr uint32_t kKq = 0, kV = kPieces * kKqPiece, kT = kV + kChunk * kGdrMaxDim * sizeof(T), kGates = kT + kSolve * 8192,
                               kP = kGates + 4096, kBytes = kP + kOut * 8192, kImage = kBytes - kT;
 };
-constexpr uint32_t kGateBytes = 2688;            // of the 4096 in an image, which align P (the preparation has them in shared memory besides: 3072 would cost it a CTA an SM)
+constexpr uint32_t kGateBytes = 2688;            // of the 4096 in an image, which align P (the preparation has them in shared memory besides: another 400 bytes would cost it a CTA an SM)
 static_assert(sizeof(GdrGates) <= kGateBytes, "gates of a chunk");
 
 // Chunks of sequence n in the workspace: slots gdr_first_slot(n) .. ; the slots of different sequences
